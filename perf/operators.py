@@ -142,7 +142,7 @@ def prepare(case, seed):
             from coconet_amd import capi
             s["plan"] = capi.AdamWPlan(counts, decay=decay, bits=case["bits"])
             cut = lambda x: [x[o:o + c] for o, c in zip(starts, counts)]  # noqa: E731
-            s["tables"] = ([cut(g) for g in s["g"]], cut(s["w"]), None if s["w16"] is None else cut(s["w16"]))
+            s["tables"] = s["plan"].tables([cut(g) for g in s["g"]], cut(s["w"]), None if s["w16"] is None else cut(s["w16"]))
         return s
     t, M, K, N, pad = TYPES[case["type"]], case["M"], case["K"], case["N"], case["pad"]
     s["X"] = _rows(gen, M, K, pad, 1.0, t)
@@ -265,9 +265,9 @@ def _plain_backward(s):
 # ---- the library's calls ---------------------------------------------------------------------------------------------
 def _own_adamw(s):
     from coconet_amd import capi
-    g, w, w16 = s["tables"]
-    s["plan"].step(g, w, s["m"], s["v"], LR, BETA1, BETA2, EPS, WD, s["step"], scales=s.get("scales"), g_type=s["type"], w16=w16,
-                   w16_type=s["copy"] if w16 else None, inv_scale=s["inv_scale"], overflow_flag=s["flag"], stream=capi.current_stream())
+    s["plan"].step(s["tables"], s["m"], s["v"], LR, BETA1, BETA2, EPS, WD, s["step"], scales=s.get("scales"), g_type=s["type"],
+                   w16_type="bf16" if s["copy"] == "none" else s["copy"], inv_scale=s["inv_scale"], overflow_flag=s["flag"],
+                   stream=capi.current_stream())
 
 
 def _own_linear(s):
