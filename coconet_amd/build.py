@@ -14,7 +14,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libcoconet_hip.so")
-SOURCES = ["runtime.hip", "reduce_update.hip", "lamb.hip", "mlp_outproj.hip"]
+SOURCES = ["runtime.hip", "reduce_update.hip", "lamb.hip", "mlp_outproj.hip", "linear.hip", "adamw.hip"]
 
 # -ffp-contract=off: the kernels promise the rounding sequence of the reference checker loops.
 # -packed-fp32-ops off: packed fp32 instructions are not used on this hardware pool.

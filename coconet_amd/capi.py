@@ -37,6 +37,9 @@ SYMBOLS = [
     "ccn_mlp_outproj_bf16_ex", "ccn_bias_dropout_residual_ex", "ccn_matmul_bf16_f32",
     "ccn_mlp_outproj_f16_ex", "ccn_bias_dropout_residual_f16_ex", "ccn_matmul_f16_f32",
     "ccn_matmul_bf16", "ccn_matmul_f16",
+    "ccn_linear_plan_create", "ccn_linear_plan_destroy", "ccn_linear_bf16", "ccn_linear_f16",
+    "ccn_linear_backward_bf16", "ccn_linear_backward_f16",
+    "ccn_adamw_plan_create", "ccn_adamw_plan_destroy", "ccn_adamw_plan_sizes", "ccn_adamw_scattered",
 ]
 
 
@@ -61,7 +64,7 @@ def load():
     return _lib
 
 
-_vp, _i, _f, _sz, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
+_vp, _i, _f, _sz, _u64, _d = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64, C.c_double
 _pp = C.POINTER(C.c_void_p)
 
 
@@ -122,6 +125,16 @@ def _declare(L):
     sig("ccn_scatter_plan_destroy", [_vp])
     sig("ccn_sgd_f32_scattered", [_vp, _pp, _i, _pp, _f, _vp])
     sig("ccn_adam_f32_scattered", [_vp, _pp, _i, _pp, _vp, _vp, _f, _f, _f, _f, _i, _vp])
+    sig("ccn_linear_plan_create", [_i, _i, _i, _pp])
+    sig("ccn_linear_plan_destroy", [_vp])
+    for t in ("bf16", "f16"):
+        sig("ccn_linear_" + t, [_vp, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _i, _i, _i, _i, _vp])
+        sig("ccn_linear_backward_" + t, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _i, _vp, _i, _i, _i,
+                                         _i, _i, _vp])
+    sig("ccn_adamw_plan_create", [C.POINTER(_sz), C.POINTER(_f), _i, _i, _pp])
+    sig("ccn_adamw_plan_destroy", [_vp])
+    sig("ccn_adamw_plan_sizes", [_vp, C.POINTER(_sz), C.POINTER(_sz)])
+    sig("ccn_adamw_scattered", [_vp, _pp, _i, _i, _pp, _pp, _i, _vp, _vp, _vp, _d, _d, _d, _d, _d, _i, _d, _vp, _vp, _vp])
     sig("ccn_graph_begin", [_vp])
     sig("ccn_graph_end", [_vp, _pp])
     sig("ccn_graph_launch", [_vp, _vp])
@@ -486,3 +499,95 @@ def matmul_16(X, W, Cmat, M, N, K, stream=None, half=False):
         _check(load().ccn_matmul_f16(addr(X), addr(W), addr(Cmat), M, N, K, stream), "ccn_matmul_f16")
     else:
         _check(load().ccn_matmul_bf16(addr(X), addr(W), addr(Cmat), M, N, K, stream), "ccn_matmul_bf16")
+
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+TYPES = {"f32": 0, "bf16": 1, "f16": 2}
+
+
+class LinearPlan:
+    """Workspace of a dense layer's forward and backward calls of up to max_m x max_n x max_k (ccn_linear_plan)."""
+
+    def __init__(self, max_m, max_n, max_k):
+        h = C.c_void_p()
+        _check(load().ccn_linear_plan_create(max_m, max_n, max_k, C.byref(h)), "ccn_linear_plan_create")
+        self.h = h
+
+    def forward(self, X, W, bias, resid, Y, M, N, K, act="none", pre=None, half=False, ldx=0, ldw=0, ldr=0, ldy=0, ldp=0,
+                stream=None):
+        """Y = act(X.W + bias) + resid; pre receives X.W + bias.  bias, resid, pre: or None.  ld* 0: the rows lie end to end."""
+        L = load()
+        fn = L.ccn_linear_f16 if half else L.ccn_linear_bf16
+        rc = fn(self.h, addr(X), ldx or K, addr(W), ldw or N, addr(bias), addr(resid), ldr or N, addr(Y), ldy or N, addr(pre),
+                ldp or N, M, N, K, ACTS[act], stream)
+        if rc:
+            _check(rc, "ccn_linear_f16" if half else "ccn_linear_bf16")
+
+    def backward(self, dY, pre, X, W, dX, dW, db, M, N, K, act="none", half=False, dw_f32=False, accumulate=False, lddy=0, ldp=0,
+                 ldx=0, ldw=0, lddx=0, lddw=0, stream=None):
+        """The layer's gradients; any of dX, dW, db may be None.  dw_f32: dW is fp32; accumulate: dW and db are added to."""
+        L = load()
+        fn = L.ccn_linear_backward_f16 if half else L.ccn_linear_backward_bf16
+        rc = fn(self.h, addr(dY), lddy or N, addr(pre), ldp or N, addr(X), ldx or K, addr(W), ldw or N, addr(dX), lddx or K,
+                addr(dW), lddw or N, 0 if dw_f32 else (2 if half else 1), addr(db), 1 if accumulate else 0, M, N, K, ACTS[act],
+                stream)
+        if rc:
+            _check(rc, "ccn_linear_backward_f16" if half else "ccn_linear_backward_bf16")
+
+    def close(self):
+        if self.h:
+            _check(load().ccn_linear_plan_destroy(self.h), "ccn_linear_plan_destroy")
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class AdamWPlan:
+    """Tile table of one AdamW step over tensors of the given element counts (ccn_adamw_plan).
+
+    elems: elements (bits 32) or bytes (bits 8) of each moment array; blocks: half the length of the 8-bit moments' scales."""
+
+    def __init__(self, counts, decay=None, bits=32):
+        self.counts, self.bits = [int(c) for c in counts], bits
+        n = len(self.counts)
+        dec = None
+        if decay is not None:
+            assert len(decay) == n
+            dec = (_f * n)(*[float(x) for x in decay])
+        h = C.c_void_p()
+        _check(load().ccn_adamw_plan_create((_sz * n)(*self.counts), dec, n, bits, C.byref(h)), "ccn_adamw_plan_create")
+        self.h = h
+        e, b = _sz(0), _sz(0)
+        _check(load().ccn_adamw_plan_sizes(h, C.byref(e), C.byref(b)), "ccn_adamw_plan_sizes")
+        self.elems, self.blocks = e.value, b.value
+
+    def tables(self, g, w, w16=None):
+        """The host pointer tables of a step: g P lists of tensors, w and w16 (or None) one list each.  A program whose tensors
+        stay where they are makes them once; they hold addresses only, the tensors have to be kept alive beside them."""
+        n = len(self.counts)
+        assert len(w) == n and all(len(gp) == n for gp in g) and (w16 is None or len(w16) == n)
+        return ((C.c_void_p * (len(g) * n))(*[addr(x) for gp in g for x in gp]), len(g), (C.c_void_p * n)(*[addr(x) for x in w]),
+                None if w16 is None else (C.c_void_p * n)(*[addr(x) for x in w16]))
+
+    def step(self, tables, m, v, lr, beta1, beta2, eps, wd, step, scales=None, g_type="f32", w16_type="bf16", inv_scale=1.0,
+             grad_scale=None, overflow_flag=None, stream=None):
+        """One step.  tables: from tables().  grad_scale: device fp32 scalar; overflow_flag: device uint32 / int32 scalar."""
+        gt, ranks, wt, ht = tables
+        _check(load().ccn_adamw_scattered(self.h, gt, ranks, TYPES[g_type], wt, ht, TYPES[w16_type] if ht is not None else 0, addr(m), addr(v),
+                                          addr(scales), lr, beta1, beta2, eps, wd, step, inv_scale, addr(grad_scale),
+                                          addr(overflow_flag), stream), "ccn_adamw_scattered")
+
+    def close(self):
+        if self.h:
+            _check(load().ccn_adamw_plan_destroy(self.h), "ccn_adamw_plan_destroy")
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

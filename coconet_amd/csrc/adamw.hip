@@ -1,0 +1,490 @@
+// AdamW over many tensors at once, moments in fp32 or in 8 bits (gfx950).
+//
+//   g = sum_p g[p] * inv_scale * *grad_scale          m <- b1*m + (1-b1)*g          v <- b2*v + ((1-b2)*g)*g
+//   w <- w*(1 - lr*wd*decay_b) - lr * (m/(1-b1^t)) / (sqrt(v/(1-b2^t)) + eps)
+//
+// 8-bit moments: the moments of a tensor are cut into blocks of 256 elements.  A block holds m/sm and sqrt(v)/sr as OCP
+// e4m3 values (round to nearest even), sm = max|m|/448 and sr = max sqrt(v)/448 in fp32.  sqrt(v) and not v: the update
+// divides by sqrt(v), and e4m3's 2^18 between its smallest and largest value then span 2^36 of v.  A sqrt(v) that is
+// not zero is held as at least the smallest e4m3 value: rounded to zero it would leave eps alone under the next step's
+// first moment.  Everything between the load and the store of a moment is fp32.
+//
+// HBM-bound: a step cannot do without P*G + 8 bytes of gradients and weights per parameter plus 16 (fp32 moments) or
+// 4 + 16/256 (8-bit ones), plus 2 for a 16-bit copy of the weights.
+#include "ccn_common.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+namespace ccn {
+
+constexpr int kAwBlock = 256;          // elements of one scale
+constexpr int kAwLane = 8;             // elements of one lane: 16 bytes of a 16-bit gradient, 8 of an 8-bit moment
+constexpr int kAwTile = kWave * kAwLane;   // one wavefront's tile: two blocks
+constexpr int kAwGroupShift = 5;       // tiles per entry of the coarse table: 32
+constexpr float kE4m3Max = 448.0f, kE4m3Tiny = 0.001953125f;
+constexpr float kAwFlush = 7.888609052210118e-31f;   // 2^-100: a block whose largest |m| is below it is held as zeros
+
+struct AdamwBuf {
+  uint64_t count;         // elements of the tensor
+  uint64_t first_block;   // its first block
+  float decay;            // factor on the weight decay
+  uint32_t pad;
+};
+struct AdamwPrm {
+  float b1, omb1, b2, omb2, eps, lr, lr_wd, inv_bc1, inv_bc2, inv_scale;
+};
+struct AdamwArgs {
+  const uint32_t* coarse;        // buffer of the first tile of every group of 32 tiles
+  const uint32_t* first_tile;    // [nbuff + kWave] first tile of every buffer, then 0xffffffff
+  const AdamwBuf* bufs;
+  const void* const* table;      // [nbuff][CCN_MAX_RANKS + 2]: gradients, weights, 16-bit copy
+  void* m;
+  void* v;
+  float* scales;                 // [2][blocks]
+  const float* grad_scale;
+  uint32_t* flag;
+  uint64_t blocks;
+  uint32_t ntiles;
+  int P, w16_type;
+};
+constexpr int kAwSlots = CCN_MAX_RANKS + 2;
+
+enum { kGF32 = 0, kGBf16 = 1, kGF16 = 2 };
+template <int G> struct GradType { typedef uint16_t T; };
+template <> struct GradType<kGF32> { typedef float T; };
+template <int G> __device__ __forceinline__ float widen(typename GradType<G>::T x) {
+  if constexpr (G == kGF32) return x;
+  else return G == kGF16 ? f16_bits_to_f32(x) : bf16_bits_to_f32(x);
+}
+
+// Eight elements from `e` on: two or one wide loads where they are all there and aligned, single ones elsewhere (zeros
+// behind the end).
+template <typename T> __device__ __forceinline__ Pack<T, kAwLane> load8(const T* p, uint64_t e, uint64_t n, bool wide) {
+  if (wide) return load_stream<T, kAwLane>(p + e);
+  Pack<T, kAwLane> r;
+#pragma unroll
+  for (int j = 0; j < kAwLane; j++) r.d[j] = e + j < n ? p[e + j] : T(0);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, uint64_t e, uint64_t n, bool wide, const Pack<T, kAwLane>& x) {
+  if (wide) {
+    store_stream<T, kAwLane>(p + e, x);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kAwLane; j++)
+    if (e + j < n) p[e + j] = x.d[j];
+}
+
+// The largest of the 32 lanes of a half wavefront, in each of them.
+template <int CTRL> __device__ __forceinline__ float dpp_max(float x) {
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float half_wave_max(float x) {
+  x = dpp_max<0xB1>(x);    // quad_perm: neighbours
+  x = dpp_max<0x4E>(x);    // quad_perm: pairs
+  x = dpp_max<0x141>(x);   // row_half_mirror: quads
+  x = dpp_max<0x140>(x);   // row_mirror: halves of 16 lanes
+  return fmaxf(x, __shfl_xor(x, 16, kWave));
+}
+
+// Eight values of a block as e4m3 with the block's scale.
+__device__ __forceinline__ u32x2 to_e4m3(const float* x, float inv) {
+  float y[kAwLane];
+#pragma unroll
+  for (int j = 0; j < kAwLane; j++) y[j] = fminf(fmaxf(x[j] * inv, -kE4m3Max), kE4m3Max);
+  u32x2 r;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], c, true);
+    r[h] = (uint32_t)c;
+  }
+  return r;
+}
+__device__ __forceinline__ void from_e4m3(u32x2 c, float scale, float* x) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], true);
+    x[4 * h] = lo[0] * scale;
+    x[4 * h + 1] = lo[1] * scale;
+    x[4 * h + 2] = hi[0] * scale;
+    x[4 * h + 3] = hi[1] * scale;
+  }
+}
+
+// One wavefront, one tile of 512 elements of one tensor.  CAP: gradient buffers loaded (all up front; those from P on
+// are skipped under a uniform condition).
+template <int G, int CAP, int BITS>
+__global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const AdamwPrm k) {
+  typedef typename GradType<G>::T T;
+  const uint32_t tile = blockIdx.x + blockIdx.y * gridDim.x;
+  if (tile >= a.ntiles) return;
+  const int lane = threadIdx.x;
+  // the tensor of this tile: at most 32 tensors start inside a group of tiles, one per lane
+  const uint32_t b0 = a.coarse[tile >> kAwGroupShift];
+  const uint64_t before = __ballot(a.first_tile[b0 + lane] <= tile);
+  const uint32_t b = b0 + (uint32_t)__popcll(before) - 1u;
+  const AdamwBuf buf = a.bufs[b];
+  const void* const* const row = a.table + (size_t)b * kAwSlots;
+  const uint32_t t = tile - a.first_tile[b];
+  const uint64_t e = (uint64_t)t * kAwTile + (uint64_t)lane * kAwLane;   // first element inside the tensor
+  const uint64_t n = buf.count;
+  float* const w = static_cast<float*>(const_cast<void*>(row[CCN_MAX_RANKS]));
+  uint16_t* const w16 = static_cast<uint16_t*>(const_cast<void*>(row[CCN_MAX_RANKS + 1]));
+  uintptr_t low = reinterpret_cast<uintptr_t>(w) | (a.w16_type ? reinterpret_cast<uintptr_t>(w16) : 0);
+#pragma unroll
+  for (int p = 0; p < CAP; p++)
+    if (p < a.P) low |= reinterpret_cast<uintptr_t>(row[p]);
+  const bool wide = (low & 15u) == 0 && e + kAwLane <= n;
+  const uint64_t blk = buf.first_block + 2ull * t + (lane >> 5);
+  const bool inside = e < ((n + kAwBlock - 1) & ~(uint64_t)(kAwBlock - 1));   // the second block may not exist
+  const uint64_t se = blk * kAwBlock + (uint64_t)(lane & 31) * kAwLane;       // this lane's place in the moment arrays
+
+  Pack<T, kAwLane> gp[CAP];
+#pragma unroll
+  for (int p = 0; p < CAP; p++)
+    if (p < a.P) gp[p] = load8(static_cast<const T*>(row[p]), e, n, wide);
+  Pack<float, kAwLane> wp = load8(w, e, n, wide), mp, vp;
+  u32x2 mc = {0u, 0u}, vc = {0u, 0u};
+  float sm = 0.0f, sr = 0.0f;
+  if (inside) {
+    if constexpr (BITS == 32) {
+      mp = load_stream<float, kAwLane>(static_cast<const float*>(a.m) + se);
+      vp = load_stream<float, kAwLane>(static_cast<const float*>(a.v) + se);
+    } else {
+      mc = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.m) + se));
+      vc = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.v) + se));
+      sm = a.scales[blk];
+      sr = a.scales[a.blocks + blk];
+    }
+  }
+  const float gs = a.grad_scale ? k.inv_scale * *a.grad_scale : k.inv_scale;
+  if constexpr (BITS == 8) {
+    from_e4m3(mc, sm, mp.d);
+    from_e4m3(vc, sr, vp.d);
+  }
+  float root[kAwLane];
+  bool any_bad = false;
+  const float keep = 1.0f - k.lr_wd * buf.decay;
+#pragma unroll
+  for (int j = 0; j < kAwLane; j++) {
+    float g = widen<G>(gp[0].d[j]);
+#pragma unroll
+    for (int p = 1; p < CAP; p++)
+      if (p < a.P) g = g + widen<G>(gp[p].d[j]);
+    g = g * gs;
+    const float m0 = mp.d[j], v0 = BITS == 8 ? vp.d[j] * vp.d[j] : vp.d[j];
+    const float m1 = k.b1 * m0 + k.omb1 * g;
+    const float v1 = k.b2 * v0 + k.omb2 * g * g;
+    // a gradient that is not finite, or whose square is not: the element keeps its weight and moments
+    const bool bad = !(fabsf(m1) < __builtin_inff()) || !(v1 < __builtin_inff());
+    any_bad = any_bad || (bad && e + j < n);
+    const float update = (m1 * k.inv_bc1) / (sqrtf(v1 * k.inv_bc2) + k.eps);
+    const float w1 = wp.d[j] * keep - k.lr * update;
+    if (!bad) wp.d[j] = w1;
+    mp.d[j] = bad ? m0 : m1;
+    if constexpr (BITS == 8) root[j] = bad ? vp.d[j] : sqrtf(v1);
+    else vp.d[j] = bad ? v0 : v1;
+  }
+  store8(w, e, n, wide, wp);
+  if (a.w16_type) {
+    Pack<uint16_t, kAwLane> h;
+#pragma unroll
+    for (int j = 0; j < kAwLane; j++) h.d[j] = a.w16_type == CCN_TYPE_F16 ? f32_to_f16_bits(wp.d[j]) : f32_to_bf16_bits(wp.d[j]);
+    store8(w16, e, n, wide, h);
+  }
+  if constexpr (BITS == 32) {
+    if (inside) {
+      store_stream<float, kAwLane>(static_cast<float*>(a.m) + se, mp);
+      store_stream<float, kAwLane>(static_cast<float*>(a.v) + se, vp);
+    }
+  } else {
+    if (!wide) {   // what lies behind a tensor's end must not weigh on its last block's scale
+#pragma unroll
+      for (int j = 0; j < kAwLane; j++)
+        if (e + j >= n) mp.d[j] = root[j] = 0.0f;
+    }
+    float mm = 0.0f, rm = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kAwLane; j++) {
+      mm = fmaxf(mm, fabsf(mp.d[j]));
+      rm = fmaxf(rm, root[j]);
+    }
+    mm = half_wave_max(mm);
+    rm = half_wave_max(rm);
+    const float sm1 = mm < kAwFlush ? 0.0f : mm / kE4m3Max, sr1 = rm / kE4m3Max;
+    const float im = sm1 > 0.0f ? 1.0f / sm1 : 0.0f, ir = sr1 > 0.0f ? 1.0f / sr1 : 0.0f;
+    const u32x2 c = to_e4m3(mp.d, im);
+    float y[kAwLane];
+#pragma unroll
+    for (int j = 0; j < kAwLane; j++) y[j] = root[j] > 0.0f ? fmaxf(root[j] * ir, kE4m3Tiny) : 0.0f;
+    const u32x2 d = to_e4m3(y, 1.0f);
+    if (inside) {
+      __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.m) + se));
+      __builtin_nontemporal_store(d, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.v) + se));
+      if ((lane & 31) == 0) {
+        a.scales[blk] = sm1;
+        a.scales[a.blocks + blk] = sr1;
+      }
+    }
+  }
+  if (a.flag && __ballot(any_bad) != 0 && lane == 0) __hip_atomic_store(a.flag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ void adamw_clear_flag(uint32_t* flag) { *flag = 0u; }
+
+}  // namespace ccn
+
+using namespace ccn;
+
+struct ccn_adamw_plan {
+  int device = -1;
+  int nbuff = 0, bits = 32;
+  std::vector<int> live;               // the tensors that have elements
+  uint64_t blocks = 0;
+  uint32_t ntiles = 0;
+  uint32_t* coarse = nullptr;
+  uint32_t* first_tile = nullptr;
+  AdamwBuf* bufs = nullptr;
+  const void** table_dev = nullptr;    // [live][kAwSlots]
+  const void** table_pinned = nullptr;
+  bool recorded = false;               // a step on this plan has been recorded
+  hipEvent_t copied = nullptr;         // the last copy out of table_pinned
+  std::vector<const void*> shadow;     // what the device table holds
+};
+
+namespace {
+
+// Brings the device pointer table in line with the caller's pointers.  The copy is queued on the caller's stream; the
+// host waits only for an earlier copy that is still reading the staging buffer.
+int adamw_sync_table(ccn_adamw_plan* p, const void* const* g, int P, float* const* w, uint16_t* const* w16, hipStream_t s) {
+  const size_t nl = p->live.size();
+  bool same = true;
+  for (size_t i = 0; i < nl; i++) {
+    const size_t b = (size_t)p->live[i];
+    const void** const row = p->shadow.data() + i * kAwSlots;
+    for (int r = 0; r < P; r++) same = same && row[r] == g[(size_t)r * p->nbuff + b];
+    same = same && row[CCN_MAX_RANKS] == w[b] && (!w16 || row[CCN_MAX_RANKS + 1] == w16[b]);
+  }
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  CCN_HIP(hipStreamIsCapturing(s, &st));
+  const bool recording = st != hipStreamCaptureStatusNone;
+  if (same) {
+    p->recorded = p->recorded || recording;
+    return CCN_OK;
+  }
+  // a recorded copy would read the staging buffer at replay; and a recorded step reads the table at replay, so that the
+  // pointers of a plan with one are not changed any more
+  if (recording || p->recorded) return CCN_EINVAL;
+  CCN_HIP(hipEventSynchronize(p->copied));
+  // the device table is in an unknown state until the copy below is queued: forget what it held
+  std::vector<const void*> next(p->shadow);
+  std::fill(p->shadow.begin(), p->shadow.end(), nullptr);
+  for (size_t i = 0; i < nl; i++) {
+    const size_t b = (size_t)p->live[i];
+    const void** const row = next.data() + i * kAwSlots;
+    for (int r = 0; r < P; r++) row[r] = g[(size_t)r * p->nbuff + b];
+    row[CCN_MAX_RANKS] = w[b];
+    if (w16) row[CCN_MAX_RANKS + 1] = w16[b];
+  }
+  std::memcpy(p->table_pinned, next.data(), next.size() * sizeof(void*));
+  CCN_HIP(hipMemcpyAsync(p->table_dev, p->table_pinned, next.size() * sizeof(void*), hipMemcpyHostToDevice, s));
+  CCN_HIP(hipEventRecord(p->copied, s));
+  p->shadow.swap(next);
+  return CCN_OK;
+}
+
+template <int G, int CAP>
+int adamw_launch(const ccn_adamw_plan* p, const AdamwArgs& a, const AdamwPrm& k, hipStream_t s) {
+  const uint32_t gx = a.ntiles < 0x40000000u ? a.ntiles : 0x40000000u;
+  const dim3 grid(gx, (a.ntiles + gx - 1) / gx);
+  if (p->bits == 8) hipLaunchKernelGGL((adamw_kernel<G, CAP, 8>), grid, dim3(kWave), 0, s, a, k);
+  else hipLaunchKernelGGL((adamw_kernel<G, CAP, 32>), grid, dim3(kWave), 0, s, a, k);
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
+}
+template <int G>
+int adamw_launch_p(const ccn_adamw_plan* p, const AdamwArgs& a, const AdamwPrm& k, hipStream_t s) {
+  if (a.P == 1) return adamw_launch<G, 1>(p, a, k, s);
+  if (a.P == 2) return adamw_launch<G, 2>(p, a, k, s);
+  if (a.P <= 4) return adamw_launch<G, 4>(p, a, k, s);
+  if (a.P <= 8) return adamw_launch<G, 8>(p, a, k, s);
+  return adamw_launch<G, CCN_MAX_RANKS>(p, a, k, s);
+}
+
+int adamw_step(ccn_adamw_plan* p, const void* const* g, int P, int g_type, float* const* w, uint16_t* const* w16, int w16_type,
+               void* m, void* v, float* scales, double lr, double beta1, double beta2, double eps, double wd, int step,
+               double inv_scale, const float* grad_scale, uint32_t* flag, void* stream) {
+  if (!p || !g || !w || P < 1 || P > CCN_MAX_RANKS || step < 1) return CCN_EINVAL;
+  if (g_type != CCN_TYPE_F32 && g_type != CCN_TYPE_BF16 && g_type != CCN_TYPE_F16) return CCN_EINVAL;
+  if (w16 && w16_type != CCN_TYPE_BF16 && w16_type != CCN_TYPE_F16) return CCN_EINVAL;
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return CCN_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(grad_scale) | reinterpret_cast<uintptr_t>(flag)) & 3u) return CCN_EINVAL;
+  const uintptr_t gmask = g_type == CCN_TYPE_F32 ? 3u : 1u;
+  for (const int b : p->live) {
+    for (int r = 0; r < P; r++) {
+      const void* const x = g[(size_t)r * p->nbuff + b];
+      if (!x || (reinterpret_cast<uintptr_t>(x) & gmask)) return CCN_EINVAL;
+    }
+    if (!w[b] || (reinterpret_cast<uintptr_t>(w[b]) & 3u)) return CCN_EINVAL;
+    if (w16 && (!w16[b] || (reinterpret_cast<uintptr_t>(w16[b]) & 1u))) return CCN_EINVAL;
+  }
+  if (p->ntiles) {
+    if (!m || !v || !aligned16(m) || !aligned16(v)) return CCN_EINVAL;
+    if (p->bits == 8 ? (!scales || (reinterpret_cast<uintptr_t>(scales) & 3u)) : scales != nullptr) return CCN_EINVAL;
+  }
+  const DeviceInfo* di = nullptr;
+  int rc = current_device_info(&di);
+  if (rc != CCN_OK) return rc;
+  if (di->device != p->device) return CCN_EINVAL;
+  hipStream_t s = as_stream(stream);
+  if (p->ntiles) {
+    rc = adamw_sync_table(p, g, P, w, w16, s);
+    if (rc != CCN_OK) return rc;
+  }
+  if (flag) {
+    hipLaunchKernelGGL(adamw_clear_flag, dim3(1), dim3(1), 0, s, flag);
+    CCN_HIP(hipGetLastError());
+  }
+  if (!p->ntiles) return CCN_OK;
+  AdamwPrm k;
+  k.b1 = (float)beta1;
+  k.omb1 = (float)(1.0 - beta1);
+  k.b2 = (float)beta2;
+  k.omb2 = (float)(1.0 - beta2);
+  k.eps = (float)eps;
+  k.lr = (float)lr;
+  k.lr_wd = (float)(lr * wd);
+  k.inv_bc1 = (float)(1.0 / (1.0 - std::pow(beta1, (double)step)));
+  k.inv_bc2 = (float)(1.0 / (1.0 - std::pow(beta2, (double)step)));
+  k.inv_scale = (float)inv_scale;
+  AdamwArgs a;
+  a.coarse = p->coarse;
+  a.first_tile = p->first_tile;
+  a.bufs = p->bufs;
+  a.table = p->table_dev;
+  a.m = m;
+  a.v = v;
+  a.scales = scales;
+  a.grad_scale = grad_scale;
+  a.flag = flag;
+  a.blocks = p->blocks;
+  a.ntiles = p->ntiles;
+  a.P = P;
+  a.w16_type = w16 ? w16_type : 0;
+  switch (g_type) {
+    case CCN_TYPE_F32: return adamw_launch_p<kGF32>(p, a, k, s);
+    case CCN_TYPE_BF16: return adamw_launch_p<kGBf16>(p, a, k, s);
+    default: return adamw_launch_p<kGF16>(p, a, k, s);
+  }
+}
+
+int adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int bits, ccn_adamw_plan** out);
+
+}  // namespace
+
+extern "C" {
+
+int ccn_adamw_plan_destroy(ccn_adamw_plan* p) {
+  if (!p) return CCN_OK;
+  int rc = CCN_OK;
+  if (p->copied && hipEventSynchronize(p->copied) != hipSuccess) rc = CCN_EHIP;
+  if (p->copied && hipEventDestroy(p->copied) != hipSuccess) rc = CCN_EHIP;
+  if (p->coarse && hipFree(p->coarse) != hipSuccess) rc = CCN_EHIP;
+  if (p->first_tile && hipFree(p->first_tile) != hipSuccess) rc = CCN_EHIP;
+  if (p->bufs && hipFree(p->bufs) != hipSuccess) rc = CCN_EHIP;
+  if (p->table_dev && hipFree(p->table_dev) != hipSuccess) rc = CCN_EHIP;
+  if (p->table_pinned && hipHostFree(p->table_pinned) != hipSuccess) rc = CCN_EHIP;
+  delete p;
+  return rc;
+}
+
+int ccn_adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int bits, ccn_adamw_plan** out) {
+  if (!out) return CCN_EINVAL;
+  *out = nullptr;
+  if (!counts || nbuff < 1 || (bits != 8 && bits != 32)) return CCN_EINVAL;
+  return guarded([&] { return adamw_plan_create(counts, decay, nbuff, bits, out); });
+}
+
+int ccn_adamw_plan_sizes(const ccn_adamw_plan* plan, size_t* elems, size_t* blocks) {
+  if (!plan) return CCN_EINVAL;
+  if (elems) *elems = (size_t)plan->blocks * kAwBlock;
+  if (blocks) *blocks = (size_t)plan->blocks;
+  return CCN_OK;
+}
+
+int ccn_adamw_scattered(ccn_adamw_plan* plan, const void* const* g, int P, int g_type, float* const* w, uint16_t* const* w16,
+                        int w16_type, void* m, void* v, float* scales, double lr, double beta1, double beta2, double eps,
+                        double wd, int step, double inv_scale, const float* grad_scale, uint32_t* overflow_flag, void* stream) {
+  return guarded([&] {
+    return adamw_step(plan, g, P, g_type, w, w16, w16_type, m, v, scales, lr, beta1, beta2, eps, wd, step, inv_scale, grad_scale,
+                      overflow_flag, stream);
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+int adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int bits, ccn_adamw_plan** out) {
+  std::vector<AdamwBuf> bufs;
+  std::vector<uint32_t> first, coarse;
+  std::vector<int> live;
+  uint64_t blocks = 0, ntiles = 0;
+  for (int b = 0; b < nbuff; b++) {
+    if (counts[b] == 0) continue;
+    if (counts[b] > ((size_t)1 << 48)) return CCN_ERANGE;
+    const uint64_t nb = ((uint64_t)counts[b] + kAwBlock - 1) / kAwBlock, nt = (nb + 1) / 2;
+    if (ntiles + nt >= 0xffffffffull) return CCN_ERANGE;   // tile numbers are 32-bit
+    const uint32_t i = (uint32_t)bufs.size();
+    bufs.push_back(AdamwBuf{(uint64_t)counts[b], blocks, decay ? decay[b] : 1.0f, 0u});
+    first.push_back((uint32_t)ntiles);
+    live.push_back(b);
+    for (uint64_t grp = (ntiles + (1u << kAwGroupShift) - 1) >> kAwGroupShift; (grp << kAwGroupShift) < ntiles + nt; grp++) coarse.push_back(i);
+    blocks += nb;
+    ntiles += nt;
+  }
+  const DeviceInfo* di = nullptr;
+  const int rc = current_device_info(&di);
+  if (rc != CCN_OK) return rc;
+  ccn_adamw_plan* const p = new ccn_adamw_plan();
+  p->device = di->device;
+  p->nbuff = nbuff;
+  p->bits = bits;
+  p->blocks = blocks;
+  p->ntiles = (uint32_t)ntiles;
+  hipError_t e = hipSuccess;
+  try {
+    p->live.swap(live);
+    first.insert(first.end(), kWave, 0xffffffffu);   // a wavefront looks at 64 tensors from the group's first one on
+    const size_t words = p->live.size() * (size_t)kAwSlots;
+    p->shadow.assign(words, nullptr);
+    if (ntiles) {
+      e = hipMalloc((void**)&p->coarse, coarse.size() * sizeof(uint32_t));
+      if (e == hipSuccess) e = hipMalloc((void**)&p->first_tile, first.size() * sizeof(uint32_t));
+      if (e == hipSuccess) e = hipMalloc((void**)&p->bufs, bufs.size() * sizeof(AdamwBuf));
+      if (e == hipSuccess) e = hipMalloc((void**)&p->table_dev, words * sizeof(void*));
+      if (e == hipSuccess) e = hipHostMalloc((void**)&p->table_pinned, words * sizeof(void*), hipHostMallocDefault);
+      if (e == hipSuccess) e = hipEventCreateWithFlags(&p->copied, hipEventDisableTiming);
+      if (e == hipSuccess) e = hipMemcpy(p->coarse, coarse.data(), coarse.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
+      if (e == hipSuccess) e = hipMemcpy(p->first_tile, first.data(), first.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
+      if (e == hipSuccess) e = hipMemcpy(p->bufs, bufs.data(), bufs.size() * sizeof(AdamwBuf), hipMemcpyHostToDevice);
+    }
+  } catch (...) {
+    ccn_adamw_plan_destroy(p);
+    throw;
+  }
+  if (e != hipSuccess) {
+    ccn_adamw_plan_destroy(p);
+    return hip_fail(e);
+  }
+  *out = p;
+  return CCN_OK;
+}
+
+}  // namespace

@@ -1,0 +1,683 @@
+// A dense layer with its epilogue fused into the product, and its gradients (gfx950).
+//
+//   forward    z = X.W + bias, Y = act(z) + resid, pre = z          X [M x K], W [K x N], row-major
+//   backward   dz = dY * act'(pre), dX = dz.W^T, dW (+)= X^T.dz, db (+)= column sums of dz
+//
+// All three products are C[rows x cols] = sum over c of P(row, c) * Q(c, col) with operands that lie in memory either with
+// the summed index contiguous ("along": X and dz in forward and dX, W in dX) or with the outer index contiguous
+// ("across": W in forward, X and dz in dW).  Both kinds are fetched as they lie, in 16-byte pieces, and both become the
+// same matrix-core fragments (8 consecutive c of one row or column per lane): an "along" tile is read from LDS by plain
+// 16-byte reads, an "across" tile through the transposing ds_read_b64_tr_b16.
+#include "ccn_common.hpp"
+
+#include <new>
+#include <type_traits>
+
+namespace ccn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+template <bool F16> __device__ __forceinline__ float half_in(uint16_t h) { return F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h); }
+template <bool F16> __device__ __forceinline__ uint16_t half_out(float f) { return F16 ? f32_to_f16_bits(f) : f32_to_bf16_bits(f); }
+
+// ---- activations, in fp32 ----------------------------------------------------------------------------------------------
+// A quarter-rate exp2 and reciprocal (1 ulp each) and a handful of multiply-adds per element: at one wavefront per SIMD the
+// library's erff / tanhf / expf and the IEEE division cost more than the tile's stores.  Absolute errors stay below 3e-7
+// of the argument, a fraction of the half step of a 16-bit output.
+// Far out the limits hold exactly (0 on the left, z and slope 1 on the right, also at infinity); a NaN stays one.
+constexpr float kLog2e = 1.44269504088896341f, kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
+constexpr float kTanhC = 0.79788456080286536f, kTanhA = 0.044715f;   // sqrt(2/pi)
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+// Phi(z) = erfc(-z/sqrt 2)/2 by formula 7.1.26 of Abramowitz and Stegun (|error of erf| <= 1.5e-7); *bell: exp(-z^2/2).
+__device__ __forceinline__ float normal_cdf(float z, float* bell) {
+  const float x = fabsf(z) * kSqrtHalf, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+  *bell = __builtin_amdgcn_exp2f(-kLog2e * x * x);
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * p * t * *bell;   // Phi(-|z|)
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+__device__ __forceinline__ float gelu_tanh_gate(float z) {   // (1 + tanh u)/2 = sigmoid(2u)
+  return sigmoid(2.0f * kTanhC * z * fmaf(kTanhA * z, z, 1.0f));
+}
+// The gate times z; a z so far left that the gate is 0 is cut off, -inf * 0 would be NaN.
+__device__ __forceinline__ float act_value(int act, float z) {
+  float bell;
+  switch (act) {
+    case CCN_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case CCN_ACT_GELU: return fmaxf(z, -104.0f) * normal_cdf(z, &bell);
+    case CCN_ACT_GELU_TANH: return fmaxf(z, -104.0f) * gelu_tanh_gate(z);
+    case CCN_ACT_SILU: return fmaxf(z, -104.0f) * sigmoid(z);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(int act, float z0) {
+  const float z = fminf(fmaxf(z0, -104.0f), 104.0f);   // the slopes are 0 and 1 from there on
+  float r;
+  switch (act) {
+    case CCN_ACT_RELU: r = z > 0.0f ? 1.0f : 0.0f; break;
+    case CCN_ACT_GELU: {
+      float bell;
+      const float p = normal_cdf(z, &bell);
+      r = fmaf(z * kInvSqrt2Pi, bell, p);
+      break;
+    }
+    case CCN_ACT_GELU_TANH: {
+      const float s = gelu_tanh_gate(z);
+      r = fmaf(z * s * (1.0f - s) * (2.0f * kTanhC), fmaf(3.0f * kTanhA * z, z, 1.0f), s);
+      break;
+    }
+    case CCN_ACT_SILU: {
+      const float s = sigmoid(z);
+      r = s * fmaf(z, 1.0f - s, 1.0f);
+      break;
+    }
+    default: r = 1.0f;
+  }
+  return z0 != z0 ? z0 : r;
+}
+
+// ---- eight neighbouring elements of a row --------------------------------------------------------------------------------
+// gfx950 loads and stores 16 bytes at any 2-byte aligned address; `n` is how many of the eight are there (behind a row's
+// end they are neither read nor written).
+__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, int n) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+      if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+  }
+  return v;
+}
+__device__ __forceinline__ void store_piece(uint16_t* p, const u32x4 v, int n) {
+  if (n >= 8) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+      if (e < n) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+  }
+}
+template <bool F16> __device__ __forceinline__ void unpack(const u32x4 v, float* x) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) x[e] = half_in<F16>((uint16_t)(v[e >> 1] >> (16 * (e & 1))));
+}
+template <bool F16> __device__ __forceinline__ u32x4 pack(const float* x) {
+  u32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = (uint32_t)half_out<F16>(x[2 * e]) | ((uint32_t)half_out<F16>(x[2 * e + 1]) << 16);
+  return v;
+}
+
+struct LinEpi {
+  const float* bias;
+  const uint16_t* resid;
+  uint16_t* pre;
+  void* out;
+  size_t ldr, ldp, ldo;
+  int act;
+  int accumulate;   // fp32 output only
+};
+
+// Finishes elements (row, col .. col+7) of the output, n of them inside the row.  OUT32: an fp32 output, stored or added
+// to; else the forward epilogue (of which a plain 16-bit product is the case with nothing to do).
+template <bool F16, bool OUT32>
+__device__ __forceinline__ void finish8(float* v, const LinEpi& ep, size_t row, size_t col, int n) {
+  if constexpr (OUT32) {
+    float* const o = static_cast<float*>(ep.out) + row * ep.ldo + col;
+    if (n >= 8) {
+      if (ep.accumulate) {
+        float old[8];
+        __builtin_memcpy(old, o, 32);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += old[e];
+      }
+      __builtin_memcpy(o, v, 32);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; e++)
+        if (e < n) o[e] = ep.accumulate ? o[e] + v[e] : v[e];
+    }
+  } else {
+    if (ep.bias) {
+      float b[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      if (n >= 8) {
+        __builtin_memcpy(b, ep.bias + col, 32);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+          if (e < n) b[e] = ep.bias[col + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += b[e];
+    }
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if (ep.resid) r = load_piece(ep.resid + row * ep.ldr + col, n);
+    if (ep.pre) store_piece(ep.pre + row * ep.ldp + col, pack<F16>(v), n);
+    if (ep.act != CCN_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = act_value(ep.act, v[e]);
+    }
+    if (ep.resid) {
+      float x[8];
+      unpack<F16>(r, x);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += x[e];
+    }
+    store_piece(static_cast<uint16_t*>(ep.out) + row * ep.ldo + col, pack<F16>(v), n);
+  }
+}
+
+// Which tile a workgroup takes.  Workgroup b runs on XCD b % 8: every XCD gets a contiguous range of tile numbers, and
+// tiles are numbered down four tile rows before the next tile column, so the workgroups an XCD runs at a time form a block
+// whose operand panels are shared in its L2.
+__device__ __forceinline__ void tile_of(uint32_t b, int tiles_r, int tiles_c, int& tr, int& tc) {
+  const uint32_t total = (uint32_t)tiles_r * (uint32_t)tiles_c, x = b & 7u, q = total >> 3, rest = total & 7u;
+  const uint32_t id = x * q + (x < rest ? x : rest) + (b >> 3);
+  const uint32_t band = 4u * (uint32_t)tiles_c, g = id / band, in = id - g * band;
+  const uint32_t first = 4u * g, left = (uint32_t)tiles_r - first, h = left < 4u ? left : 4u;
+  tr = (int)(first + in % h);
+  tc = (int)(in / h);
+}
+
+struct LinProd {
+  const uint16_t* p;   // row operand
+  const uint16_t* q;   // column operand
+  size_t ldp, ldq;
+  int rows, cols, sum;
+  int tiles_r, tiles_c;
+  int per_split;       // summed elements per split (a multiple of kGK)
+  float* partial;      // [splits][rows][cols rounded up to 8] when splits > 1
+};
+
+// ---- any shape, any alignment -----------------------------------------------------------------------------------------
+// 128 x 128 tiles, 64 summed elements per step, four wavefronts of 64 x 64 (2 x 2 blocks of v_mfma_f32_32x32x16).  The
+// pieces of step k+1 travel from memory to registers while step k is multiplied from LDS.  Tiles at the edge read the
+// last row again instead of one behind it (its results are not stored); pieces that cross the end of a row, and steps
+// that cross the end of the sum, are filled with zeros, on both operands (0 * inf would not be 0).
+constexpr int kGT = 128, kGK = 64;
+constexpr int kGTile = kGT * kGK * 2;      // bytes of one operand's step
+constexpr int kGCStride = 64 + 4;          // floats per row of a wavefront's 32 x 64 piece of the output
+constexpr int kGLds = (2 * kGTile > 4 * 32 * kGCStride * 4) ? 2 * kGTile : 4 * 32 * kGCStride * 4;
+
+enum { kOut16 = 0, kOut32 = 1, kOutPartial = 2 };
+
+template <bool ALONG> struct GSide {
+  // thread t stages pieces j = 0..3: along: row t/8 + 32j, piece t%8 of the step;  across: step row t/16 + 16j, piece t%16
+  const uint16_t* base[4];
+  int edge;   // across: valid elements of this thread's piece
+  __device__ __forceinline__ void init(const uint16_t* p, size_t ld, int o0, int outer, int t) {
+    if constexpr (ALONG) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int r = o0 + (t >> 3) + 32 * j;
+        base[j] = p + (size_t)(r < outer ? r : outer - 1) * ld + 8 * (t & 7);
+      }
+      edge = 8;
+    } else {
+      const int c = o0 + 8 * (t & 15);
+#pragma unroll
+      for (int j = 0; j < 4; j++) base[j] = p + (size_t)((t >> 4) + 16 * j) * ld + c;
+      edge = outer - c;
+    }
+  }
+  __device__ __forceinline__ void fetch(u32x4* v, size_t ld, int k, int sum, int t, bool whole) const {
+    const size_t off = ALONG ? (size_t)k : (size_t)k * ld;
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) __builtin_memcpy(&v[j], base[j] + off, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int n = ALONG ? sum - k - 8 * (t & 7) : (k + (t >> 4) + 16 * j < sum ? edge : 0);
+        v[j] = load_piece(base[j] + off, n);
+      }
+    }
+  }
+  static __device__ __forceinline__ int swz(int row) { return (row & 7) ^ ((row >> 3) & 7); }
+  static __device__ __forceinline__ void put(uint8_t* lds, const u32x4* v, int t) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (ALONG) {
+        const int row = (t >> 3) + 32 * j;
+        *reinterpret_cast<u32x4*>(lds + row * 128 + (((t & 7) ^ swz(row)) << 4)) = v[j];
+      } else {
+        const int k = (t >> 4) + 16 * j;
+        *reinterpret_cast<u32x4*>(lds + k * 256 + (((t & 15) ^ (4 * (k & 3))) << 4)) = v[j];
+      }
+    }
+  }
+  // fragment f (32 rows or columns), summed elements 16*ks + 8*(lane/32) .. +7 of row or column 32*f + lane%32
+  static __device__ __forceinline__ s16x8 frag(const uint8_t* lds, int f, int ks, int lane) {
+    const int li = lane & 31, lh = lane >> 5;
+    if constexpr (ALONG) {
+      const int row = 32 * f + li;
+      return *reinterpret_cast<const s16x8*>(lds + row * 128 + (((2 * ks + lh) ^ swz(row)) << 4));
+    } else {
+      const int a16 = lane & 15, g2 = (lane >> 4) & 1;
+      const int at = ((lh * 8 + (a16 >> 2)) * 16 + ((2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2)))) * 16 + 8 * (a16 & 1);
+      const uint8_t* p = lds + (at ^ (f * 64)) + ks * 4096;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 1024));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16, bool PA, bool QA, int OUT>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 4)))
+void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kGLds];
+  uint8_t* const lp = lds;
+  uint8_t* const lq = lds + kGTile;
+  int tr, tc;
+  tile_of(blockIdx.x, pr.tiles_r, pr.tiles_c, tr, tc);
+  const int r0 = tr * kGT, c0 = tc * kGT;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wr = wave >> 1, wc = wave & 1, li = lane & 31, lh = lane >> 5;
+  const int k_begin = (int)blockIdx.y * pr.per_split;
+  const int k_end = pr.sum - k_begin < pr.per_split ? pr.sum : k_begin + pr.per_split;
+  const bool pin = PA || r0 + kGT <= pr.rows, qin = QA || c0 + kGT <= pr.cols;
+
+  GSide<PA> sp;
+  GSide<QA> sq;
+  sp.init(pr.p, pr.ldp, r0, pr.rows, t);
+  sq.init(pr.q, pr.ldq, c0, pr.cols, t);
+  f32x16 acc[2][2];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
+#pragma unroll
+  for (int a = 0; a < 2; a++)
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[a][b][i] = 0.0f;
+
+  u32x4 vp[4], vq[4];
+  auto fetch = [&](int k) {
+    const bool whole = k + kGK <= k_end;
+    sp.fetch(vp, pr.ldp, k, k_end, t, whole && pin);
+    sq.fetch(vq, pr.ldq, k, k_end, t, whole && qin);
+  };
+  if (k_begin < k_end) fetch(k_begin);
+  for (int k = k_begin; k < k_end; k += kGK) {
+    __syncthreads();   // everybody has read the step before
+    GSide<PA>::put(lp, vp, t);
+    GSide<QA>::put(lq, vq, t);
+    if (k + kGK < k_end) fetch(k + kGK);
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) {
+      s16x8 fp[2], fq[2];
+#pragma unroll
+      for (int f = 0; f < 2; f++) {
+        fq[f] = GSide<QA>::frag(lq, 2 * wc + f, ks, lane);
+        fp[f] = GSide<PA>::frag(lp, 2 * wr + f, ks, lane);
+      }
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) acc[a][b] = mfma32<F16>(fq[a], fp[b], acc[a][b]);
+    }
+  }
+  __syncthreads();   // LDS becomes four private pieces of the output
+  float* const cw = reinterpret_cast<float*>(lds) + wave * (32 * kGCStride);
+  const int r8 = lane >> 3, c8 = lane & 7;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 v = {acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
+        *reinterpret_cast<f32x4*>(cw + li * kGCStride + 32 * a + 8 * i + 4 * lh) = v;
+      }
+    __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const int row = r0 + 64 * wr + 32 * b + 8 * s + r8, col = c0 + 64 * wc + 8 * c8;
+      float v[8];
+      __builtin_memcpy(v, cw + (8 * s + r8) * kGCStride + 8 * c8, 32);
+      if (row < pr.rows && col < pr.cols) {
+        if constexpr (OUT == kOutPartial) {
+          const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
+          float* const o = pr.partial + ((size_t)blockIdx.y * pr.rows + row) * ld + col;
+          __builtin_memcpy(o, v, 32);
+        } else {
+          finish8<F16, OUT == kOut32>(v, ep, (size_t)row, (size_t)col, pr.cols - col);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Adds the splits up in ascending order and finishes the output: eight columns of a row per thread.
+template <bool F16, bool OUT32>
+__global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __restrict__ partial, const int splits, const int rows,
+                                                             const int cols, const LinEpi ep) {
+  const size_t ld = ((size_t)cols + 7) & ~(size_t)7, pieces = ld / 8;
+  const size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= pieces * (size_t)rows) return;
+  const size_t row = i / pieces, col = (i - row * pieces) * 8;
+  const float* p = partial + row * ld + col;
+  float v[8];
+  __builtin_memcpy(v, p, 32);
+  for (int s = 1; s < splits; s++) {
+    p += (size_t)rows * ld;
+    float x[8];
+    __builtin_memcpy(x, p, 32);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += x[e];
+  }
+  finish8<F16, OUT32>(v, ep, row, col, cols - (int)col);
+}
+
+// ---- dz and the column sums ------------------------------------------------------------------------------------------------
+// dz = dY * act'(pre), rounded to the operands' type into the workspace (rows of N rounded up to 8, zeros in the rest),
+// and fp32 sums over a chunk of rows of the unrounded dz.  Four wavefronts walk a chunk's rows, 512 columns wide.
+template <bool F16>
+__global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __restrict__ dY, const size_t lddy,
+                                                           const uint16_t* __restrict__ pre, const size_t ldp,
+                                                           uint16_t* __restrict__ dz, const size_t lddz, float* __restrict__ sums,
+                                                           const int M, const int N, const int act, const int rows_per_chunk) {
+  __shared__ float part[4][512 + 8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = (int)blockIdx.x * 512 + lane * 8, n = N - col;
+  const int m0 = (int)blockIdx.y * rows_per_chunk;
+  const int m1 = M - m0 < rows_per_chunk ? M : m0 + rows_per_chunk;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) s[e] = 0.0f;
+  if (n > 0) {
+    for (int m = m0 + wave; m < m1; m += 4) {
+      float g[8];
+      unpack<F16>(load_piece(dY + (size_t)m * lddy + col, n), g);
+      if (act != CCN_ACT_NONE) {
+        float z[8];
+        unpack<F16>(load_piece(pre + (size_t)m * ldp + col, n), z);
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[e] = e < n ? g[e] * act_slope(act, z[e]) : 0.0f;
+        if (dz) {
+          const u32x4 v = pack<F16>(g);
+          __builtin_memcpy(dz + (size_t)m * lddz + col, &v, 16);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[e] += g[e];
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int e = 0; e < 8; e++) part[wave][lane * 8 + e] = s[e];
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int c = threadIdx.x + 256 * h, at = (int)blockIdx.x * 512 + c;
+    if (at < N) sums[(size_t)blockIdx.y * N + at] = ((part[0][c] + part[1][c]) + part[2][c]) + part[3][c];
+  }
+}
+// db[n] = (db[n] +) the sum of the chunks' sums: 64 columns per workgroup, each wavefront a quarter of the chunks.
+__global__ __launch_bounds__(kBlock) void linear_db_kernel(const float* __restrict__ sums, float* __restrict__ db, const int N,
+                                                           const int chunks, const int accumulate) {
+  __shared__ float part[4][kWave];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * kWave + lane;
+  float s = 0.0f;
+  if (c < N)
+    for (int k = wave; k < chunks; k += 4) s += sums[(size_t)k * N + c];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < N) {
+    const float x = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+    db[c] = accumulate ? db[c] + x : x;
+  }
+}
+
+constexpr size_t kMaxLd = (size_t)1 << 22;
+constexpr int kMaxChunks = 256;      // row chunks of the column sums
+constexpr size_t kMaxSplitTiles = 1024;   // tiles x splits of a split product, which bounds the partial sums' workspace
+
+inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+}  // namespace ccn
+
+using namespace ccn;
+
+struct ccn_linear_plan {
+  int device = -1;
+  int max_m = 0, max_n = 0, max_k = 0;
+  uint16_t* dz = nullptr;
+  float* sums = nullptr;
+  float* partial = nullptr;
+  size_t partial_floats = 0;
+};
+
+namespace {
+
+// How often a product is split along its sum: few tiles leave CUs idle; a split has at least two steps.
+int splits_for(int tiles, int sum, int cus) {
+  if (tiles >= cus || sum < 4 * kGK) return 1;
+  int s = (2 * cus) / tiles;
+  const int most = sum / (2 * kGK);
+  if (s > most) s = most;
+  if ((size_t)s * (size_t)tiles > kMaxSplitTiles) s = (int)(kMaxSplitTiles / (size_t)tiles);
+  return s < 1 ? 1 : s;
+}
+
+template <bool F16, bool PA, bool QA>
+int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum,
+            const LinEpi& ep, bool out32, int cus, hipStream_t s) {
+  LinProd pr;
+  pr.p = p;
+  pr.q = q;
+  pr.ldp = ldp;
+  pr.ldq = ldq;
+  pr.rows = rows;
+  pr.cols = cols;
+  pr.sum = sum;
+  pr.tiles_r = (rows + kGT - 1) / kGT;
+  pr.tiles_c = (cols + kGT - 1) / kGT;
+  pr.partial = plan->partial;
+  if ((size_t)pr.tiles_r * (size_t)pr.tiles_c > 0x7fffffffull) return CCN_ERANGE;
+  const int tiles = pr.tiles_r * pr.tiles_c;
+  int splits = splits_for(tiles, sum, cus);
+  const size_t each = (size_t)rows * (((size_t)cols + 7) & ~(size_t)7);
+  if ((size_t)splits * each > plan->partial_floats) splits = (int)(plan->partial_floats / each);
+  if (splits < 2) splits = 1;
+  const int steps = (sum + kGK - 1) / kGK;
+  pr.per_split = ((steps + splits - 1) / splits) * kGK;
+  if (splits > 1) splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
+  if (pr.per_split < kGK) pr.per_split = kGK;
+  const dim3 grid((unsigned)tiles, (unsigned)splits), block(kBlock);
+  if (splits > 1) {
+    hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOutPartial>), grid, block, 0, s, pr, ep);
+    CCN_HIP(hipGetLastError());
+    const size_t threads = (each / 8);
+    const dim3 jg((unsigned)((threads + kBlock - 1) / kBlock));
+    if (out32) hipLaunchKernelGGL((linear_join_kernel<F16, true>), jg, block, 0, s, pr.partial, splits, rows, cols, ep);
+    else hipLaunchKernelGGL((linear_join_kernel<F16, false>), jg, block, 0, s, pr.partial, splits, rows, cols, ep);
+  } else if (out32) {
+    if constexpr (!PA && !QA) hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut32>), grid, block, 0, s, pr, ep);
+    else return CCN_EINVAL;
+  } else {
+    hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut16>), grid, block, 0, s, pr, ep);
+  }
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
+}
+
+int check_plan(const ccn_linear_plan* plan, int M, int N, int K, int act, const DeviceInfo** di) {
+  if (!plan || M < 0 || N < 1 || K < 1 || act < CCN_ACT_NONE || act > CCN_ACT_SILU) return CCN_EINVAL;
+  if (M > plan->max_m || N > plan->max_n || K > plan->max_k) return CCN_ERANGE;
+  const int rc = current_device_info(di);
+  if (rc != CCN_OK) return rc;
+  return (*di)->device == plan->device ? CCN_OK : CCN_EINVAL;
+}
+// A 16-bit matrix argument: 0, or why it is refused.
+int check16(const void* p, size_t ld, int cols) {
+  if (!p || !aligned2(p) || ld < (size_t)cols) return CCN_EINVAL;
+  return ld > kMaxLd ? CCN_ERANGE : CCN_OK;
+}
+#define CCN_TRY(expr)                  \
+  do {                                 \
+    const int _rc = (expr);            \
+    if (_rc != CCN_OK) return _rc;     \
+  } while (0)
+
+template <bool F16>
+int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
+                   const uint16_t* resid, size_t ldr, uint16_t* Y, size_t ldy, uint16_t* pre, size_t ldp, int M, int N, int K,
+                   int act, void* stream) {
+  const DeviceInfo* di = nullptr;
+  CCN_TRY(check_plan(plan, M, N, K, act, &di));
+  if (M == 0) return CCN_OK;
+  CCN_TRY(check16(X, ldx, K));
+  CCN_TRY(check16(W, ldw, N));
+  CCN_TRY(check16(Y, ldy, N));
+  if (resid) CCN_TRY(check16(resid, ldr, N));
+  if (pre) CCN_TRY(check16(pre, ldp, N));
+  if (!aligned4(bias)) return CCN_EINVAL;
+  const LinEpi ep{bias, resid, pre, Y, ldr, ldp, ldy, act, 0};
+  return product<F16, true, false>(plan, X, ldx, W, ldw, M, N, K, ep, false, di->cu_count, as_stream(stream));
+}
+
+template <bool F16>
+int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, const uint16_t* pre, size_t ldp, const uint16_t* X,
+                    size_t ldx, const uint16_t* W, size_t ldw, uint16_t* dX, size_t lddx, void* dW, size_t lddw, int dw_type,
+                    float* db, int accumulate, int M, int N, int K, int act, void* stream) {
+  const DeviceInfo* di = nullptr;
+  CCN_TRY(check_plan(plan, M, N, K, act, &di));
+  const bool dw32 = dw_type == CCN_TYPE_F32;
+  if (!dw32 && dw_type != (F16 ? CCN_TYPE_F16 : CCN_TYPE_BF16)) return CCN_EINVAL;
+  if (accumulate && dW && !dw32) return CCN_EINVAL;
+  if (dW && (lddw < (size_t)N || !(dw32 ? aligned4(dW) : aligned2(dW)))) return CCN_EINVAL;
+  if (dW && lddw > kMaxLd) return CCN_ERANGE;
+  if (!aligned4(db)) return CCN_EINVAL;
+  if (M > 0) {
+    CCN_TRY(check16(dY, lddy, N));
+    if (act != CCN_ACT_NONE) CCN_TRY(check16(pre, ldp, N));
+    if (dX) {
+      CCN_TRY(check16(dX, lddx, K));
+      CCN_TRY(check16(W, ldw, N));
+    }
+    if (dW) CCN_TRY(check16(X, ldx, K));
+  }
+  hipStream_t s = as_stream(stream);
+  const bool want_dz = act != CCN_ACT_NONE && (dX || dW);
+  const size_t lddz = ((size_t)plan->max_n + 7) & ~(size_t)7;
+  int chunks = 0;
+  if (M > 0 && (want_dz || db)) {
+    const int strips = (N + 511) / 512;
+    // rows per chunk: enough workgroups for the whole chip, at least four rows for each wavefront
+    int per = (int)(((size_t)M * strips + 4 * (size_t)di->cu_count - 1) / (4 * (size_t)di->cu_count));
+    if (per < 16) per = 16;
+    if ((M + per - 1) / per > kMaxChunks) per = (M + kMaxChunks - 1) / kMaxChunks;
+    chunks = (M + per - 1) / per;
+    hipLaunchKernelGGL((linear_dz_kernel<F16>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp,
+                       want_dz ? plan->dz : nullptr, lddz, db ? plan->sums : nullptr, M, N, act, per);
+    CCN_HIP(hipGetLastError());
+  }
+  if (db) {
+    hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kBlock), 0, s, plan->sums, db, N, chunks, accumulate);
+    CCN_HIP(hipGetLastError());
+  }
+  const uint16_t* const g = act != CCN_ACT_NONE ? plan->dz : dY;
+  const size_t ldg = act != CCN_ACT_NONE ? lddz : lddy;
+  if (dX && M > 0) {
+    const LinEpi ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
+    CCN_TRY((product<F16, true, true>(plan, g, ldg, W, ldw, M, K, N, ep, false, di->cu_count, s)));
+  }
+  if (dW) {
+    const LinEpi ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
+    CCN_TRY((product<F16, false, false>(plan, X, ldx, g, ldg, K, N, M, ep, dw32, di->cu_count, s)));
+  }
+  return CCN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ccn_linear_plan_destroy(ccn_linear_plan* plan) {
+  if (!plan) return CCN_OK;
+  int rc = CCN_OK;
+  if (plan->dz && hipFree(plan->dz) != hipSuccess) rc = CCN_EHIP;
+  if (plan->sums && hipFree(plan->sums) != hipSuccess) rc = CCN_EHIP;
+  if (plan->partial && hipFree(plan->partial) != hipSuccess) rc = CCN_EHIP;
+  delete plan;
+  return rc;
+}
+
+int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** out) {
+  if (!out) return CCN_EINVAL;
+  *out = nullptr;
+  if (max_M < 1 || max_N < 1 || max_K < 1) return CCN_EINVAL;
+  if ((size_t)max_N > kMaxLd || (size_t)max_K > kMaxLd) return CCN_ERANGE;
+  const DeviceInfo* di = nullptr;
+  CCN_TRY(current_device_info(&di));
+  ccn_linear_plan* const p = new (std::nothrow) ccn_linear_plan();
+  if (!p) return CCN_ENOMEM;
+  p->device = di->device;
+  p->max_m = max_M;
+  p->max_n = max_N;
+  p->max_k = max_K;
+  // a split product has at most kMaxSplitTiles tiles x splits, and a split at least two steps
+  auto floats = [](int rows, int cols, int sum) {
+    const size_t tiles = (size_t)((rows + kGT - 1) / kGT) * (size_t)((cols + kGT - 1) / kGT);
+    const size_t most = tiles * (size_t)(sum / (2 * kGK) + 1);
+    return (most < kMaxSplitTiles ? most : kMaxSplitTiles) * (size_t)(kGT * kGT);
+  };
+  const size_t need[3] = {floats(max_M, max_N, max_K), floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
+  for (const size_t f : need) p->partial_floats = f > p->partial_floats ? f : p->partial_floats;
+  const size_t lddz = ((size_t)max_N + 7) & ~(size_t)7;
+  hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * lddz * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
+  if (e != hipSuccess) {
+    ccn_linear_plan_destroy(p);
+    return hip_fail(e);
+  }
+  *out = p;
+  return CCN_OK;
+}
+
+int ccn_linear_bf16(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
+                    const uint16_t* resid, size_t ldr, uint16_t* Y, size_t ldy, uint16_t* pre, size_t ldp, int M, int N, int K,
+                    int act, void* stream) {
+  return linear_forward<false>(plan, X, ldx, W, ldw, bias, resid, ldr, Y, ldy, pre, ldp, M, N, K, act, stream);
+}
+
+int ccn_linear_f16(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
+                   const uint16_t* resid, size_t ldr, uint16_t* Y, size_t ldy, uint16_t* pre, size_t ldp, int M, int N, int K,
+                   int act, void* stream) {
+  return linear_forward<true>(plan, X, ldx, W, ldw, bias, resid, ldr, Y, ldy, pre, ldp, M, N, K, act, stream);
+}
+
+int ccn_linear_backward_bf16(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, const uint16_t* pre, size_t ldp,
+                             const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, uint16_t* dX, size_t lddx, void* dW,
+                             size_t lddw, int dw_type, float* db, int accumulate, int M, int N, int K, int act, void* stream) {
+  return linear_backward<false>(plan, dY, lddy, pre, ldp, X, ldx, W, ldw, dX, lddx, dW, lddw, dw_type, db, accumulate, M, N, K, act, stream);
+}
+
+int ccn_linear_backward_f16(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, const uint16_t* pre, size_t ldp,
+                            const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, uint16_t* dX, size_t lddx, void* dW,
+                            size_t lddw, int dw_type, float* db, int accumulate, int M, int N, int K, int act, void* stream) {
+  return linear_backward<true>(plan, dY, lddy, pre, ldp, X, ldx, W, ldw, dX, lddx, dW, lddw, dw_type, db, accumulate, M, N, K, act, stream);
+}
+
+}  // extern "C"

@@ -300,6 +300,88 @@ int  ccn_matmul_f16_f32(const uint16_t* X, const uint16_t* W, float* C, int M, i
 int  ccn_matmul_bf16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, int N, int K, void* stream);
 int  ccn_matmul_f16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, int N, int K, void* stream);
 
+/* ---- element types of the calls below that take several ---- */
+#define CCN_TYPE_F32  0
+#define CCN_TYPE_BF16 1
+#define CCN_TYPE_F16  2
+
+/* ---- a dense layer with its epilogue fused into the product, and its gradients (no counterpart in the reference, whose
+ *      MatMul stage has no activation and no backward pass; they stand beside ccn_mlp_outproj_* and ccn_matmul_*).
+ *
+ *      forward    z = X[MxK].W[KxN] + bias        Y = act(z) + resid        pre = z (kept for the backward pass)
+ *      backward   dz = dY * act'(pre)             dX = dz.W^T    dW = X^T.dz    db[n] = sum_m dz[m][n]
+ *
+ *      X, W, resid, Y, pre, dY, dX: bf16 (_bf16) or IEEE-half (_f16) bit patterns, row-major; ld*: elements from one row to
+ *      the next (at least the row's length).  bias, db: fp32.  dW: the operands' type, or fp32 (dw_type CCN_TYPE_F32).
+ *      Any M >= 0, N >= 1, K >= 1, any alignment that the element type allows (fp32 arrays 4 bytes, 16-bit ones 2): whole
+ *      rows of 16-byte pieces on the fast kernels, everything else on the same matrix cores at a lower rate.  M = 0 (an
+ *      empty batch): forward writes nothing; backward writes zero gradients, or leaves them when accumulating.
+ *      Products are accumulated in fp32 on the matrix cores, Y is computed from the fp32 z, every output is rounded to
+ *      nearest even once.  dz is rounded to the operands' type before the two products when there is an activation (the
+ *      matrix cores take 16-bit operands); db is summed in fp32 from the unrounded dz.  Sums run in a fixed order: the
+ *      same call gives the same bits.
+ *      act: CCN_ACT_*; GELU is z*Phi(z), GELU_TANH its tanh form, SILU z*sigmoid(z); the slope of RELU at 0 is 0.
+ *      bias, resid, pre may be NULL (not wanted); so may any of dX, dW, db.  backward needs pre unless act is NONE (it is
+ *      then ignored and dz is dY itself); it needs W for dX and X for dW.  accumulate != 0: db, and dW, which must be fp32
+ *      then, are added to.  resid's gradient is dY.
+ *      Y may be resid itself (same address and ld); otherwise outputs must not overlap inputs or each other.
+ *      Rows and columns outside the matrices (the padding of a row) are neither read for the result nor written.
+ *
+ *      A plan owns the workspace (dz, partial sums) for calls of up to max_M x max_N x max_K; one plan serves any number of
+ *      layers of up to that size.  Calls on one plan must be ordered (one stream, or events), also calls replayed from
+ *      recordings.  Every call on a plan can be recorded.  CCN_ERANGE: a size beyond the plan's, or rows too long for
+ *      32-bit addressing inside a tile (ld > 2^22). ---- */
+#define CCN_ACT_NONE      0
+#define CCN_ACT_RELU      1
+#define CCN_ACT_GELU      2
+#define CCN_ACT_GELU_TANH 3
+#define CCN_ACT_SILU      4
+typedef struct ccn_linear_plan ccn_linear_plan;
+int  ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** plan);
+int  ccn_linear_plan_destroy(ccn_linear_plan* plan);
+int  ccn_linear_bf16(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
+                     const uint16_t* resid, size_t ldr, uint16_t* Y, size_t ldy, uint16_t* pre, size_t ldp, int M, int N, int K,
+                     int act, void* stream);
+int  ccn_linear_f16(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
+                    const uint16_t* resid, size_t ldr, uint16_t* Y, size_t ldy, uint16_t* pre, size_t ldp, int M, int N, int K,
+                    int act, void* stream);
+int  ccn_linear_backward_bf16(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, const uint16_t* pre, size_t ldp,
+                              const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, uint16_t* dX, size_t lddx, void* dW,
+                              size_t lddw, int dw_type, float* db, int accumulate, int M, int N, int K, int act, void* stream);
+int  ccn_linear_backward_f16(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, const uint16_t* pre, size_t ldp,
+                             const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, uint16_t* dX, size_t lddx, void* dW,
+                             size_t lddw, int dw_type, float* db, int accumulate, int M, int N, int K, int act, void* stream);
+
+/* ---- AdamW over many tensors at once, moments in fp32 or in 8 bits (no counterpart in the reference; stands beside
+ *      ccn_adam_f32_scattered, which has no decoupled decay, takes fp32 gradients only and keeps fp32 moments).
+ *        g = (sum_p g[p]) * inv_scale * *grad_scale       (the P rank buffers in ascending order, in fp32)
+ *        m <- beta1*m + (1-beta1)*g;   v <- beta2*v + (1-beta2)*g*g
+ *        w <- w*(1 - lr*wd*decay_b) - lr * (m/(1-beta1^step)) / (sqrt(v/(1-beta2^step)) + eps)
+ *      A plan describes nbuff tensors of counts[b] elements (0 allowed), decay[b] the factor on the weight decay of tensor b
+ *      (NULL: 1 for all; 0 is the usual choice for biases and norms), bits = 32 or 8 the width of the moments.
+ *      g: HOST array of P*nbuff device pointers, rank-major, of g_type (CCN_TYPE_*); w: HOST array of nbuff device pointers
+ *      (fp32, updated); w16: HOST array of nbuff device pointers that receive the new weights in w16_type (CCN_TYPE_BF16 or
+ *      _F16), or NULL.  Pointers of tensors of 0 elements are not looked at.  The tensors must not overlap.
+ *      The moments are single arrays, 16-byte aligned, over all tensors: each tensor takes a whole number of blocks of 256
+ *      elements, in order (ccn_adamw_plan_sizes gives elements and blocks).  bits 32: m, v fp32, scales NULL.  bits 8: m, v
+ *      one byte per element, scales an fp32 array of 2*blocks: element i of block b stands for m = e4m3(m[i])*scales[b] and
+ *      sqrt(v) = e4m3(v[i])*scales[blocks + b], with OCP e4m3 codes.  The step computes in fp32 and rounds m and sqrt(v)
+ *      to nearest even with the scale max/448 of their block; a sqrt(v) that is not zero is held as at least the smallest
+ *      code; a block whose largest |m| is below 2^-100 is held as zeros.  All-zero arrays are the state to start from.
+ *      Elements behind a tensor's end are not part of the state; an 8-bit step writes zeros there.
+ *      grad_scale: DEVICE fp32 scalar (a clipping factor, a loss scale's inverse), or NULL for 1.
+ *      overflow_flag (DEVICE uint32, or NULL): set by the call, 1 if the gradient of any element, or its square, is not
+ *      finite in fp32, else 0.  Such an element keeps its w, m, v (8-bit ones rounded again with the block's new scale).
+ *      The device's pointer table is refreshed on the call's stream when pointers change; such a call cannot be recorded, and
+ *      once a call on the plan has been recorded its pointers stay (CCN_EINVAL for others).  `step` is evaluated on the host, as for Adam.  Calls on one plan must be ordered. ---- */
+typedef struct ccn_adamw_plan ccn_adamw_plan;
+int  ccn_adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int bits, ccn_adamw_plan** plan);
+int  ccn_adamw_plan_destroy(ccn_adamw_plan* plan);
+int  ccn_adamw_plan_sizes(const ccn_adamw_plan* plan, size_t* elems, size_t* blocks);
+int  ccn_adamw_scattered(ccn_adamw_plan* plan, const void* const* g, int P, int g_type, float* const* w, uint16_t* const* w16,
+                         int w16_type, void* m, void* v, float* scales, double lr, double beta1, double beta2, double eps, double wd,
+                         int step, double inv_scale, const float* grad_scale, uint32_t* overflow_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
