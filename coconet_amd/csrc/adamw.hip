@@ -10,7 +10,12 @@
 // first moment.  Everything between the load and the store of a moment is fp32.
 //
 // HBM-bound: a step cannot do without P*G + 8 bytes of gradients and weights per parameter plus 16 (fp32 moments) or
-// 4 + 16/256 (8-bit ones), plus 2 for a 16-bit copy of the weights.
+// 4 + 16/256 (8-bit ones), plus 2 for a 16-bit copy of the weights.  One wavefront works on one block, four neighbouring
+// elements per lane, so that every access of a wavefront is one contiguous piece of 256 bytes to 1 KiB (eight elements per
+// lane, whose fp32 pieces leave every other 16 bytes to the next instruction: 5.2 TB/s instead of 6.5 with fp32 moments),
+// and the block's largest values are found by lane exchanges alone.  Two or four blocks per wavefront are slower (2^27
+// elements, bf16 gradients and copy: 8-bit moments 346 / 354 / 365 us, fp32 ones 580 / 599 / 624).  With 8-bit moments the
+// arithmetic is worth the memory's time: with IEEE divisions and square roots the same kernel took 428 us.
 #include "ccn_common.hpp"
 
 #include <algorithm>
@@ -22,24 +27,23 @@
 namespace ccn {
 
 constexpr int kAwBlock = 256;          // elements of one scale
-constexpr int kAwLane = 8;             // elements of one lane: 16 bytes of a 16-bit gradient, 8 of an 8-bit moment
-constexpr int kAwTile = kWave * kAwLane;   // one wavefront's tile: two blocks
-constexpr int kAwGroupShift = 5;       // tiles per entry of the coarse table: 32
+constexpr int kAwLane = kAwBlock / kWave;   // 4 elements of a block per lane: every access of a wavefront is one contiguous piece
+constexpr int kAwGroupShift = 5;       // blocks per entry of the coarse table: 32
 constexpr float kE4m3Max = 448.0f, kE4m3Tiny = 0.001953125f;
 constexpr float kAwFlush = 7.888609052210118e-31f;   // 2^-100: a block whose largest |m| is below it is held as zeros
 
 struct AdamwBuf {
   uint64_t count;         // elements of the tensor
-  uint64_t first_block;   // its first block
+  uint32_t first_block;   // its first block
   float decay;            // factor on the weight decay
-  uint32_t pad;
 };
 struct AdamwPrm {
-  float b1, omb1, b2, omb2, eps, lr, lr_wd, inv_bc1, inv_bc2, inv_scale;
+  float b1, omb1, b2, omb2, eps, lr_wd, inv_scale;
+  float rate, root_bc2;   // lr / (1-b1^t), 1 / sqrt(1-b2^t)
 };
 struct AdamwArgs {
-  const uint32_t* coarse;        // buffer of the first tile of every group of 32 tiles
-  const uint32_t* first_tile;    // [nbuff + kWave] first tile of every buffer, then 0xffffffff
+  const uint32_t* coarse;        // tensor of the first block of every group of 32 blocks
+  const uint32_t* first_block;   // [nbuff + kWave] first block of every tensor, then 0xffffffff
   const AdamwBuf* bufs;
   const void* const* table;      // [nbuff][CCN_MAX_RANKS + 2]: gradients, weights, 16-bit copy
   void* m;
@@ -47,8 +51,7 @@ struct AdamwArgs {
   float* scales;                 // [2][blocks]
   const float* grad_scale;
   uint32_t* flag;
-  uint64_t blocks;
-  uint32_t ntiles;
+  uint32_t blocks;
   int P, w16_type;
 };
 constexpr int kAwSlots = CCN_MAX_RANKS + 2;
@@ -61,16 +64,16 @@ template <int G> __device__ __forceinline__ float widen(typename GradType<G>::T 
   else return G == kGF16 ? f16_bits_to_f32(x) : bf16_bits_to_f32(x);
 }
 
-// Eight elements from `e` on: two or one wide loads where they are all there and aligned, single ones elsewhere (zeros
-// behind the end).
-template <typename T> __device__ __forceinline__ Pack<T, kAwLane> load8(const T* p, uint64_t e, uint64_t n, bool wide) {
+// Four elements from `e` on: one wide load where they are all there and aligned, single ones elsewhere (zeros behind the
+// end).
+template <typename T> __device__ __forceinline__ Pack<T, kAwLane> load4(const T* p, uint64_t e, uint64_t n, bool wide) {
   if (wide) return load_stream<T, kAwLane>(p + e);
   Pack<T, kAwLane> r;
 #pragma unroll
   for (int j = 0; j < kAwLane; j++) r.d[j] = e + j < n ? p[e + j] : T(0);
   return r;
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, uint64_t e, uint64_t n, bool wide, const Pack<T, kAwLane>& x) {
+template <typename T> __device__ __forceinline__ void store4(T* p, uint64_t e, uint64_t n, bool wide, const Pack<T, kAwLane>& x) {
   if (wide) {
     store_stream<T, kAwLane>(p + e, x);
     return;
@@ -80,59 +83,69 @@ template <typename T> __device__ __forceinline__ void store8(T* p, uint64_t e, u
     if (e + j < n) p[e + j] = x.d[j];
 }
 
-// The largest of the 32 lanes of a half wavefront, in each of them.
-template <int CTRL> __device__ __forceinline__ float dpp_max(float x) {
-  return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true)));
+// The largest of a wavefront's values, none of which is negative: their bit patterns compare as integers.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
+  return x > y ? x : y;
 }
-__device__ __forceinline__ float half_wave_max(float x) {
+__device__ __forceinline__ float wave_max(float f) {
+  uint32_t x = __float_as_uint(f);
   x = dpp_max<0xB1>(x);    // quad_perm: neighbours
   x = dpp_max<0x4E>(x);    // quad_perm: pairs
   x = dpp_max<0x141>(x);   // row_half_mirror: quads
   x = dpp_max<0x140>(x);   // row_mirror: halves of 16 lanes
-  return fmaxf(x, __shfl_xor(x, 16, kWave));
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)x, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)x, 16);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)x, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)x, 48);
+  const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
+  return __uint_as_float(ab > cd ? ab : cd);
+}
+// The correctly rounded square root from the 1-ulp one by a Newton step on the residual (its result before the last
+// rounding is within 2^-46 of the root).  Below 2^-96 the argument is scaled: the instruction flushes denormals.
+__device__ __forceinline__ float square_root(float x) {
+  const bool small = x < 1.262177448353619e-29f;
+  const float z = x * (small ? 18446744073709551616.0f : 1.0f);
+  const float s = __builtin_amdgcn_sqrtf(z), h = 0.5f * __builtin_amdgcn_rcpf(s);
+  const float r = fmaf(fmaf(-s, s, z), h, s) * (small ? 2.3283064365386963e-10f : 1.0f);
+  return x > 0.0f ? r : 0.0f;
 }
 
-// Eight values of a block as e4m3 with the block's scale.
-__device__ __forceinline__ u32x2 to_e4m3(const float* x, float inv) {
-  float y[kAwLane];
-#pragma unroll
-  for (int j = 0; j < kAwLane; j++) y[j] = fminf(fmaxf(x[j] * inv, -kE4m3Max), kE4m3Max);
-  u32x2 r;
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
-    c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], c, true);
-    r[h] = (uint32_t)c;
-  }
-  return r;
+// 1/s, and x / s (inv: 1/s), correctly rounded by a Newton step each.  A code then depends on the values alone and not on
+// how a quotient next to a rounding border came about; the IEEE division sequence is three times as long.
+__device__ __forceinline__ float inverse(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return fmaf(fmaf(-s, r, 1.0f), r, r);
 }
-__device__ __forceinline__ void from_e4m3(u32x2 c, float scale, float* x) {
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], true);
-    x[4 * h] = lo[0] * scale;
-    x[4 * h + 1] = lo[1] * scale;
-    x[4 * h + 2] = hi[0] * scale;
-    x[4 * h + 3] = hi[1] * scale;
-  }
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  const float q = x * inv;
+  return fmaf(fmaf(-q, s, x), inv, q);
+}
+// Four values in units of the block's scale as e4m3.
+__device__ __forceinline__ uint32_t to_e4m3(const float* x) {
+  const int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], c, true);
+}
+__device__ __forceinline__ void from_e4m3(uint32_t c, float scale, float* x) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  x[0] = lo[0] * scale;
+  x[1] = lo[1] * scale;
+  x[2] = hi[0] * scale;
+  x[3] = hi[1] * scale;
 }
 
-// One wavefront, one tile of 512 elements of one tensor.  CAP: gradient buffers loaded (all up front; those from P on
-// are skipped under a uniform condition).
+// One wavefront, one block.  CAP: gradient buffers loaded, all up front (those from P on are skipped under a uniform
+// condition).
 template <int G, int CAP, int BITS>
 __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const AdamwPrm k) {
   typedef typename GradType<G>::T T;
-  const uint32_t tile = blockIdx.x + blockIdx.y * gridDim.x;
-  if (tile >= a.ntiles) return;
+  const uint32_t blk = blockIdx.x + blockIdx.y * gridDim.x;
+  if (blk >= a.blocks) return;
   const int lane = threadIdx.x;
-  // the tensor of this tile: at most 32 tensors start inside a group of tiles, one per lane
-  const uint32_t b0 = a.coarse[tile >> kAwGroupShift];
-  const uint64_t before = __ballot(a.first_tile[b0 + lane] <= tile);
+  // the tensor of this block: at most 32 tensors start inside a group of blocks, one per lane
+  const uint32_t b0 = a.coarse[blk >> kAwGroupShift];
+  const uint64_t before = __ballot(a.first_block[b0 + lane] <= blk);
   const uint32_t b = b0 + (uint32_t)__popcll(before) - 1u;
   const AdamwBuf buf = a.bufs[b];
   const void* const* const row = a.table + (size_t)b * kAwSlots;
-  const uint32_t t = tile - a.first_tile[b];
-  const uint64_t e = (uint64_t)t * kAwTile + (uint64_t)lane * kAwLane;   // first element inside the tensor
   const uint64_t n = buf.count;
   float* const w = static_cast<float*>(const_cast<void*>(row[CCN_MAX_RANKS]));
   uint16_t* const w16 = static_cast<uint16_t*>(const_cast<void*>(row[CCN_MAX_RANKS + 1]));
@@ -140,37 +153,35 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
 #pragma unroll
   for (int p = 0; p < CAP; p++)
     if (p < a.P) low |= reinterpret_cast<uintptr_t>(row[p]);
+  const uint64_t e = (uint64_t)(blk - buf.first_block) * kAwBlock + lane * kAwLane;   // first element inside the tensor
+  const uint64_t se = (uint64_t)blk * kAwBlock + lane * kAwLane;                      // and inside the moment arrays
   const bool wide = (low & 15u) == 0 && e + kAwLane <= n;
-  const uint64_t blk = buf.first_block + 2ull * t + (lane >> 5);
-  const bool inside = e < ((n + kAwBlock - 1) & ~(uint64_t)(kAwBlock - 1));   // the second block may not exist
-  const uint64_t se = blk * kAwBlock + (uint64_t)(lane & 31) * kAwLane;       // this lane's place in the moment arrays
 
   Pack<T, kAwLane> gp[CAP];
+  Pack<float, kAwLane> wp, mp, vp;
+  uint32_t mc = 0, vc = 0;
+  float sm = 0.0f, sr = 0.0f;
 #pragma unroll
   for (int p = 0; p < CAP; p++)
-    if (p < a.P) gp[p] = load8(static_cast<const T*>(row[p]), e, n, wide);
-  Pack<float, kAwLane> wp = load8(w, e, n, wide), mp, vp;
-  u32x2 mc = {0u, 0u}, vc = {0u, 0u};
-  float sm = 0.0f, sr = 0.0f;
-  if (inside) {
-    if constexpr (BITS == 32) {
-      mp = load_stream<float, kAwLane>(static_cast<const float*>(a.m) + se);
-      vp = load_stream<float, kAwLane>(static_cast<const float*>(a.v) + se);
-    } else {
-      mc = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.m) + se));
-      vc = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(a.v) + se));
-      sm = a.scales[blk];
-      sr = a.scales[a.blocks + blk];
-    }
+    if (p < a.P) gp[p] = load4(static_cast<const T*>(row[p]), e, n, wide);
+  wp = load4(w, e, n, wide);
+  if constexpr (BITS == 32) {
+    mp = load_stream<float, kAwLane>(static_cast<const float*>(a.m) + se);
+    vp = load_stream<float, kAwLane>(static_cast<const float*>(a.v) + se);
+  } else {
+    mc = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + se));
+    vc = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + se));
+    sm = a.scales[blk];
+    sr = a.scales[a.blocks + blk];
   }
   const float gs = a.grad_scale ? k.inv_scale * *a.grad_scale : k.inv_scale;
+  const float keep = 1.0f - k.lr_wd * buf.decay;
+  bool any_bad = false;
   if constexpr (BITS == 8) {
     from_e4m3(mc, sm, mp.d);
     from_e4m3(vc, sr, vp.d);
   }
   float root[kAwLane];
-  bool any_bad = false;
-  const float keep = 1.0f - k.lr_wd * buf.decay;
 #pragma unroll
   for (int j = 0; j < kAwLane; j++) {
     float g = widen<G>(gp[0].d[j]);
@@ -182,55 +193,49 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
     const float m1 = k.b1 * m0 + k.omb1 * g;
     const float v1 = k.b2 * v0 + k.omb2 * g * g;
     // a gradient that is not finite, or whose square is not: the element keeps its weight and moments
-    const bool bad = !(fabsf(m1) < __builtin_inff()) || !(v1 < __builtin_inff());
-    any_bad = any_bad || (bad && e + j < n);
-    const float update = (m1 * k.inv_bc1) / (sqrtf(v1 * k.inv_bc2) + k.eps);
-    const float w1 = wp.d[j] * keep - k.lr * update;
-    if (!bad) wp.d[j] = w1;
+    const bool bad = !(v1 < __builtin_inff());
+    any_bad = any_bad || bad;
+    const float r1 = square_root(v1);
+    const float w1 = wp.d[j] * keep - (k.rate * m1) * __builtin_amdgcn_rcpf(r1 * k.root_bc2 + k.eps);
+    wp.d[j] = bad ? wp.d[j] : w1;
     mp.d[j] = bad ? m0 : m1;
-    if constexpr (BITS == 8) root[j] = bad ? vp.d[j] : sqrtf(v1);
+    if constexpr (BITS == 8) root[j] = bad ? vp.d[j] : r1;
     else vp.d[j] = bad ? v0 : v1;
   }
-  store8(w, e, n, wide, wp);
+  store4(w, e, n, wide, wp);
   if (a.w16_type) {
     Pack<uint16_t, kAwLane> h;
 #pragma unroll
-    for (int j = 0; j < kAwLane; j++) h.d[j] = a.w16_type == CCN_TYPE_F16 ? f32_to_f16_bits(wp.d[j]) : f32_to_bf16_bits(wp.d[j]);
-    store8(w16, e, n, wide, h);
+    for (int j = 0; j < kAwLane; j++)
+      h.d[j] = a.w16_type == CCN_TYPE_F16 ? f32_to_f16_bits(wp.d[j]) : __builtin_bit_cast(uint16_t, (__bf16)wp.d[j]);
+    store4(w16, e, n, wide, h);
   }
   if constexpr (BITS == 32) {
-    if (inside) {
-      store_stream<float, kAwLane>(static_cast<float*>(a.m) + se, mp);
-      store_stream<float, kAwLane>(static_cast<float*>(a.v) + se, vp);
-    }
+    store_stream<float, kAwLane>(static_cast<float*>(a.m) + se, mp);
+    store_stream<float, kAwLane>(static_cast<float*>(a.v) + se, vp);
   } else {
     if (!wide) {   // what lies behind a tensor's end must not weigh on its last block's scale
 #pragma unroll
       for (int j = 0; j < kAwLane; j++)
         if (e + j >= n) mp.d[j] = root[j] = 0.0f;
     }
-    float mm = 0.0f, rm = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kAwLane; j++) {
-      mm = fmaxf(mm, fabsf(mp.d[j]));
-      rm = fmaxf(rm, root[j]);
-    }
-    mm = half_wave_max(mm);
-    rm = half_wave_max(rm);
-    const float sm1 = mm < kAwFlush ? 0.0f : mm / kE4m3Max, sr1 = rm / kE4m3Max;
-    const float im = sm1 > 0.0f ? 1.0f / sm1 : 0.0f, ir = sr1 > 0.0f ? 1.0f / sr1 : 0.0f;
-    const u32x2 c = to_e4m3(mp.d, im);
+    const float mm = wave_max(fmaxf(fmaxf(fabsf(mp.d[0]), fabsf(mp.d[1])), fmaxf(fabsf(mp.d[2]), fabsf(mp.d[3]))));
+    const float rm = wave_max(fmaxf(fmaxf(root[0], root[1]), fmaxf(root[2], root[3])));
+    const float sm1 = mm < kAwFlush ? 0.0f : mm * (1.0f / kE4m3Max), sr1 = rm * (1.0f / kE4m3Max);
+    const float im = sm1 > 0.0f ? inverse(sm1) : 0.0f, ir = sr1 > 0.0f ? inverse(sr1) : 0.0f;
     float y[kAwLane];
 #pragma unroll
-    for (int j = 0; j < kAwLane; j++) y[j] = root[j] > 0.0f ? fmaxf(root[j] * ir, kE4m3Tiny) : 0.0f;
-    const u32x2 d = to_e4m3(y, 1.0f);
-    if (inside) {
-      __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.m) + se));
-      __builtin_nontemporal_store(d, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.v) + se));
-      if ((lane & 31) == 0) {
-        a.scales[blk] = sm1;
-        a.scales[a.blocks + blk] = sr1;
-      }
+    for (int j = 0; j < kAwLane; j++) y[j] = __builtin_amdgcn_fmed3f(quotient(mp.d[j], sm1, im), -kE4m3Max, kE4m3Max);
+    const uint32_t c = to_e4m3(y);
+#pragma unroll
+    for (int j = 0; j < kAwLane; j++)
+      y[j] = root[j] > 0.0f ? __builtin_amdgcn_fmed3f(quotient(root[j], sr1, ir), kE4m3Tiny, kE4m3Max) : 0.0f;
+    const uint32_t d = to_e4m3(y);
+    __builtin_nontemporal_store(c, reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + se));
+    __builtin_nontemporal_store(d, reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + se));
+    if (lane == 0) {
+      a.scales[blk] = sm1;
+      a.scales[a.blocks + blk] = sr1;
     }
   }
   if (a.flag && __ballot(any_bad) != 0 && lane == 0) __hip_atomic_store(a.flag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -246,10 +251,9 @@ struct ccn_adamw_plan {
   int device = -1;
   int nbuff = 0, bits = 32;
   std::vector<int> live;               // the tensors that have elements
-  uint64_t blocks = 0;
-  uint32_t ntiles = 0;
+  uint32_t blocks = 0;
   uint32_t* coarse = nullptr;
-  uint32_t* first_tile = nullptr;
+  uint32_t* first_block = nullptr;
   AdamwBuf* bufs = nullptr;
   const void** table_dev = nullptr;    // [live][kAwSlots]
   const void** table_pinned = nullptr;
@@ -301,10 +305,16 @@ int adamw_sync_table(ccn_adamw_plan* p, const void* const* g, int P, float* cons
 
 template <int G, int CAP>
 int adamw_launch(const ccn_adamw_plan* p, const AdamwArgs& a, const AdamwPrm& k, hipStream_t s) {
-  const uint32_t gx = a.ntiles < 0x40000000u ? a.ntiles : 0x40000000u;
-  const dim3 grid(gx, (a.ntiles + gx - 1) / gx);
-  if (p->bits == 8) hipLaunchKernelGGL((adamw_kernel<G, CAP, 8>), grid, dim3(kWave), 0, s, a, k);
-  else hipLaunchKernelGGL((adamw_kernel<G, CAP, 32>), grid, dim3(kWave), 0, s, a, k);
+  const uint32_t gx = a.blocks < 0x40000000u ? a.blocks : 0x40000000u;
+  const dim3 grid(gx, (a.blocks + gx - 1) / gx);
+  // Wavefronts kept resident per CU, by a request for LDS that the kernel never touches (0: as many as fit, 32).  GB/s at
+  // 2^26 elements with no cap / 24 / 20 / 16 / 13 wavefronts: fp32 moments and fp32 gradients 6095 / 6199 / 6391 / 6465 /
+  // 6273 at 1 rank, 6145 / 6311 / 6468 / 6535 / 6001 at 8; fp32 moments and bf16 gradients 6214 / 6348 / 6416 / 6292 /
+  // 5615 at 1 rank, 6331 / 6170 / 5393 / 5028 / 4110 at 8; 8-bit moments 6060 / 5616 / 4725 (bf16 gradients, 1 rank),
+  // 6127 / 6344 / 6254 (fp32, 8 ranks): narrow accesses want every wavefront there is.
+  const unsigned lds = p->bits == 8 ? 0u : G == kGF32 ? 10240u : a.P == 1 ? 8192u : 0u;
+  if (p->bits == 8) hipLaunchKernelGGL((adamw_kernel<G, CAP, 8>), grid, dim3(kWave), lds, s, a, k);
+  else hipLaunchKernelGGL((adamw_kernel<G, CAP, 32>), grid, dim3(kWave), lds, s, a, k);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
@@ -334,7 +344,7 @@ int adamw_step(ccn_adamw_plan* p, const void* const* g, int P, int g_type, float
     if (!w[b] || (reinterpret_cast<uintptr_t>(w[b]) & 3u)) return CCN_EINVAL;
     if (w16 && (!w16[b] || (reinterpret_cast<uintptr_t>(w16[b]) & 1u))) return CCN_EINVAL;
   }
-  if (p->ntiles) {
+  if (p->blocks) {
     if (!m || !v || !aligned16(m) || !aligned16(v)) return CCN_EINVAL;
     if (p->bits == 8 ? (!scales || (reinterpret_cast<uintptr_t>(scales) & 3u)) : scales != nullptr) return CCN_EINVAL;
   }
@@ -343,7 +353,7 @@ int adamw_step(ccn_adamw_plan* p, const void* const* g, int P, int g_type, float
   if (rc != CCN_OK) return rc;
   if (di->device != p->device) return CCN_EINVAL;
   hipStream_t s = as_stream(stream);
-  if (p->ntiles) {
+  if (p->blocks) {
     rc = adamw_sync_table(p, g, P, w, w16, s);
     if (rc != CCN_OK) return rc;
   }
@@ -351,21 +361,20 @@ int adamw_step(ccn_adamw_plan* p, const void* const* g, int P, int g_type, float
     hipLaunchKernelGGL(adamw_clear_flag, dim3(1), dim3(1), 0, s, flag);
     CCN_HIP(hipGetLastError());
   }
-  if (!p->ntiles) return CCN_OK;
+  if (!p->blocks) return CCN_OK;
   AdamwPrm k;
   k.b1 = (float)beta1;
   k.omb1 = (float)(1.0 - beta1);
   k.b2 = (float)beta2;
   k.omb2 = (float)(1.0 - beta2);
   k.eps = (float)eps;
-  k.lr = (float)lr;
   k.lr_wd = (float)(lr * wd);
-  k.inv_bc1 = (float)(1.0 / (1.0 - std::pow(beta1, (double)step)));
-  k.inv_bc2 = (float)(1.0 / (1.0 - std::pow(beta2, (double)step)));
+  k.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+  k.root_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   k.inv_scale = (float)inv_scale;
   AdamwArgs a;
   a.coarse = p->coarse;
-  a.first_tile = p->first_tile;
+  a.first_block = p->first_block;
   a.bufs = p->bufs;
   a.table = p->table_dev;
   a.m = m;
@@ -374,7 +383,6 @@ int adamw_step(ccn_adamw_plan* p, const void* const* g, int P, int g_type, float
   a.grad_scale = grad_scale;
   a.flag = flag;
   a.blocks = p->blocks;
-  a.ntiles = p->ntiles;
   a.P = P;
   a.w16_type = w16 ? w16_type : 0;
   switch (g_type) {
@@ -396,7 +404,7 @@ int ccn_adamw_plan_destroy(ccn_adamw_plan* p) {
   if (p->copied && hipEventSynchronize(p->copied) != hipSuccess) rc = CCN_EHIP;
   if (p->copied && hipEventDestroy(p->copied) != hipSuccess) rc = CCN_EHIP;
   if (p->coarse && hipFree(p->coarse) != hipSuccess) rc = CCN_EHIP;
-  if (p->first_tile && hipFree(p->first_tile) != hipSuccess) rc = CCN_EHIP;
+  if (p->first_block && hipFree(p->first_block) != hipSuccess) rc = CCN_EHIP;
   if (p->bufs && hipFree(p->bufs) != hipSuccess) rc = CCN_EHIP;
   if (p->table_dev && hipFree(p->table_dev) != hipSuccess) rc = CCN_EHIP;
   if (p->table_pinned && hipHostFree(p->table_pinned) != hipSuccess) rc = CCN_EHIP;
@@ -435,19 +443,18 @@ int adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int b
   std::vector<AdamwBuf> bufs;
   std::vector<uint32_t> first, coarse;
   std::vector<int> live;
-  uint64_t blocks = 0, ntiles = 0;
+  uint64_t blocks = 0;
   for (int b = 0; b < nbuff; b++) {
     if (counts[b] == 0) continue;
     if (counts[b] > ((size_t)1 << 48)) return CCN_ERANGE;
-    const uint64_t nb = ((uint64_t)counts[b] + kAwBlock - 1) / kAwBlock, nt = (nb + 1) / 2;
-    if (ntiles + nt >= 0xffffffffull) return CCN_ERANGE;   // tile numbers are 32-bit
+    const uint64_t nb = ((uint64_t)counts[b] + kAwBlock - 1) / kAwBlock;
+    if (blocks + nb >= 0xffffffffull) return CCN_ERANGE;   // block numbers are 32-bit
     const uint32_t i = (uint32_t)bufs.size();
-    bufs.push_back(AdamwBuf{(uint64_t)counts[b], blocks, decay ? decay[b] : 1.0f, 0u});
-    first.push_back((uint32_t)ntiles);
+    bufs.push_back(AdamwBuf{(uint64_t)counts[b], (uint32_t)blocks, decay ? decay[b] : 1.0f});
+    first.push_back((uint32_t)blocks);
     live.push_back(b);
-    for (uint64_t grp = (ntiles + (1u << kAwGroupShift) - 1) >> kAwGroupShift; (grp << kAwGroupShift) < ntiles + nt; grp++) coarse.push_back(i);
+    for (uint64_t grp = (blocks + (1u << kAwGroupShift) - 1) >> kAwGroupShift; (grp << kAwGroupShift) < blocks + nb; grp++) coarse.push_back(i);
     blocks += nb;
-    ntiles += nt;
   }
   const DeviceInfo* di = nullptr;
   const int rc = current_device_info(&di);
@@ -456,23 +463,22 @@ int adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int b
   p->device = di->device;
   p->nbuff = nbuff;
   p->bits = bits;
-  p->blocks = blocks;
-  p->ntiles = (uint32_t)ntiles;
+  p->blocks = (uint32_t)blocks;
   hipError_t e = hipSuccess;
   try {
     p->live.swap(live);
-    first.insert(first.end(), kWave, 0xffffffffu);   // a wavefront looks at 64 tensors from the group's first one on
+    first.insert(first.end(), kWave, 0xffffffffu);   // a wavefront looks at 64 tensors from its group's first one on
     const size_t words = p->live.size() * (size_t)kAwSlots;
     p->shadow.assign(words, nullptr);
-    if (ntiles) {
+    if (blocks) {
       e = hipMalloc((void**)&p->coarse, coarse.size() * sizeof(uint32_t));
-      if (e == hipSuccess) e = hipMalloc((void**)&p->first_tile, first.size() * sizeof(uint32_t));
+      if (e == hipSuccess) e = hipMalloc((void**)&p->first_block, first.size() * sizeof(uint32_t));
       if (e == hipSuccess) e = hipMalloc((void**)&p->bufs, bufs.size() * sizeof(AdamwBuf));
       if (e == hipSuccess) e = hipMalloc((void**)&p->table_dev, words * sizeof(void*));
       if (e == hipSuccess) e = hipHostMalloc((void**)&p->table_pinned, words * sizeof(void*), hipHostMallocDefault);
       if (e == hipSuccess) e = hipEventCreateWithFlags(&p->copied, hipEventDisableTiming);
       if (e == hipSuccess) e = hipMemcpy(p->coarse, coarse.data(), coarse.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
-      if (e == hipSuccess) e = hipMemcpy(p->first_tile, first.data(), first.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
+      if (e == hipSuccess) e = hipMemcpy(p->first_block, first.data(), first.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
       if (e == hipSuccess) e = hipMemcpy(p->bufs, bufs.data(), bufs.size() * sizeof(AdamwBuf), hipMemcpyHostToDevice);
     }
   } catch (...) {

@@ -366,7 +366,7 @@ int  ccn_linear_backward_f16(ccn_linear_plan* plan, const uint16_t* dY, size_t l
  *      elements, in order (ccn_adamw_plan_sizes gives elements and blocks).  bits 32: m, v fp32, scales NULL.  bits 8: m, v
  *      one byte per element, scales an fp32 array of 2*blocks: element i of block b stands for m = e4m3(m[i])*scales[b] and
  *      sqrt(v) = e4m3(v[i])*scales[blocks + b], with OCP e4m3 codes.  The step computes in fp32 and rounds m and sqrt(v)
- *      to nearest even with the scale max/448 of their block; a sqrt(v) that is not zero is held as at least the smallest
+ *      to nearest even with the scale max * fp32(1/448) of their block; a sqrt(v) that is not zero is held as at least the smallest
  *      code; a block whose largest |m| is below 2^-100 is held as zeros.  All-zero arrays are the state to start from.
  *      Elements behind a tensor's end are not part of the state; an 8-bit step writes zeros there.
  *      grad_scale: DEVICE fp32 scalar (a clipping factor, a loss scale's inverse), or NULL for 1.
