@@ -23,7 +23,9 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 
 template <bool F16> __device__ __forceinline__ float half_in(uint16_t h) { return F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h); }
-template <bool F16> __device__ __forceinline__ uint16_t half_out(float f) { return F16 ? f32_to_f16_bits(f) : f32_to_bf16_bits(f); }
+template <bool F16> __device__ __forceinline__ uint16_t half_out(float f) {   // round to nearest even (gfx950 converts to bfloat16 itself)
+  return F16 ? f32_to_f16_bits(f) : __builtin_bit_cast(uint16_t, (__bf16)f);
+}
 
 // ---- activations, in fp32 ----------------------------------------------------------------------------------------------
 // A quarter-rate exp2 and reciprocal (1 ulp each) and a handful of multiply-adds per element: at one wavefront per SIMD the
@@ -49,15 +51,22 @@ __device__ __forceinline__ float normal_cdf(float z, float* bell) {
 __device__ __forceinline__ float gelu_tanh_gate(float z) {   // (1 + tanh u)/2 = sigmoid(2u)
   return sigmoid(2.0f * kTanhC * z * fmaf(kTanhA * z, z, 1.0f));
 }
-// The gate times z; a z so far left that the gate is 0 is cut off, -inf * 0 would be NaN.
-__device__ __forceinline__ float act_value(int act, float z) {
-  float bell;
-  switch (act) {
-    case CCN_ACT_RELU: return z < 0.0f ? 0.0f : z;
-    case CCN_ACT_GELU: return fmaxf(z, -104.0f) * normal_cdf(z, &bell);
-    case CCN_ACT_GELU_TANH: return fmaxf(z, -104.0f) * gelu_tanh_gate(z);
-    case CCN_ACT_SILU: return fmaxf(z, -104.0f) * sigmoid(z);
-    default: return z;
+// v <- act(v) for eight values.  The gate times z; a z so far left that the gate is 0 is cut off, -inf * 0 would be NaN.
+__device__ __forceinline__ void act_values(int act, float* v) {
+  if (act == CCN_ACT_NONE) return;
+  if (act == CCN_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = v[e] < 0.0f ? 0.0f : v[e];
+  } else if (act == CCN_ACT_GELU) {
+    float bell;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = fmaxf(v[e], -104.0f) * normal_cdf(v[e], &bell);
+  } else if (act == CCN_ACT_GELU_TANH) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = fmaxf(v[e], -104.0f) * gelu_tanh_gate(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = fmaxf(v[e], -104.0f) * sigmoid(v[e]);
   }
 }
 __device__ __forceinline__ float act_slope(int act, float z0) {
@@ -130,48 +139,68 @@ struct LinEpi {
   int accumulate;   // fp32 output only
 };
 
-// Finishes elements (row, col .. col+7) of the output, n of them inside the row.  OUT32: an fp32 output, stored or added
-// to; else the forward epilogue (of which a plain 16-bit product is the case with nothing to do).
+// Finishing elements (row, col .. col+7) of the output, n of them inside the row, in two steps, so that the loads of
+// several pieces can be in flight together.  OUT32: an fp32 output, stored or added to; else the forward epilogue (of
+// which a plain 16-bit product is the case with nothing to do).  The bias depends on the column alone.
+struct Bias8 { float b[8]; };
+__device__ __forceinline__ void load_bias(Bias8& x, const LinEpi& ep, size_t col, int n) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) x.b[e] = 0.0f;
+  if (!ep.bias) return;
+  if (n >= 8) {
+    __builtin_memcpy(x.b, ep.bias + col, 32);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+      if (e < n) x.b[e] = ep.bias[col + e];
+  }
+}
+template <bool OUT32> struct Old8 { u32x4 r; };        // the residual
+template <> struct Old8<true> { float d[8]; };         // what is added to
+template <bool OUT32>
+__device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, size_t row, size_t col, int n) {
+  if constexpr (OUT32) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x.d[e] = 0.0f;
+    if (!ep.accumulate) return;
+    const float* const o = static_cast<const float*>(ep.out) + row * ep.ldo + col;
+    if (n >= 8) {
+      __builtin_memcpy(x.d, o, 32);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 7; e++)
+        if (e < n) x.d[e] = o[e];
+    }
+  } else {
+    x.r = u32x4{0u, 0u, 0u, 0u};
+    if (ep.resid) x.r = load_piece(ep.resid + row * ep.ldr + col, n);
+  }
+}
 template <bool F16, bool OUT32>
-__device__ __forceinline__ void finish8(float* v, const LinEpi& ep, size_t row, size_t col, int n) {
+__device__ __forceinline__ void finish8(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, size_t row, size_t col, int n) {
   if constexpr (OUT32) {
     float* const o = static_cast<float*>(ep.out) + row * ep.ldo + col;
-    if (n >= 8) {
-      if (ep.accumulate) {
-        float old[8];
-        __builtin_memcpy(old, o, 32);
+    if (ep.accumulate) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += old[e];
-      }
+      for (int e = 0; e < 8; e++) v[e] = old.d[e] + v[e];
+    }
+    if (n >= 8) {
       __builtin_memcpy(o, v, 32);
     } else {
 #pragma unroll
       for (int e = 0; e < 7; e++)
-        if (e < n) o[e] = ep.accumulate ? o[e] + v[e] : v[e];
+        if (e < n) o[e] = v[e];
     }
   } else {
     if (ep.bias) {
-      float b[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      if (n >= 8) {
-        __builtin_memcpy(b, ep.bias + col, 32);
-      } else {
 #pragma unroll
-        for (int e = 0; e < 7; e++)
-          if (e < n) b[e] = ep.bias[col + e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] += b[e];
+      for (int e = 0; e < 8; e++) v[e] += bias.b[e];
     }
-    u32x4 r = {0u, 0u, 0u, 0u};
-    if (ep.resid) r = load_piece(ep.resid + row * ep.ldr + col, n);
     if (ep.pre) store_piece(ep.pre + row * ep.ldp + col, pack<F16>(v), n);
-    if (ep.act != CCN_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = act_value(ep.act, v[e]);
-    }
+    act_values(ep.act, v);
     if (ep.resid) {
       float x[8];
-      unpack<F16>(r, x);
+      unpack<F16>(old.r, x);
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] += x[e];
     }
@@ -337,8 +366,18 @@ void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
   __syncthreads();   // LDS becomes four private pieces of the output
   float* const cw = reinterpret_cast<float*>(lds) + wave * (32 * kGCStride);
   const int r8 = lane >> 3, c8 = lane & 7;
+  const int col = c0 + 64 * wc + 8 * c8, n = pr.cols - col;
+  Bias8 bias;
+  if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)col, n);
 #pragma unroll
   for (int b = 0; b < 2; b++) {
+    const int row0 = r0 + 64 * wr + 32 * b + r8;
+    Old8<OUT == kOut32> old[4];
+    if constexpr (OUT != kOutPartial) {
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+        if (row0 + 8 * s < pr.rows && n > 0) load_old<OUT == kOut32>(old[s], ep, (size_t)(row0 + 8 * s), (size_t)col, n);
+    }
 #pragma unroll
     for (int a = 0; a < 2; a++)
 #pragma unroll
@@ -349,17 +388,262 @@ void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
     __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
 #pragma unroll
     for (int s = 0; s < 4; s++) {
-      const int row = r0 + 64 * wr + 32 * b + 8 * s + r8, col = c0 + 64 * wc + 8 * c8;
+      const int row = row0 + 8 * s;
       float v[8];
       __builtin_memcpy(v, cw + (8 * s + r8) * kGCStride + 8 * c8, 32);
-      if (row < pr.rows && col < pr.cols) {
+      if (row < pr.rows && n > 0) {
         if constexpr (OUT == kOutPartial) {
           const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
           float* const o = pr.partial + ((size_t)blockIdx.y * pr.rows + row) * ld + col;
           __builtin_memcpy(o, v, 32);
         } else {
-          finish8<F16, OUT == kOut32>(v, ep, (size_t)row, (size_t)col, pr.cols - col);
+          finish8<F16, OUT == kOut32>(v, bias, old[s], ep, (size_t)row, (size_t)col, n);
         }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---- large tiles, 16-byte aligned rows --------------------------------------------------------------------------------------
+// A 256-thread workgroup owns a 256 x 256 tile, one wavefront per SIMD, each 128 x 128 as sixteen 32 x 32 blocks (256
+// accumulators, in the accumulation half of the register file); per 16 summed elements a wavefront reads four fragments of
+// each operand from LDS for sixteen matrix instructions.  The operands travel from memory to LDS directly, into a ring of
+// four stages of 32 summed elements: a wavefront requests 1 KiB every fourth matrix instruction, all the time, and a request
+// is waited for three steps after it was made.  An "along" stage is 256 rows of 64 bytes, its 16-byte pieces swizzled by
+// (row/4)%4; an "across" stage is 32 rows of 512 bytes as in memory, swizzled by 4*(k%4).  Tiles at the edge read the last
+// row or the last 8 columns again (results not stored); a sum that is no multiple of 32 ends with a step loaded through
+// registers with zeros behind the end.
+constexpr int kBT = 256, kBK = 32;
+constexpr int kBSide = kBT * kBK * 2;        // one operand's stage: 16 KiB
+constexpr int kBStage = 2 * kBSide;
+constexpr int kBLds = 4 * kBStage;
+constexpr int kBCStride = 128 + 4;           // floats per row of a wavefront's 32 x 128 piece of the output
+constexpr size_t kBMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
+
+__device__ __forceinline__ u32x4 descriptor(const void* base) {   // no stride; the offsets used below stay inside the matrix
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return u32x4{(uint32_t)a, (uint32_t)(a >> 32), 0x7ffffffcu, 0x00020000u};
+}
+// 1 KiB from memory to LDS, lane L's 16 bytes to position L.  In assembly, because the compiler puts a wait for ALL
+// outstanding loads before every LDS read that follows a direct load which it can see; here the waits are placed by hand:
+// a stage is read only behind the wait and the barrier of its step.
+__device__ __forceinline__ void load_to_lds(u32x4 rs, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rs), "s"(soff) : "memory");
+}
+
+template <bool ALONG> struct BSide {
+  const uint16_t* base;   // along: the tile's first row;  across: its first column
+  uint32_t voff[4], soff0, soffj;
+  size_t ld;
+  // wavefront w makes requests j = 0..3 of a stage: along: rows 16*(w + 4j) .. +15;  across: summed elements 2*(w + 4j), +1
+  __device__ __forceinline__ void init(const uint16_t* p, size_t ld_, int o0, int outer, int lane, int wave) {
+    ld = ld_;
+    if constexpr (ALONG) {
+      base = p + (size_t)o0 * ld;
+      const int last = outer - 1 - o0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int r = 16 * (wave + 4 * j) + (lane >> 2);
+        voff[j] = (uint32_t)(r < last ? r : last) * (uint32_t)(ld * 2) + 16u * (uint32_t)((lane & 3) ^ ((lane >> 4) & 3));
+      }
+      soff0 = soffj = 0;
+    } else {
+      base = p + o0;
+      const int c = 8 * ((lane & 31) ^ (4 * (2 * (wave & 1) + (lane >> 5)))), last = outer - 8 - o0;
+      voff[0] = (uint32_t)(lane >> 5) * (uint32_t)(ld * 2) + 2u * (uint32_t)(c < last ? c : last);
+      soff0 = (uint32_t)(2 * wave) * (uint32_t)(ld * 2);
+      soffj = 8u * (uint32_t)(ld * 2);
+    }
+  }
+  __device__ __forceinline__ void request(uint32_t lds_addr, int step, int j) const {
+    if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (kBK * 2));
+    else load_to_lds(descriptor(base + (size_t)step * kBK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
+  }
+  // the summed elements from `k` on, fewer than 32, through registers
+  __device__ __forceinline__ void put_tail(uint8_t* lds, int k, int left, int o0, int outer, int t) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int id = t + 256 * i;
+      u32x4 v;
+      if constexpr (ALONG) {
+        const int row = id >> 2, c = 8 * ((id & 3) ^ ((row >> 2) & 3)), last = outer - 1 - o0;
+        v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c);
+      } else {
+        const int kr = id >> 5, c = 8 * ((id & 31) ^ (4 * (kr & 3)));
+        v = load_piece(base + (size_t)(k + kr) * ld + c, kr < left ? outer - o0 - c : 0);
+      }
+      *reinterpret_cast<u32x4*>(lds + id * 16) = v;
+    }
+  }
+  // fragment f (32 rows or columns from 32*f of this wavefront's 128 at `half`), 16 summed elements from 16*ks
+  static __device__ __forceinline__ int address(int half, int lane) {
+    const int li = lane & 31, lh = lane >> 5;
+    if constexpr (ALONG) return (128 * half + li) * 64;
+    const int a16 = lane & 15, g2 = (lane >> 4) & 1;
+    return ((lh * 8 + (a16 >> 2)) * 32 + ((16 * half + 2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2)))) * 16 + 8 * (a16 & 1);
+  }
+  static __device__ __forceinline__ s16x8 frag(const uint8_t* lds, int at, int f, int ks, int lane) {
+    if constexpr (ALONG) {
+      const int li = lane & 31, lh = lane >> 5;
+      return *reinterpret_cast<const s16x8*>(lds + at + f * 2048 + (((2 * ks + lh) ^ ((li >> 2) & 3)) << 4));
+    } else {
+      const uint8_t* p = lds + (at ^ (f * 64)) + ks * (16 * 512);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 4 * 512));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+template <bool F16, bool PA, bool QA, bool OUT32>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_big[];
+  int tr, tc;
+  tile_of(blockIdx.x, pr.tiles_r, pr.tiles_c, tr, tc);
+  const int r0 = tr * kBT, c0 = tc * kBT;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);   // a scalar: it goes into descriptors
+  const int wr = wave >> 1, wc = wave & 1, li = lane & 31, lh = lane >> 5;
+  const int nk = pr.sum / kBK;   // at least 1
+
+  BSide<PA> sp;
+  BSide<QA> sq;
+  sp.init(pr.p, pr.ldp, r0, pr.rows, lane, wave);
+  sq.init(pr.q, pr.ldq, c0, pr.cols, lane, wave);
+  typedef __attribute__((address_space(3))) void* lds_void_ptr;
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_ptr)lds_big) + (uint32_t)wave * 1024u;
+  // request j of step `kt` (past the end: the last step's again, unused), into stage `stage`
+  auto request_p = [&](int stage, int kt, int j) { sp.request(lds0 + stage * kBStage, kt < nk ? kt : nk - 1, j); };
+  auto request_q = [&](int stage, int kt, int j) { sq.request(lds0 + stage * kBStage + kBSide, kt < nk ? kt : nk - 1, j); };
+  const int pat = BSide<PA>::address(wr, lane), qat = BSide<QA>::address(wc, lane);
+  auto read_p = [&](int stage, int f, int ks) { return BSide<PA>::frag(lds_big + stage * kBStage, pat, f, ks, lane); };
+  auto read_q = [&](int stage, int f, int ks) { return BSide<QA>::frag(lds_big + stage * kBStage + kBSide, qat, f, ks, lane); };
+
+  f32x16 acc[4][4];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
+#pragma unroll
+  for (int a = 0; a < 4; a++)
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[a][b][i] = 0.0f;
+
+  // A round of 16 summed elements multiplies from fragment set `set` while the fragments of the next round are read into the
+  // other set from (stage rbuf, half rks), in the order in which that round needs them; after every fourth matrix instruction
+  // one request for step `lkt` goes out.  Every piece is pinned in place: the order is the schedule.
+  s16x8 fq[2][4], fp[2][4];
+  auto mfma = [&](int set, int rb, int cb) { acc[cb][rb] = mfma32<F16>(fq[set][cb], fp[set][rb], acc[cb][rb]); };
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int half) {
+    const int o = set ^ 1;
+    fq[o][0] = read_q(rbuf, 0, rks); mfma(set, 0, 0); pin();
+    fp[o][0] = read_p(rbuf, 0, rks); mfma(set, 0, 1); pin();
+    fq[o][1] = read_q(rbuf, 1, rks); mfma(set, 0, 2); pin();
+    mfma(set, 0, 3); pin();
+    request_p(lstage, lkt, 2 * half); pin();
+    fq[o][2] = read_q(rbuf, 2, rks); mfma(set, 1, 0); pin();
+    fq[o][3] = read_q(rbuf, 3, rks); mfma(set, 1, 1); pin();
+    fp[o][1] = read_p(rbuf, 1, rks); mfma(set, 1, 2); pin();
+    mfma(set, 1, 3); pin();
+    request_p(lstage, lkt, 2 * half + 1); pin();
+    fp[o][2] = read_p(rbuf, 2, rks); mfma(set, 2, 0); pin();
+    mfma(set, 2, 1); pin();
+    mfma(set, 2, 2); pin();
+    mfma(set, 2, 3); pin();
+    request_q(lstage, lkt, 2 * half); pin();
+    fp[o][3] = read_p(rbuf, 3, rks); mfma(set, 3, 0); pin();
+    mfma(set, 3, 1); pin();
+    mfma(set, 3, 2); pin();
+    mfma(set, 3, 3); pin();
+    request_q(lstage, lkt, 2 * half + 1); pin();
+  };
+  // Step kt multiplies from stage kt%4:
+  //   round 0   reads the second half of this step's fragments; second half of the requests for step kt+3
+  //   barrier   every wavefront waits for its own requests for step kt+1 (the sixteen newer ones stay in flight) and for
+  //             its LDS reads, then for the others: stage (kt+1)%4 is complete, nobody reads stage kt%4 any more
+  //   round 1   reads the first half of step kt+1; first half of the requests for step kt+4, into stage kt%4
+  auto step = [&](int st, int kt) {
+    round(0, st, 1, (st + 3) & 3, kt + 3, 1);
+    __builtin_amdgcn_s_waitcnt(0x4070);   // vmcnt(16) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    pin();
+    round(1, (st + 1) & 3, 0, st, kt + 4, 0);
+  };
+#pragma unroll
+  for (int st = 0; st < 3; st++) {
+    request_p(st, st, 0); request_p(st, st, 1); request_q(st, st, 0); request_q(st, st, 1);
+    request_p(st, st, 2); request_p(st, st, 3); request_q(st, st, 2); request_q(st, st, 3);
+  }
+  request_p(3, 3, 0); request_p(3, 3, 1); request_q(3, 3, 0); request_q(3, 3, 1);
+  __builtin_amdgcn_s_waitcnt(0x4074);   // vmcnt(20) lgkmcnt(0): the requests for step 0 have landed
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int f = 0; f < 4; f++) fq[0][f] = read_q(0, f, 0);
+#pragma unroll
+  for (int f = 0; f < 4; f++) fp[0][f] = read_p(0, f, 0);
+  int kt = 0;
+  for (; kt + 4 <= nk; kt += 4) {
+    step(0, kt);
+    step(1, kt + 1);
+    step(2, kt + 2);
+    step(3, kt + 3);
+  }
+  if (kt < nk) step(0, kt);
+  if (kt + 1 < nk) step(1, kt + 1);
+  if (kt + 2 < nk) step(2, kt + 2);
+  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): the last reads of LDS and the last (unused) loads into it are done
+  __builtin_amdgcn_s_barrier();         // ... everywhere, before the stages are written to
+  const int left = pr.sum - nk * kBK;
+  if (left) {
+    sp.put_tail(lds_big, nk * kBK, left, r0, pr.rows, t);
+    sq.put_tail(lds_big + kBSide, nk * kBK, left, c0, pr.cols, t);
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+      for (int f = 0; f < 4; f++) {
+        fq[0][f] = read_q(0, f, ks);
+        fp[0][f] = read_p(0, f, ks);
+      }
+#pragma unroll
+      for (int rb = 0; rb < 4; rb++)
+#pragma unroll
+        for (int cb = 0; cb < 4; cb++) mfma(0, rb, cb);
+    }
+    __syncthreads();
+  }
+  // the accumulators leave through wavefront-private pieces of LDS, 32 rows of 128 columns at a time, as whole rows
+  float* const cw = reinterpret_cast<float*>(lds_big) + wave * (32 * kBCStride);
+  const int r4 = lane >> 4, c16 = lane & 15;
+  const int col = c0 + 128 * wc + 8 * c16, n = pr.cols - col;
+  const int row0 = r0 + 128 * wr + r4;   // piece i of 32 is row row0 + 4*i
+  Bias8 bias;
+  if constexpr (!OUT32) load_bias(bias, ep, (size_t)col, n);
+  Old8<OUT32> old[4];                    // four pieces ahead
+  auto fetch_old = [&](int u, int i) {
+    if (i < 32 && row0 + 4 * i < pr.rows && n > 0) load_old<OUT32>(old[u], ep, (size_t)(row0 + 4 * i), (size_t)col, n);
+  };
+#pragma unroll
+  for (int u = 0; u < 4; u++) fetch_old(u, u);
+#pragma unroll
+  for (int b = 0; b < 4; b++) {
+#pragma unroll
+    for (int a = 0; a < 4; a++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const f32x4 v = {acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
+        *reinterpret_cast<f32x4*>(cw + li * kBCStride + 32 * a + 8 * i + 4 * lh) = v;
+      }
+    __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
+#pragma unroll 1
+    for (int s = 0; s < 8; s += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int row = row0 + 32 * b + 4 * (s + u);
+        float v[8];
+        __builtin_memcpy(v, cw + (4 * (s + u) + r4) * kBCStride + 8 * c16, 32);
+        if (row < pr.rows && n > 0) finish8<F16, OUT32>(v, bias, old[u], ep, (size_t)row, (size_t)col, n);
+        fetch_old(u, 8 * b + s + u + 4);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -384,7 +668,12 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] += x[e];
   }
-  finish8<F16, OUT32>(v, ep, row, col, cols - (int)col);
+  const int n = cols - (int)col;
+  Bias8 bias;
+  Old8<OUT32> old;
+  load_bias(bias, ep, col, n);
+  load_old<OUT32>(old, ep, row, col, n);
+  finish8<F16, OUT32>(v, bias, old, ep, row, col, n);
 }
 
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
@@ -479,9 +768,43 @@ int splits_for(int tiles, int sum, int cus) {
   return s < 1 ? 1 : s;
 }
 
+template <bool F16, bool PA, bool QA, bool OUT32>
+int launch_tile256(const LinProd& pr, const LinEpi& ep, hipStream_t s) {
+  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_tile256_kernel<F16, PA, QA, OUT32>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kBLds);
+  if (attr != hipSuccess) return hip_fail(attr);
+  hipLaunchKernelGGL((linear_tile256_kernel<F16, PA, QA, OUT32>), dim3((unsigned)(pr.tiles_r * pr.tiles_c)), dim3(kBlock), kBLds, s, pr, ep);
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
+}
+template <bool F16, bool PA, bool QA>
+int product_tile256(const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum, const LinEpi& ep,
+                    bool out32, hipStream_t s) {
+  LinProd pr{};
+  pr.p = p;
+  pr.q = q;
+  pr.ldp = ldp;
+  pr.ldq = ldq;
+  pr.rows = rows;
+  pr.cols = cols;
+  pr.sum = sum;
+  pr.tiles_r = (rows + kBT - 1) / kBT;
+  pr.tiles_c = (cols + kBT - 1) / kBT;
+  if (!out32) return launch_tile256<F16, PA, QA, false>(pr, ep, s);
+  if constexpr (!PA && !QA) return launch_tile256<F16, PA, QA, true>(pr, ep, s);
+  else return CCN_EINVAL;
+}
+
 template <bool F16, bool PA, bool QA>
 int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum,
             const LinEpi& ep, bool out32, int cus, hipStream_t s) {
+  // Whole 16-byte pieces everywhere, enough steps to fill the ring, and enough large tiles for half of the CUs
+  const auto pieces = [](const uint16_t* x, size_t ld, bool along, int outer) {
+    return aligned16(x) && ld % 8 == 0 && ld <= kBMaxLd && (along || outer % 8 == 0);
+  };
+  const size_t big = (size_t)((rows + kBT - 1) / kBT) * (size_t)((cols + kBT - 1) / kBT);
+  if (pieces(p, ldp, PA, rows) && pieces(q, ldq, QA, cols) && sum >= 4 * kBK && 2 * big >= (size_t)cus && big <= 0x7fffffffull)
+    return product_tile256<F16, PA, QA>(p, ldp, q, ldq, rows, cols, sum, ep, out32, s);
   LinProd pr;
   pr.p = p;
   pr.q = q;
