@@ -155,15 +155,36 @@ __device__ __forceinline__ void load_bias(Bias8& x, const LinEpi& ep, size_t col
       if (e < n) x.b[e] = ep.bias[col + e];
   }
 }
+// Where the pieces of one lane lie: uniform bases and steps (scalar registers) and one 32-bit offset per lane and array.
+struct Places {
+  uint8_t *out, *pre;
+  const uint8_t* res;
+  size_t sout, spre, sres;     // bytes from a piece to the lane's next one
+  uint32_t vout, vpre, vres;
+};
+// row0, col0: uniform corner; the lane's first piece is at (row0 + lr, col0 + lc), the next ones `step` rows further each.
+template <bool OUT32>
+__device__ __forceinline__ Places places(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc, int step) {
+  constexpr int kOut = OUT32 ? 4 : 2;
+  Places w;
+  w.out = static_cast<uint8_t*>(ep.out) + (row0 * ep.ldo + col0) * kOut;
+  w.sout = (size_t)step * ep.ldo * kOut;
+  w.vout = (uint32_t)(lr * (int)ep.ldo + lc) * kOut;
+  w.res = reinterpret_cast<const uint8_t*>(ep.resid) + (row0 * ep.ldr + col0) * 2;
+  w.sres = (size_t)step * ep.ldr * 2;
+  w.vres = (uint32_t)(lr * (int)ep.ldr + lc) * 2;
+  w.pre = reinterpret_cast<uint8_t*>(ep.pre) + (row0 * ep.ldp + col0) * 2;
+  w.spre = (size_t)step * ep.ldp * 2;
+  w.vpre = (uint32_t)(lr * (int)ep.ldp + lc) * 2;
+  return w;
+}
 template <bool OUT32> struct Old8 { u32x4 r; };        // the residual
 template <> struct Old8<true> { float d[8]; };         // what is added to
 template <bool OUT32>
-__device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, size_t row, size_t col, int n) {
+__device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, const Places& w, int i, int n) {
   if constexpr (OUT32) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) x.d[e] = 0.0f;
     if (!ep.accumulate) return;
-    const float* const o = static_cast<const float*>(ep.out) + row * ep.ldo + col;
+    const float* const o = reinterpret_cast<const float*>(w.out + i * w.sout + w.vout);
     if (n >= 8) {
       __builtin_memcpy(x.d, o, 32);
     } else {
@@ -172,14 +193,13 @@ __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, size_
         if (e < n) x.d[e] = o[e];
     }
   } else {
-    x.r = u32x4{0u, 0u, 0u, 0u};
-    if (ep.resid) x.r = load_piece(ep.resid + row * ep.ldr + col, n);
+    if (ep.resid) x.r = load_piece(reinterpret_cast<const uint16_t*>(w.res + i * w.sres + w.vres), n);
   }
 }
 template <bool F16, bool OUT32>
-__device__ __forceinline__ void finish8(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, size_t row, size_t col, int n) {
+__device__ __forceinline__ void finish8(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, const Places& w, int i, int n) {
   if constexpr (OUT32) {
-    float* const o = static_cast<float*>(ep.out) + row * ep.ldo + col;
+    float* const o = reinterpret_cast<float*>(w.out + i * w.sout + w.vout);
     if (ep.accumulate) {
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] = old.d[e] + v[e];
@@ -196,7 +216,7 @@ __device__ __forceinline__ void finish8(float* v, const Bias8& bias, const Old8<
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] += bias.b[e];
     }
-    if (ep.pre) store_piece(ep.pre + row * ep.ldp + col, pack<F16>(v), n);
+    if (ep.pre) store_piece(reinterpret_cast<uint16_t*>(w.pre + i * w.spre + w.vpre), pack<F16>(v), n);
     act_values(ep.act, v);
     if (ep.resid) {
       float x[8];
@@ -204,7 +224,7 @@ __device__ __forceinline__ void finish8(float* v, const Bias8& bias, const Old8<
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] += x[e];
     }
-    store_piece(static_cast<uint16_t*>(ep.out) + row * ep.ldo + col, pack<F16>(v), n);
+    store_piece(reinterpret_cast<uint16_t*>(w.out + i * w.sout + w.vout), pack<F16>(v), n);
   }
 }
 
@@ -367,16 +387,18 @@ void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
   float* const cw = reinterpret_cast<float*>(lds) + wave * (32 * kGCStride);
   const int r8 = lane >> 3, c8 = lane & 7;
   const int col = c0 + 64 * wc + 8 * c8, n = pr.cols - col;
+  const int row0 = r0 + 64 * wr + r8;   // piece i of 8 is row row0 + 8*i
+  const int pieces = n > 0 ? (pr.rows - row0 + 7) >> 3 : 0;   // those inside the matrix
+  const Places where = places<OUT == kOut32>(ep, (size_t)(r0 + 64 * wr), (size_t)(c0 + 64 * wc), r8, 8 * c8, 8);
   Bias8 bias;
   if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)col, n);
 #pragma unroll
   for (int b = 0; b < 2; b++) {
-    const int row0 = r0 + 64 * wr + 32 * b + r8;
     Old8<OUT == kOut32> old[4];
     if constexpr (OUT != kOutPartial) {
 #pragma unroll
       for (int s = 0; s < 4; s++)
-        if (row0 + 8 * s < pr.rows && n > 0) load_old<OUT == kOut32>(old[s], ep, (size_t)(row0 + 8 * s), (size_t)col, n);
+        if (4 * b + s < pieces) load_old<OUT == kOut32>(old[s], ep, where, 4 * b + s, n);
     }
 #pragma unroll
     for (int a = 0; a < 2; a++)
@@ -388,16 +410,15 @@ void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
     __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
 #pragma unroll
     for (int s = 0; s < 4; s++) {
-      const int row = row0 + 8 * s;
       float v[8];
       __builtin_memcpy(v, cw + (8 * s + r8) * kGCStride + 8 * c8, 32);
-      if (row < pr.rows && n > 0) {
+      if (4 * b + s < pieces) {
         if constexpr (OUT == kOutPartial) {
           const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
-          float* const o = pr.partial + ((size_t)blockIdx.y * pr.rows + row) * ld + col;
+          float* const o = pr.partial + ((size_t)blockIdx.y * pr.rows + row0 + 8 * (4 * b + s)) * ld + col;
           __builtin_memcpy(o, v, 32);
         } else {
-          finish8<F16, OUT == kOut32>(v, bias, old[s], ep, (size_t)row, (size_t)col, n);
+          finish8<F16, OUT == kOut32>(v, bias, old[s], ep, where, 4 * b + s, n);
         }
       }
     }
@@ -492,6 +513,67 @@ template <bool ALONG> struct BSide {
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 4 * 512));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// finish8 for pieces that are all inside the row, addressed as the large tile wants it: a descriptor per array, the piece in
+// a scalar offset (it moves 4 rows from one to the next) and one 32-bit offset per lane.
+template <bool OUT32> struct WholePieces {
+  typedef __amdgpu_buffer_rsrc_t rsrc_t;
+  rsrc_t out, res, pre;
+  uint32_t vout, vres, vpre, sout, sres, spre;
+  static constexpr int kOut = OUT32 ? 4 : 2;
+  static __device__ __forceinline__ rsrc_t at(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7ffffffc, 0x00020000);
+  }
+  __device__ __forceinline__ WholePieces(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc) {
+    out = at(static_cast<uint8_t*>(ep.out) + (row0 * ep.ldo + col0) * kOut);
+    res = at(ep.resid + (row0 * ep.ldr + col0));
+    pre = at(ep.pre + (row0 * ep.ldp + col0));
+    vout = (uint32_t)(lr * (int)ep.ldo + lc) * kOut;
+    vres = (uint32_t)(lr * (int)ep.ldr + lc) * 2;
+    vpre = (uint32_t)(lr * (int)ep.ldp + lc) * 2;
+    sout = 4u * (uint32_t)ep.ldo * kOut;
+    sres = 4u * (uint32_t)ep.ldr * 2;
+    spre = 4u * (uint32_t)ep.ldp * 2;
+  }
+  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i) const {
+    if constexpr (OUT32) {
+      if (!ep.accumulate) return;
+      const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(out, vout, i * sout, 0));
+      const u32x4 hi = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(out, vout + 16, i * sout, 0));
+      __builtin_memcpy(x.d, &lo, 16);
+      __builtin_memcpy(x.d + 4, &hi, 16);
+    } else {
+      if (ep.resid) x.r = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(res, vres, i * sres, 0));
+    }
+  }
+  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i) const {
+    if constexpr (OUT32) {
+      if (ep.accumulate) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = old.d[e] + v[e];
+      }
+      u32x4 lo, hi;
+      __builtin_memcpy(&lo, v, 16);
+      __builtin_memcpy(&hi, v + 4, 16);
+      __builtin_amdgcn_raw_buffer_store_b128(lo, out, vout, i * sout, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(hi, out, vout + 16, i * sout, 0);
+    } else {
+      if (ep.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += bias.b[e];
+      }
+      if (ep.pre) __builtin_amdgcn_raw_buffer_store_b128(pack<F16>(v), pre, vpre, i * spre, 0);
+      act_values(ep.act, v);
+      if (ep.resid) {
+        float x[8];
+        unpack<F16>(old.r, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += x[e];
+      }
+      __builtin_amdgcn_raw_buffer_store_b128(pack<F16>(v), out, vout, i * sout, 0);
     }
   }
 };
@@ -617,11 +699,13 @@ void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
   const int r4 = lane >> 4, c16 = lane & 15;
   const int col = c0 + 128 * wc + 8 * c16, n = pr.cols - col;
   const int row0 = r0 + 128 * wr + r4;   // piece i of 32 is row row0 + 4*i
+  const int pieces = n > 0 ? (pr.rows - row0 + 3) >> 2 : 0;   // those inside the matrix
+  const WholePieces<OUT32> where(ep, (size_t)(r0 + 128 * wr), (size_t)(c0 + 128 * wc), r4, 8 * c16);
   Bias8 bias;
-  if constexpr (!OUT32) load_bias(bias, ep, (size_t)col, n);
+  if constexpr (!OUT32) load_bias(bias, ep, (size_t)col, n > 0 ? 8 : 0);
   Old8<OUT32> old[4];                    // four pieces ahead
   auto fetch_old = [&](int u, int i) {
-    if (i < 32 && row0 + 4 * i < pr.rows && n > 0) load_old<OUT32>(old[u], ep, (size_t)(row0 + 4 * i), (size_t)col, n);
+    if (i < pieces && i < 32) where.load_old(old[u], ep, i);
   };
 #pragma unroll
   for (int u = 0; u < 4; u++) fetch_old(u, u);
@@ -639,11 +723,11 @@ void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
     for (int s = 0; s < 8; s += 4) {
 #pragma unroll
       for (int u = 0; u < 4; u++) {
-        const int row = row0 + 32 * b + 4 * (s + u);
+        const int i = 8 * b + s + u;
         float v[8];
         __builtin_memcpy(v, cw + (4 * (s + u) + r4) * kBCStride + 8 * c16, 32);
-        if (row < pr.rows && n > 0) finish8<F16, OUT32>(v, bias, old[u], ep, (size_t)row, (size_t)col, n);
-        fetch_old(u, 8 * b + s + u + 4);
+        if (i < pieces) where.template finish<F16>(v, bias, old[u], ep, i);
+        fetch_old(u, i + 4);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -671,9 +755,10 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
   const int n = cols - (int)col;
   Bias8 bias;
   Old8<OUT32> old;
+  const Places where = places<OUT32>(ep, row, col, 0, 0, 0);
   load_bias(bias, ep, col, n);
-  load_old<OUT32>(old, ep, row, col, n);
-  finish8<F16, OUT32>(v, bias, old, ep, row, col, n);
+  load_old<OUT32>(old, ep, where, 0, n);
+  finish8<F16, OUT32>(v, bias, old, ep, where, 0, n);
 }
 
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
@@ -799,11 +884,13 @@ template <bool F16, bool PA, bool QA>
 int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum,
             const LinEpi& ep, bool out32, int cus, hipStream_t s) {
   // Whole 16-byte pieces everywhere, enough steps to fill the ring, and enough large tiles for half of the CUs
-  const auto pieces = [](const uint16_t* x, size_t ld, bool along, int outer) {
-    return aligned16(x) && ld % 8 == 0 && ld <= kBMaxLd && (along || outer % 8 == 0);
+  const auto pieces = [](const void* x, size_t ld, int size) {
+    return aligned16(x) && ld % (size_t)(16 / size) == 0 && ld * (size_t)size <= 2 * kBMaxLd;
   };
   const size_t big = (size_t)((rows + kBT - 1) / kBT) * (size_t)((cols + kBT - 1) / kBT);
-  if (pieces(p, ldp, PA, rows) && pieces(q, ldq, QA, cols) && sum >= 4 * kBK && 2 * big >= (size_t)cus && big <= 0x7fffffffull)
+  if (pieces(p, ldp, 2) && pieces(q, ldq, 2) && (PA || rows % 8 == 0) && cols % 8 == 0 && pieces(ep.out, ep.ldo, out32 ? 4 : 2) &&
+      (!ep.resid || pieces(ep.resid, ep.ldr, 2)) && (!ep.pre || pieces(ep.pre, ep.ldp, 2)) && sum >= 4 * kBK &&
+      2 * big >= (size_t)cus && big <= 0x7fffffffull)
     return product_tile256<F16, PA, QA>(p, ldp, q, ldq, rows, cols, sum, ep, out32, s);
   LinProd pr;
   pr.p = p;
