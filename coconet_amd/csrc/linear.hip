@@ -619,8 +619,11 @@ void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
   s16x8 fq[2][4], fp[2][4];
   auto mfma = [&](int set, int rb, int cb) { acc[cb][rb] = mfma32<F16>(fq[set][cb], fp[set][rb], acc[cb][rb]); };
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
-  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int half) {
-    const int o = set ^ 1;
+  // Odd steps make their two halves of the requests in the other order: a request of an "along" operand touches half of every
+  // 128-byte line, and the other half then follows one round later, while the line is still in L1 (dX of 8192 x 8192 x 4096:
+  // 430 -> 412 us).
+  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int first) {
+    const int o = set ^ 1, half = first ^ (lstage & 1);
     fq[o][0] = read_q(rbuf, 0, rks); mfma(set, 0, 0); pin();
     fp[o][0] = read_p(rbuf, 0, rks); mfma(set, 0, 1); pin();
     fq[o][1] = read_q(rbuf, 1, rks); mfma(set, 0, 2); pin();
@@ -659,7 +662,7 @@ void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
     request_p(st, st, 0); request_p(st, st, 1); request_q(st, st, 0); request_q(st, st, 1);
     request_p(st, st, 2); request_p(st, st, 3); request_q(st, st, 2); request_q(st, st, 3);
   }
-  request_p(3, 3, 0); request_p(3, 3, 1); request_q(3, 3, 0); request_q(3, 3, 1);
+  request_p(3, 3, 2); request_p(3, 3, 3); request_q(3, 3, 2); request_q(3, 3, 3);
   __builtin_amdgcn_s_waitcnt(0x4074);   // vmcnt(20) lgkmcnt(0): the requests for step 0 have landed
   __builtin_amdgcn_s_barrier();
 #pragma unroll
