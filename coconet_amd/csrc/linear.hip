@@ -245,6 +245,7 @@ struct LinProd {
   const uint16_t* q;   // column operand
   size_t ldp, ldq;
   int rows, cols, sum;
+  int read_r, read_c;  // rows or columns of the operands that may be read: rows, cols, or for an "across" operand that many rounded up to 8
   int tiles_r, tiles_c;
   int per_split;       // summed elements per split (a multiple of kGK)
   float* partial;      // [splits][rows][cols rounded up to 8] when splits > 1
@@ -426,21 +427,25 @@ void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
   }
 }
 
-// ---- large tiles, 16-byte aligned rows --------------------------------------------------------------------------------------
-// A 256-thread workgroup owns a 256 x 256 tile, one wavefront per SIMD, each 128 x 128 as sixteen 32 x 32 blocks (256
-// accumulators, in the accumulation half of the register file); per 16 summed elements a wavefront reads four fragments of
-// each operand from LDS for sixteen matrix instructions.  The operands travel from memory to LDS directly, into a ring of
-// four stages of 32 summed elements: a wavefront requests 1 KiB every fourth matrix instruction, all the time, and a request
-// is waited for three steps after it was made.  An "along" stage is 256 rows of 64 bytes, its 16-byte pieces swizzled by
-// (row/4)%4; an "across" stage is 32 rows of 512 bytes as in memory, swizzled by 4*(k%4).  Tiles at the edge read the last
-// row or the last 8 columns again (results not stored); a sum that is no multiple of 32 ends with a step loaded through
-// registers with zeros behind the end.
-constexpr int kBT = 256, kBK = 32;
-constexpr int kBSide = kBT * kBK * 2;        // one operand's stage: 16 KiB
-constexpr int kBStage = 2 * kBSide;
-constexpr int kBLds = 4 * kBStage;
-constexpr int kBCStride = 128 + 4;           // floats per row of a wavefront's 32 x 128 piece of the output
-constexpr size_t kBMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
+// ---- 16-byte aligned operands: tiles on a ring of direct-to-LDS stages -------------------------------------------------------
+// A 256-thread workgroup owns a tile of (64*FR) x (64*FC), its four wavefronts a quarter each, FR x FC blocks of 32 x 32.
+// The operands travel from memory to LDS directly, into a ring of four stages of 32 summed elements; requests of 1 KiB are
+// spread between the matrix instructions, and one is waited for three steps after it was made.  An "along" stage holds rows
+// of 64 bytes, the 16-byte pieces swizzled by (row/4)%4; an "across" stage 32 rows as in memory, swizzled by 4*(k%4).  Tiles
+// at the edge read the last row or the last 8 columns again (results not stored); a sum that is no multiple of 32 ends with
+// a step loaded through registers with zeros behind the end.
+//   4 x 4   256 x 256, one wavefront per SIMD (256 accumulators each, in the accumulation half of the register file), one
+//           workgroup per CU: per 16 summed elements a wavefront reads eight fragments for sixteen matrix instructions
+//   2 x 2   128 x 128, two workgroups per CU: four fragments for four matrix instructions, for outputs of few large tiles
+constexpr int kRK = 32;                      // summed elements per stage
+constexpr size_t kRMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
+template <int FR, int FC> struct Ring {
+  static constexpr int kRows = 64 * FR, kCols = 64 * FC;
+  static constexpr int kSideP = kRows * kRK * 2, kSideQ = kCols * kRK * 2, kStage = kSideP + kSideQ;
+  static constexpr int kCStride = 32 * FC + 4;   // floats per row of a wavefront's 32 x (32*FC) piece of the output
+  static constexpr int kLds = 4 * kStage > 4 * 32 * kCStride * 4 ? 4 * kStage : 4 * 32 * kCStride * 4;
+  static constexpr int kPerStep = FR + FC;       // requests of a wavefront per step
+};
 
 __device__ __forceinline__ u32x4 descriptor(const void* base) {   // no stride; the offsets used below stay inside the matrix
   const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -452,73 +457,81 @@ __device__ __forceinline__ u32x4 descriptor(const void* base) {   // no stride; 
 __device__ __forceinline__ void load_to_lds(u32x4 rs, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rs), "s"(soff) : "memory");
 }
+constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
 
-template <bool ALONG> struct BSide {
+// One operand of F 64-row (or 64-column) bands.
+template <bool ALONG, int F> struct RSide {
+  static constexpr int kOuter = 64 * F;
+  static constexpr int kRowBytes = kOuter * 2;             // across: one summed element
+  static constexpr int kLanes = kRowBytes / 16;            // across: lanes per summed element (32 or 16)
+  static constexpr int kPer = 64 / kLanes;                 // across: summed elements per request (2 or 4)
   const uint16_t* base;   // along: the tile's first row;  across: its first column
-  uint32_t voff[4], soff0, soffj;
+  uint32_t voff[F], soff0, soffj;
   size_t ld;
-  // wavefront w makes requests j = 0..3 of a stage: along: rows 16*(w + 4j) .. +15;  across: summed elements 2*(w + 4j), +1
+  // wavefront w makes requests j = 0..F-1 of a stage: along: rows 16*(w + 4j) .. +15;  across: summed elements
+  // kPer*(w + 4j) .. +kPer-1.  outer: rows, or columns that may be read (a multiple of 8)
   __device__ __forceinline__ void init(const uint16_t* p, size_t ld_, int o0, int outer, int lane, int wave) {
     ld = ld_;
     if constexpr (ALONG) {
       base = p + (size_t)o0 * ld;
       const int last = outer - 1 - o0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < F; j++) {
         const int r = 16 * (wave + 4 * j) + (lane >> 2);
         voff[j] = (uint32_t)(r < last ? r : last) * (uint32_t)(ld * 2) + 16u * (uint32_t)((lane & 3) ^ ((lane >> 4) & 3));
       }
       soff0 = soffj = 0;
     } else {
       base = p + o0;
-      const int c = 8 * ((lane & 31) ^ (4 * (2 * (wave & 1) + (lane >> 5)))), last = outer - 8 - o0;
-      voff[0] = (uint32_t)(lane >> 5) * (uint32_t)(ld * 2) + 2u * (uint32_t)(c < last ? c : last);
-      soff0 = (uint32_t)(2 * wave) * (uint32_t)(ld * 2);
-      soffj = 8u * (uint32_t)(ld * 2);
+      const int kr = lane / kLanes, k4 = kPer == 4 ? kr : 2 * (wave & 1) + kr;   // (kPer*(w + 4j) + kr) % 4
+      const int c = 8 * ((lane % kLanes) ^ (4 * k4)), last = outer - 8 - o0;
+      voff[0] = (uint32_t)kr * (uint32_t)(ld * 2) + 2u * (uint32_t)(c < last ? c : last);
+      soff0 = (uint32_t)(kPer * wave) * (uint32_t)(ld * 2);
+      soffj = (uint32_t)(4 * kPer) * (uint32_t)(ld * 2);
     }
   }
   __device__ __forceinline__ void request(uint32_t lds_addr, int step, int j) const {
-    if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (kBK * 2));
-    else load_to_lds(descriptor(base + (size_t)step * kBK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
+    if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (kRK * 2));
+    else load_to_lds(descriptor(base + (size_t)step * kRK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
   }
-  // the summed elements from `k` on, fewer than 32, through registers
+  // the summed elements from `k` on, `left` < 32 of them, through registers
   __device__ __forceinline__ void put_tail(uint8_t* lds, int k, int left, int o0, int outer, int t) const {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < F; i++) {
       const int id = t + 256 * i;
       u32x4 v;
       if constexpr (ALONG) {
         const int row = id >> 2, c = 8 * ((id & 3) ^ ((row >> 2) & 3)), last = outer - 1 - o0;
         v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c);
       } else {
-        const int kr = id >> 5, c = 8 * ((id & 31) ^ (4 * (kr & 3)));
+        const int kr = id / kLanes, c = 8 * ((id % kLanes) ^ (4 * (kr & 3)));
         v = load_piece(base + (size_t)(k + kr) * ld + c, kr < left ? outer - o0 - c : 0);
       }
       *reinterpret_cast<u32x4*>(lds + id * 16) = v;
     }
   }
-  // fragment f (32 rows or columns from 32*f of this wavefront's 128 at `half`), 16 summed elements from 16*ks
+  // fragment f: 32 rows or columns from 32*f of this wavefront's half of the tile, 16 summed elements from 16*ks on
   static __device__ __forceinline__ int address(int half, int lane) {
     const int li = lane & 31, lh = lane >> 5;
-    if constexpr (ALONG) return (128 * half + li) * 64;
+    if constexpr (ALONG) return (32 * F * half + li) * 64;
     const int a16 = lane & 15, g2 = (lane >> 4) & 1;
-    return ((lh * 8 + (a16 >> 2)) * 32 + ((16 * half + 2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2)))) * 16 + 8 * (a16 & 1);
+    return (lh * 8 + (a16 >> 2)) * kRowBytes + (((4 * F * half + 2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2))) * 16) + 8 * (a16 & 1);
   }
   static __device__ __forceinline__ s16x8 frag(const uint8_t* lds, int at, int f, int ks, int lane) {
     if constexpr (ALONG) {
       const int li = lane & 31, lh = lane >> 5;
       return *reinterpret_cast<const s16x8*>(lds + at + f * 2048 + (((2 * ks + lh) ^ ((li >> 2) & 3)) << 4));
     } else {
-      const uint8_t* p = lds + (at ^ (f * 64)) + ks * (16 * 512);
+      const uint8_t* p = lds + (at ^ (f * 64)) + ks * (16 * kRowBytes);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 4 * 512));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 4 * kRowBytes));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 };
 
-// finish8 for pieces that are all inside the row, addressed as the large tile wants it: a descriptor per array, the piece in
-// a scalar offset (it moves 4 rows from one to the next) and one 32-bit offset per lane.
+// finish8 for pieces that are all inside the row, addressed as the ring's tiles want it: a descriptor per array, the piece in
+// a scalar offset (it moves `step` rows from one to the next) and one 32-bit offset per lane.
 template <bool OUT32> struct WholePieces {
   typedef __amdgpu_buffer_rsrc_t rsrc_t;
   rsrc_t out, res, pre;
@@ -530,18 +543,18 @@ template <bool OUT32> struct WholePieces {
   static __device__ __forceinline__ rsrc_t at(const void* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7ffffffc, 0x00020000);
   }
-  __device__ __forceinline__ WholePieces(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc) {
+  __device__ __forceinline__ WholePieces(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc, int step) {
     out = at(static_cast<uint8_t*>(ep.out) + (row0 * ep.ldo + col0) * kOut);
     res = at(ep.resid + (row0 * ep.ldr + col0));
     pre = at(ep.pre + (row0 * ep.ldp + col0));
     vout = (uint32_t)(lr * (int)ep.ldo + lc) * kOut;
     vres = (uint32_t)(lr * (int)ep.ldr + lc) * 2;
     vpre = (uint32_t)(lr * (int)ep.ldp + lc) * 2;
-    sout = 4u * (uint32_t)ep.ldo * kOut;
-    sres = 4u * (uint32_t)ep.ldr * 2;
-    spre = 4u * (uint32_t)ep.ldp * 2;
+    sout = (uint32_t)step * (uint32_t)ep.ldo * kOut;
+    sres = (uint32_t)step * (uint32_t)ep.ldr * 2;
+    spre = (uint32_t)step * (uint32_t)ep.ldp * 2;
   }
-  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i) const {
+  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i, int) const {
     if constexpr (OUT32) {
       if (!ep.accumulate) return;
       const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(out, vout, i * sout, 0));
@@ -552,7 +565,7 @@ template <bool OUT32> struct WholePieces {
       if (ep.resid) x.r = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(res, vres, i * sres, 0));
     }
   }
-  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i) const {
+  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i, int) const {
     if constexpr (OUT32) {
       if (ep.accumulate) {
 #pragma unroll
@@ -580,166 +593,209 @@ template <bool OUT32> struct WholePieces {
     }
   }
 };
+// The same interface for rows that may start anywhere and end inside a piece.
+template <bool OUT32> struct AnyPieces {
+  Places w;
+  __device__ __forceinline__ AnyPieces(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc, int step)
+      : w(places<OUT32>(ep, row0, col0, lr, lc, step)) {}
+  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i, int n) const { ccn::load_old<OUT32>(x, ep, w, i, n); }
+  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i, int n) const {
+    finish8<F16, OUT32>(v, bias, old, ep, w, i, n);
+  }
+};
 
-template <bool F16, bool PA, bool QA, bool OUT32>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void linear_tile256_kernel(const LinProd pr, const LinEpi ep) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds_big[];
+// OUT: kOut16, kOut32 or kOutPartial.  WHOLE: every piece of an output row is inside it and 16-byte aligned.
+template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(FR * FC == 16 ? 1 : 2, FR * FC == 16 ? 1 : 2)))
+void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
+  typedef Ring<FR, FC> R;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
   int tr, tc;
   tile_of(blockIdx.x, pr.tiles_r, pr.tiles_c, tr, tc);
-  const int r0 = tr * kBT, c0 = tc * kBT;
+  const int r0 = tr * R::kRows, c0 = tc * R::kCols;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);   // a scalar: it goes into descriptors
   const int wr = wave >> 1, wc = wave & 1, li = lane & 31, lh = lane >> 5;
-  const int nk = pr.sum / kBK;   // at least 1
+  // this split's steps: first .. first + nk, and the elements behind the last whole step
+  const int first = OUT == kOutPartial ? (int)blockIdx.y * (pr.per_split / kRK) : 0;
+  const int k_begin = first * kRK;
+  const int k_end = OUT == kOutPartial && pr.sum - k_begin > pr.per_split ? k_begin + pr.per_split : pr.sum;
+  const int nk = (k_end - k_begin) / kRK, left = (k_end - k_begin) - nk * kRK;
 
-  BSide<PA> sp;
-  BSide<QA> sq;
-  sp.init(pr.p, pr.ldp, r0, pr.rows, lane, wave);
-  sq.init(pr.q, pr.ldq, c0, pr.cols, lane, wave);
+  RSide<PA, FR> sp;
+  RSide<QA, FC> sq;
+  sp.init(pr.p, pr.ldp, r0, pr.read_r, lane, wave);
+  sq.init(pr.q, pr.ldq, c0, pr.read_c, lane, wave);
   typedef __attribute__((address_space(3))) void* lds_void_ptr;
-  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_ptr)lds_big) + (uint32_t)wave * 1024u;
+  const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_ptr)lds_ring) + (uint32_t)wave * 1024u;
   // request j of step `kt` (past the end: the last step's again, unused), into stage `stage`
-  auto request_p = [&](int stage, int kt, int j) { sp.request(lds0 + stage * kBStage, kt < nk ? kt : nk - 1, j); };
-  auto request_q = [&](int stage, int kt, int j) { sq.request(lds0 + stage * kBStage + kBSide, kt < nk ? kt : nk - 1, j); };
-  const int pat = BSide<PA>::address(wr, lane), qat = BSide<QA>::address(wc, lane);
-  auto read_p = [&](int stage, int f, int ks) { return BSide<PA>::frag(lds_big + stage * kBStage, pat, f, ks, lane); };
-  auto read_q = [&](int stage, int f, int ks) { return BSide<QA>::frag(lds_big + stage * kBStage + kBSide, qat, f, ks, lane); };
+  auto request_p = [&](int stage, int kt, int j) { sp.request(lds0 + stage * R::kStage, first + (kt < nk ? kt : nk - 1), j); };
+  auto request_q = [&](int stage, int kt, int j) { sq.request(lds0 + stage * R::kStage + R::kSideP, first + (kt < nk ? kt : nk - 1), j); };
+  const int pat = RSide<PA, FR>::address(wr, lane), qat = RSide<QA, FC>::address(wc, lane);
+  auto read_p = [&](int stage, int f, int ks) { return RSide<PA, FR>::frag(lds_ring + stage * R::kStage, pat, f, ks, lane); };
+  auto read_q = [&](int stage, int f, int ks) { return RSide<QA, FC>::frag(lds_ring + stage * R::kStage + R::kSideP, qat, f, ks, lane); };
 
-  f32x16 acc[4][4];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
+  f32x16 acc[FC][FR];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
 #pragma unroll
-  for (int a = 0; a < 4; a++)
+  for (int a = 0; a < FC; a++)
 #pragma unroll
-    for (int b = 0; b < 4; b++)
+    for (int b = 0; b < FR; b++)
 #pragma unroll
       for (int i = 0; i < 16; i++) acc[a][b][i] = 0.0f;
 
   // A round of 16 summed elements multiplies from fragment set `set` while the fragments of the next round are read into the
-  // other set from (stage rbuf, half rks), in the order in which that round needs them; after every fourth matrix instruction
-  // one request for step `lkt` goes out.  Every piece is pinned in place: the order is the schedule.
-  s16x8 fq[2][4], fp[2][4];
-  auto mfma = [&](int set, int rb, int cb) { acc[cb][rb] = mfma32<F16>(fq[set][cb], fp[set][rb], acc[cb][rb]); };
-  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+  // other set from (stage rbuf, half rks), in the order in which that round needs them; between the matrix instructions half
+  // of the requests for step `lkt` go out.  Every piece is pinned in place: the order is the schedule.
   // Odd steps make their two halves of the requests in the other order: a request of an "along" operand touches half of every
   // 128-byte line, and the other half then follows one round later, while the line is still in L1 (dX of 8192 x 8192 x 4096:
   // 430 -> 412 us).
-  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int first) {
-    const int o = set ^ 1, half = first ^ (lstage & 1);
-    fq[o][0] = read_q(rbuf, 0, rks); mfma(set, 0, 0); pin();
-    fp[o][0] = read_p(rbuf, 0, rks); mfma(set, 0, 1); pin();
-    fq[o][1] = read_q(rbuf, 1, rks); mfma(set, 0, 2); pin();
-    mfma(set, 0, 3); pin();
-    request_p(lstage, lkt, 2 * half); pin();
-    fq[o][2] = read_q(rbuf, 2, rks); mfma(set, 1, 0); pin();
-    fq[o][3] = read_q(rbuf, 3, rks); mfma(set, 1, 1); pin();
-    fp[o][1] = read_p(rbuf, 1, rks); mfma(set, 1, 2); pin();
-    mfma(set, 1, 3); pin();
-    request_p(lstage, lkt, 2 * half + 1); pin();
-    fp[o][2] = read_p(rbuf, 2, rks); mfma(set, 2, 0); pin();
-    mfma(set, 2, 1); pin();
-    mfma(set, 2, 2); pin();
-    mfma(set, 2, 3); pin();
-    request_q(lstage, lkt, 2 * half); pin();
-    fp[o][3] = read_p(rbuf, 3, rks); mfma(set, 3, 0); pin();
-    mfma(set, 3, 1); pin();
-    mfma(set, 3, 2); pin();
-    mfma(set, 3, 3); pin();
-    request_q(lstage, lkt, 2 * half + 1); pin();
+  s16x8 fq[2][FC], fp[2][FR];
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int first_half) {
+    const int o = set ^ 1, half = first_half ^ (lstage & 1);
+    auto m = [&](int rb, int cb) { acc[cb][rb] = mfma32<F16>(fq[set][cb], fp[set][rb], acc[cb][rb]); };
+    if constexpr (FR == 4 && FC == 4) {
+      fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
+      fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
+      fq[o][1] = read_q(rbuf, 1, rks); m(0, 2); pin();
+      m(0, 3); pin();
+      request_p(lstage, lkt, 2 * half); pin();
+      fq[o][2] = read_q(rbuf, 2, rks); m(1, 0); pin();
+      fq[o][3] = read_q(rbuf, 3, rks); m(1, 1); pin();
+      fp[o][1] = read_p(rbuf, 1, rks); m(1, 2); pin();
+      m(1, 3); pin();
+      request_p(lstage, lkt, 2 * half + 1); pin();
+      fp[o][2] = read_p(rbuf, 2, rks); m(2, 0); pin();
+      m(2, 1); pin();
+      m(2, 2); pin();
+      m(2, 3); pin();
+      request_q(lstage, lkt, 2 * half); pin();
+      fp[o][3] = read_p(rbuf, 3, rks); m(3, 0); pin();
+      m(3, 1); pin();
+      m(3, 2); pin();
+      m(3, 3); pin();
+      request_q(lstage, lkt, 2 * half + 1); pin();
+    } else {
+      static_assert(FR == 2 && FC == 2, "a schedule is written out for 4 x 4 and 2 x 2 blocks");
+      fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
+      fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
+      request_p(lstage, lkt, half); pin();
+      fq[o][1] = read_q(rbuf, 1, rks); m(1, 0); pin();
+      fp[o][1] = read_p(rbuf, 1, rks); m(1, 1); pin();
+      request_q(lstage, lkt, half); pin();
+    }
   };
   // Step kt multiplies from stage kt%4:
   //   round 0   reads the second half of this step's fragments; second half of the requests for step kt+3
-  //   barrier   every wavefront waits for its own requests for step kt+1 (the sixteen newer ones stay in flight) and for
+  //   barrier   every wavefront waits for its own requests for step kt+1 (those of two newer steps stay in flight) and for
   //             its LDS reads, then for the others: stage (kt+1)%4 is complete, nobody reads stage kt%4 any more
   //   round 1   reads the first half of step kt+1; first half of the requests for step kt+4, into stage kt%4
   auto step = [&](int st, int kt) {
     round(0, st, 1, (st + 3) & 3, kt + 3, 1);
-    __builtin_amdgcn_s_waitcnt(0x4070);   // vmcnt(16) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(waitcnt(2 * R::kPerStep, 0));
     __builtin_amdgcn_s_barrier();
     pin();
     round(1, (st + 1) & 3, 0, st, kt + 4, 0);
   };
+  if (nk > 0) {
 #pragma unroll
-  for (int st = 0; st < 3; st++) {
-    request_p(st, st, 0); request_p(st, st, 1); request_q(st, st, 0); request_q(st, st, 1);
-    request_p(st, st, 2); request_p(st, st, 3); request_q(st, st, 2); request_q(st, st, 3);
+    for (int st = 0; st < 4; st++) {
+      // stage 3 is odd: its first half is the second half of the rows
+#pragma unroll
+      for (int j = st < 3 ? 0 : FR / 2; j < FR; j++) request_p(st, st, j);
+#pragma unroll
+      for (int j = st < 3 ? 0 : FC / 2; j < FC; j++) request_q(st, st, j);
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt(5 * R::kPerStep / 2, 0));   // the requests for step 0 have landed
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int f = 0; f < FC; f++) fq[0][f] = read_q(0, f, 0);
+#pragma unroll
+    for (int f = 0; f < FR; f++) fp[0][f] = read_p(0, f, 0);
+    int kt = 0;
+    for (; kt + 4 <= nk; kt += 4) {
+      step(0, kt);
+      step(1, kt + 1);
+      step(2, kt + 2);
+      step(3, kt + 3);
+    }
+    if (kt < nk) step(0, kt);
+    if (kt + 1 < nk) step(1, kt + 1);
+    if (kt + 2 < nk) step(2, kt + 2);
+    __builtin_amdgcn_s_waitcnt(waitcnt(0, 0));   // the last reads of LDS and the last (unused) loads into it are done
+    __builtin_amdgcn_s_barrier();                // ... everywhere, before the stages are written to
   }
-  request_p(3, 3, 2); request_p(3, 3, 3); request_q(3, 3, 2); request_q(3, 3, 3);
-  __builtin_amdgcn_s_waitcnt(0x4074);   // vmcnt(20) lgkmcnt(0): the requests for step 0 have landed
-  __builtin_amdgcn_s_barrier();
-#pragma unroll
-  for (int f = 0; f < 4; f++) fq[0][f] = read_q(0, f, 0);
-#pragma unroll
-  for (int f = 0; f < 4; f++) fp[0][f] = read_p(0, f, 0);
-  int kt = 0;
-  for (; kt + 4 <= nk; kt += 4) {
-    step(0, kt);
-    step(1, kt + 1);
-    step(2, kt + 2);
-    step(3, kt + 3);
-  }
-  if (kt < nk) step(0, kt);
-  if (kt + 1 < nk) step(1, kt + 1);
-  if (kt + 2 < nk) step(2, kt + 2);
-  __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): the last reads of LDS and the last (unused) loads into it are done
-  __builtin_amdgcn_s_barrier();         // ... everywhere, before the stages are written to
-  const int left = pr.sum - nk * kBK;
   if (left) {
-    sp.put_tail(lds_big, nk * kBK, left, r0, pr.rows, t);
-    sq.put_tail(lds_big + kBSide, nk * kBK, left, c0, pr.cols, t);
+    sp.put_tail(lds_ring, k_begin + nk * kRK, left, r0, pr.read_r, t);
+    sq.put_tail(lds_ring + R::kSideP, k_begin + nk * kRK, left, c0, pr.read_c, t);
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-      for (int f = 0; f < 4; f++) {
-        fq[0][f] = read_q(0, f, ks);
-        fp[0][f] = read_p(0, f, ks);
-      }
+      for (int f = 0; f < FC; f++) fq[0][f] = read_q(0, f, ks);
 #pragma unroll
-      for (int rb = 0; rb < 4; rb++)
+      for (int f = 0; f < FR; f++) fp[0][f] = read_p(0, f, ks);
 #pragma unroll
-        for (int cb = 0; cb < 4; cb++) mfma(0, rb, cb);
+      for (int rb = 0; rb < FR; rb++)
+#pragma unroll
+        for (int cb = 0; cb < FC; cb++) acc[cb][rb] = mfma32<F16>(fq[0][cb], fp[0][rb], acc[cb][rb]);
     }
     __syncthreads();
   }
-  // The accumulators leave through wavefront-private pieces of LDS, 32 rows of 128 columns at a time, as whole rows.  In a row
-  // of a piece the first and the second halves of all 8-column groups lie together (conflict-free 16-byte reads).
-  float* const cw = reinterpret_cast<float*>(lds_big) + wave * (32 * kBCStride);
-  const int r4 = lane >> 4, c16 = lane & 15;
-  const int col = c0 + 128 * wc + 8 * c16, n = pr.cols - col;
-  const int row0 = r0 + 128 * wr + r4;   // piece i of 32 is row row0 + 4*i
-  const int pieces = n > 0 ? (pr.rows - row0 + 3) >> 2 : 0;   // those inside the matrix
-  const WholePieces<OUT32> where(ep, (size_t)(r0 + 128 * wr), (size_t)(c0 + 128 * wc), r4, 8 * c16);
+  // The accumulators leave through wavefront-private pieces of LDS, 32 rows of 32*FC columns at a time, as whole rows.  In a
+  // row of a piece the first and the second halves of all 8-column groups lie together (conflict-free 16-byte reads).
+  constexpr int kLanesPerRow = 4 * FC, kStep = kWave / kLanesPerRow, kBlockPieces = 32 / kStep, kPieces = FR * kBlockPieces;
+  constexpr int kAhead = 4;
+  constexpr bool kO32 = OUT == kOut32;
+  float* const cw = reinterpret_cast<float*>(lds_ring) + wave * (32 * R::kCStride);
+  const int lr = lane / kLanesPerRow, lc = lane % kLanesPerRow;
+  const int row_first = r0 + 32 * FR * wr, col_first = c0 + 32 * FC * wc;
+  const int n = pr.cols - (col_first + 8 * lc);
+  const int pieces = n > 0 ? (pr.rows - (row_first + lr) + kStep - 1) / kStep : 0;   // piece i is row row_first + lr + kStep*i
+  typedef std::conditional_t<WHOLE, WholePieces<kO32>, AnyPieces<kO32>> Where;
+  const Where where(ep, (size_t)row_first, (size_t)col_first, lr, 8 * lc, kStep);
   Bias8 bias;
-  if constexpr (!OUT32) load_bias(bias, ep, (size_t)col, n > 0 ? 8 : 0);
-  Old8<OUT32> old[4];                    // four pieces ahead
+  if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)(col_first + 8 * lc), n);
+  Old8<kO32> old[kAhead];
   auto fetch_old = [&](int u, int i) {
-    if (i < pieces && i < 32) where.load_old(old[u], ep, i);
+    if constexpr (OUT != kOutPartial) {
+      if (i < pieces && i < kPieces) where.load_old(old[u], ep, i, n);
+    }
   };
 #pragma unroll
-  for (int u = 0; u < 4; u++) fetch_old(u, u);
+  for (int u = 0; u < kAhead; u++) fetch_old(u, u);
 #pragma unroll
-  for (int b = 0; b < 4; b++) {
+  for (int b = 0; b < FR; b++) {
 #pragma unroll
-    for (int a = 0; a < 4; a++)
+    for (int a = 0; a < FC; a++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const f32x4 v = {acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
-        *reinterpret_cast<f32x4*>(cw + li * kBCStride + 4 * (4 * a + i) + 64 * lh) = v;
+        *reinterpret_cast<f32x4*>(cw + li * R::kCStride + 4 * (4 * a + i) + 16 * FC * lh) = v;
       }
     __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
 #pragma unroll 1
-    for (int s = 0; s < 8; s += 4) {
-      float v[4][8];
+    for (int s = 0; s < kBlockPieces; s += kAhead) {
+      float v[kAhead][8];
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float* const src = cw + (4 * (s + u) + r4) * kBCStride + 4 * c16;
+      for (int u = 0; u < kAhead; u++) {
+        const float* const src = cw + (kStep * (s + u) + lr) * R::kCStride + 4 * lc;
         __builtin_memcpy(v[u], src, 16);
-        __builtin_memcpy(v[u] + 4, src + 64, 16);
+        __builtin_memcpy(v[u] + 4, src + 16 * FC, 16);
       }
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const int i = 8 * b + s + u;
-        if (i < pieces) where.template finish<F16>(v[u], bias, old[u], ep, i);
-        fetch_old(u, i + 4);
+      for (int u = 0; u < kAhead; u++) {
+        const int i = kBlockPieces * b + s + u;
+        if constexpr (OUT == kOutPartial) {
+          if (i < pieces) {
+            const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
+            f32x4* const o = reinterpret_cast<f32x4*>(pr.partial + ((size_t)blockIdx.y * pr.rows + (row_first + lr + kStep * i)) * ld + col_first + 8 * lc);
+            o[0] = f32x4{v[u][0], v[u][1], v[u][2], v[u][3]};
+            o[1] = f32x4{v[u][4], v[u][5], v[u][6], v[u][7]};
+          }
+        } else {
+          if (i < pieces) where.template finish<F16>(v[u], bias, old[u], ep, i, n);
+          fetch_old(u, i + kAhead);
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -837,6 +893,12 @@ constexpr size_t kMaxLd = (size_t)1 << 22;
 constexpr int kMaxChunks = 256;      // row chunks of the column sums
 constexpr size_t kMaxSplitTiles = 1024;   // tiles x splits of a split product, which bounds the partial sums' workspace
 
+#define CCN_TRY(expr)                  \
+  do {                                 \
+    const int _rc = (expr);            \
+    if (_rc != CCN_OK) return _rc;     \
+  } while (0)
+
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -865,45 +927,53 @@ int splits_for(int tiles, int sum, int cus) {
   return s < 1 ? 1 : s;
 }
 
-template <bool F16, bool PA, bool QA, bool OUT32>
-int launch_tile256(const LinProd& pr, const LinEpi& ep, hipStream_t s) {
-  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_tile256_kernel<F16, PA, QA, OUT32>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kBLds);
-  if (attr != hipSuccess) return hip_fail(attr);
-  hipLaunchKernelGGL((linear_tile256_kernel<F16, PA, QA, OUT32>), dim3((unsigned)(pr.tiles_r * pr.tiles_c)), dim3(kBlock), kBLds, s, pr, ep);
+template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
+int launch_ring(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) {
+  constexpr int kLds = Ring<FR, FC>::kLds;
+  if (kLds > 64 * 1024) {
+    static const hipError_t attr = hipFuncSetAttribute((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>,
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return hip_fail(attr);
+  }
+  hipLaunchKernelGGL((linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>), dim3((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits),
+                     dim3(kBlock), kLds, s, pr, ep);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
-template <bool F16, bool PA, bool QA>
-int product_tile256(const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum, const LinEpi& ep,
-                    bool out32, hipStream_t s) {
-  LinProd pr{};
-  pr.p = p;
-  pr.q = q;
-  pr.ldp = ldp;
-  pr.ldq = ldq;
-  pr.rows = rows;
-  pr.cols = cols;
-  pr.sum = sum;
-  pr.tiles_r = (rows + kBT - 1) / kBT;
-  pr.tiles_c = (cols + kBT - 1) / kBT;
-  if (!out32) return launch_tile256<F16, PA, QA, false>(pr, ep, s);
-  if constexpr (!PA && !QA) return launch_tile256<F16, PA, QA, true>(pr, ep, s);
-  else return CCN_EINVAL;
+template <bool F16, bool OUT32>
+int launch_join(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) {
+  const size_t threads = (size_t)pr.rows * (((size_t)pr.cols + 7) / 8);
+  hipLaunchKernelGGL((linear_join_kernel<F16, OUT32>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, pr.partial, splits,
+                     pr.rows, pr.cols, ep);
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
+}
+template <bool F16, bool PA, bool QA, int FR, int FC>
+int product_ring(LinProd& pr, const LinEpi& ep, bool out32, bool whole, int splits, hipStream_t s) {
+  pr.tiles_r = (pr.rows + 64 * FR - 1) / (64 * FR);
+  pr.tiles_c = (pr.cols + 64 * FC - 1) / (64 * FC);
+  if constexpr (FR * FC < 16) {
+    if (splits > 1) {
+      CCN_TRY((launch_ring<F16, PA, QA, FR, FC, kOutPartial, true>(pr, ep, splits, s)));
+      return out32 ? launch_join<F16, true>(pr, ep, splits, s) : launch_join<F16, false>(pr, ep, splits, s);
+    }
+  }
+  if (out32) {
+    if constexpr (!PA && !QA) {
+      if (whole) return launch_ring<F16, PA, QA, FR, FC, kOut32, true>(pr, ep, 1, s);
+      return launch_ring<F16, PA, QA, FR, FC, kOut32, false>(pr, ep, 1, s);
+    } else {
+      return CCN_EINVAL;
+    }
+  }
+  if (whole) return launch_ring<F16, PA, QA, FR, FC, kOut16, true>(pr, ep, 1, s);
+  return launch_ring<F16, PA, QA, FR, FC, kOut16, false>(pr, ep, 1, s);
 }
 
+// One product.  read_r, read_c: see LinProd.
 template <bool F16, bool PA, bool QA>
-int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t* q, size_t ldq, int rows, int cols, int sum,
-            const LinEpi& ep, bool out32, int cus, hipStream_t s) {
-  // Whole 16-byte pieces everywhere, enough steps to fill the ring, and enough large tiles for half of the CUs
-  const auto pieces = [](const void* x, size_t ld, int size) {
-    return aligned16(x) && ld % (size_t)(16 / size) == 0 && ld * (size_t)size <= 2 * kBMaxLd;
-  };
-  const size_t big = (size_t)((rows + kBT - 1) / kBT) * (size_t)((cols + kBT - 1) / kBT);
-  if (pieces(p, ldp, 2) && pieces(q, ldq, 2) && (PA || rows % 8 == 0) && cols % 8 == 0 && pieces(ep.out, ep.ldo, out32 ? 4 : 2) &&
-      (!ep.resid || pieces(ep.resid, ep.ldr, 2)) && (!ep.pre || pieces(ep.pre, ep.ldp, 2)) && sum >= 4 * kBK &&
-      2 * big >= (size_t)cus && big <= 0x7fffffffull)
-    return product_tile256<F16, PA, QA>(p, ldp, q, ldq, rows, cols, sum, ep, out32, s);
+int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, int read_r, const uint16_t* q, size_t ldq, int read_c, int rows, int cols,
+            int sum, const LinEpi& ep, bool out32, int cus, hipStream_t s) {
   LinProd pr;
   pr.p = p;
   pr.q = q;
@@ -912,12 +982,16 @@ int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t
   pr.rows = rows;
   pr.cols = cols;
   pr.sum = sum;
-  pr.tiles_r = (rows + kGT - 1) / kGT;
-  pr.tiles_c = (cols + kGT - 1) / kGT;
+  pr.read_r = read_r;
+  pr.read_c = read_c;
   pr.partial = plan->partial;
-  if ((size_t)pr.tiles_r * (size_t)pr.tiles_c > 0x7fffffffull) return CCN_ERANGE;
-  const int tiles = pr.tiles_r * pr.tiles_c;
-  int splits = splits_for(tiles, sum, cus);
+  const auto tiles = [&](int edge) { return (size_t)((rows + edge - 1) / edge) * (size_t)((cols + edge - 1) / edge); };
+  if (tiles(128) > 0x7fffffffull) return CCN_ERANGE;
+  const auto aligned = [](const void* x, size_t ld, int size) {
+    return aligned16(x) && ld % (size_t)(16 / size) == 0 && ld * (size_t)size <= 2 * kRMaxLd;
+  };
+  // how the sum is split when there are few tiles of 128 x 128
+  int splits = splits_for((int)tiles(128), sum, cus);
   const size_t each = (size_t)rows * (((size_t)cols + 7) & ~(size_t)7);
   if ((size_t)splits * each > plan->partial_floats) splits = (int)(plan->partial_floats / each);
   if (splits < 2) splits = 1;
@@ -925,15 +999,22 @@ int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, const uint16_t
   pr.per_split = ((steps + splits - 1) / splits) * kGK;
   if (splits > 1) splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
   if (pr.per_split < kGK) pr.per_split = kGK;
-  const dim3 grid((unsigned)tiles, (unsigned)splits), block(kBlock);
+  if (aligned(p, ldp, 2) && aligned(q, ldq, 2) && (PA || read_r % 8 == 0) && (QA || read_c % 8 == 0)) {
+    const bool whole = cols % 8 == 0 && aligned(ep.out, ep.ldo, out32 ? 4 : 2) && (!ep.resid || aligned(ep.resid, ep.ldr, 2)) &&
+                       (!ep.pre || aligned(ep.pre, ep.ldp, 2));
+    // large tiles where they occupy half of the CUs at least
+    if (2 * tiles(256) >= (size_t)cus && sum >= 4 * kRK) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
+    return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, splits, s);
+  }
+  pr.tiles_r = (rows + kGT - 1) / kGT;
+  pr.tiles_c = (cols + kGT - 1) / kGT;
+  const dim3 grid((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits), block(kBlock);
   if (splits > 1) {
     hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOutPartial>), grid, block, 0, s, pr, ep);
     CCN_HIP(hipGetLastError());
-    const size_t threads = (each / 8);
-    const dim3 jg((unsigned)((threads + kBlock - 1) / kBlock));
-    if (out32) hipLaunchKernelGGL((linear_join_kernel<F16, true>), jg, block, 0, s, pr.partial, splits, rows, cols, ep);
-    else hipLaunchKernelGGL((linear_join_kernel<F16, false>), jg, block, 0, s, pr.partial, splits, rows, cols, ep);
-  } else if (out32) {
+    return out32 ? launch_join<F16, true>(pr, ep, splits, s) : launch_join<F16, false>(pr, ep, splits, s);
+  }
+  if (out32) {
     if constexpr (!PA && !QA) hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut32>), grid, block, 0, s, pr, ep);
     else return CCN_EINVAL;
   } else {
@@ -955,11 +1036,6 @@ int check16(const void* p, size_t ld, int cols) {
   if (!p || !aligned2(p) || ld < (size_t)cols) return CCN_EINVAL;
   return ld > kMaxLd ? CCN_ERANGE : CCN_OK;
 }
-#define CCN_TRY(expr)                  \
-  do {                                 \
-    const int _rc = (expr);            \
-    if (_rc != CCN_OK) return _rc;     \
-  } while (0)
 
 template <bool F16>
 int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const uint16_t* W, size_t ldw, const float* bias,
@@ -975,7 +1051,7 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   if (pre) CCN_TRY(check16(pre, ldp, N));
   if (!aligned4(bias)) return CCN_EINVAL;
   const LinEpi ep{bias, resid, pre, Y, ldr, ldp, ldy, act, 0};
-  return product<F16, true, false>(plan, X, ldx, W, ldw, M, N, K, ep, false, di->cu_count, as_stream(stream));
+  return product<F16, true, false>(plan, X, ldx, M, W, ldw, N, M, N, K, ep, false, di->cu_count, as_stream(stream));
 }
 
 template <bool F16>
@@ -1022,11 +1098,11 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const size_t ldg = act != CCN_ACT_NONE ? lddz : lddy;
   if (dX && M > 0) {
     const LinEpi ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
-    CCN_TRY((product<F16, true, true>(plan, g, ldg, W, ldw, M, K, N, ep, false, di->cu_count, s)));
+    CCN_TRY((product<F16, true, true>(plan, g, ldg, M, W, ldw, K, M, K, N, ep, false, di->cu_count, s)));
   }
   if (dW) {
     const LinEpi ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
-    CCN_TRY((product<F16, false, false>(plan, X, ldx, g, ldg, K, N, M, ep, dw32, di->cu_count, s)));
+    CCN_TRY((product<F16, false, false>(plan, X, ldx, K, g, ldg, g == plan->dz ? (N + 7) & ~7 : N, K, N, M, ep, dw32, di->cu_count, s)));
   }
   return CCN_OK;
 }
