@@ -829,6 +829,205 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
   finish8<F16, OUT32>(v, bias, old, ep, where, 0, n);
 }
 
+// ---- few rows: the weights are read once, at the memory's rate ---------------------------------------------------------------
+// Up to 64 rows (16*MT): what counts is reading W, and every wavefront keeps 8 KiB of it in flight beside the 8 KiB it works on.
+// W goes from memory to registers and from there into v_mfma_f32_16x16x32, whose row operand it is; X (16 rows of it per
+// instruction) comes from the caches.  A wavefront's step:
+//   across (forward)   32 summed elements x 128 columns: lane (q, c) = (lane/16, lane%16) loads rows 8q .. 8q+7 of columns
+//                      8c .. 8c+7 and turns that 8 x 8 block over in registers: eight fragments of column 8c + j
+//   along (dX)         64 rows of W x 64 summed elements, fragments as they lie; row tiles are dealt so that a lane ends up
+//                      with eight neighbouring outputs
+// The four wavefronts of a workgroup take steps in turn and add up through LDS.  A strip whose sum is split over workgroups is
+// finished by the one that arrives last: partial sums go out and come back as relaxed agent-scope atomics (written through to
+// where the XCDs are coherent), complete (vmcnt 0) before the workgroup counts itself in; splits are added in ascending order
+// whoever does it.  The counter is back at zero when the call ends.
+constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16;
+template <bool ALONG> struct Few {
+  static constexpr int kWidth = ALONG ? 64 : 128;   // outputs of a strip
+  static constexpr int kStep = ALONG ? 64 : 32;     // summed elements of a wavefront's step
+  static constexpr int kAcc = ALONG ? 4 : 8;
+};
+struct FewArgs {
+  const uint16_t* x;
+  const uint16_t* w;
+  size_t ldx, ldw;
+  int rows, cols, sum;
+  int per_split;        // a multiple of kStep
+  float* partial;       // [splits][strips][16*MT][kWidth]
+  uint32_t* counters;   // [strips], zero
+};
+__device__ __forceinline__ void store_through(float* p, const float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    uint64_t x;
+    __builtin_memcpy(&x, v + 2 * e, 8);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p) + e, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+__device__ __forceinline__ void load_through(float* v, const float* p) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_memcpy(v + 2 * e, &x, 8);
+  }
+}
+template <bool F16> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16, int MT, bool ALONG>
+__global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const FewArgs a, const LinEpi ep) {
+  typedef Few<ALONG> D;
+  constexpr int kStride = D::kWidth + 4;
+  __shared__ __attribute__((aligned(16))) float red[kFewWaves][16 * kStride];
+  __shared__ uint32_t arrived;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), q = lane >> 4, c = lane & 15;
+  const int strip = blockIdx.x, split = blockIdx.y, splits = gridDim.y;
+  const int n0 = strip * D::kWidth;
+  const int k_begin = split * a.per_split, k_end = a.sum - k_begin < a.per_split ? a.sum : k_begin + a.per_split;
+
+  // W pieces i = 0..7 of a step.  across: row 8q + i, columns 8c..;  along: row tile i/2, half i%2 of the summed elements
+  const uint16_t* wp[ALONG ? 4 : 1];
+  if constexpr (ALONG) {
+#pragma unroll
+    for (int T = 0; T < 4; T++) {
+      const int r = n0 + 32 * (T >> 1) + 8 * (c >> 2) + 4 * (T & 1) + (c & 3);
+      wp[T] = a.w + (size_t)(r < a.cols ? r : a.cols - 1) * a.ldw + 8 * q;
+    }
+  } else {
+    wp[0] = a.w + (size_t)(8 * q) * a.ldw + n0 + 8 * c;
+  }
+  const bool inside = ALONG || n0 + D::kWidth <= a.cols;
+  const uint16_t* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    const int r = 16 * m + c;
+    xp[m] = a.x + (size_t)(r < a.rows ? r : a.rows - 1) * a.ldx + 8 * q;
+  }
+  struct Step {
+    u32x4 w[8], x[MT][ALONG ? 2 : 1];
+  };
+  auto fetch = [&](Step& s, int k) {
+    const bool whole = inside && k + D::kStep <= k_end;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint16_t* const p = ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw;
+      if (whole) __builtin_memcpy(&s.w[i], p, 16);
+      else s.w[i] = load_piece(p, ALONG ? k_end - (k + 32 * (i & 1) + 8 * q) : (k + 8 * q + i < k_end ? a.cols - (n0 + 8 * c) : 0));
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int h = 0; h < (ALONG ? 2 : 1); h++) {
+        if (whole) __builtin_memcpy(&s.x[m][h], xp[m] + k + 32 * h, 16);
+        else s.x[m][h] = load_piece(xp[m] + k + 32 * h, k_end - (k + 32 * h + 8 * q));
+      }
+  };
+  f32x4 acc[MT][D::kAcc];
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int j = 0; j < D::kAcc; j++) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const Step& s) {
+    if constexpr (ALONG) {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[m][i >> 1] = mfma16<F16>(s.w[i], s.x[m][i & 1], acc[m][i >> 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        u32x4 f;   // column 8c + j, summed elements 8q .. 8q+7
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          f[e] = __builtin_amdgcn_perm(s.w[2 * e + 1][j >> 1], s.w[2 * e][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[m][j] = mfma16<F16>(f, s.x[m][0], acc[m][j]);
+      }
+    }
+  };
+  {
+    constexpr int kStride2 = kFewWaves * D::kStep;
+    Step s0, s1;
+    int k = k_begin + wave * D::kStep;
+    if (k < k_end) fetch(s0, k);
+    for (; k < k_end; k += 2 * kStride2) {
+      if (k + kStride2 < k_end) fetch(s1, k + kStride2);
+      multiply(s0);
+      if (k + 2 * kStride2 < k_end) fetch(s0, k + 2 * kStride2);
+      if (k + kStride2 < k_end) multiply(s1);
+    }
+  }
+  // element (m, col) of the strip: across: lane (q, c = m) holds columns 8*(4q + i) + j in acc[..][j][i];
+  // along: 32*(T/2) + 8q + 4*(T%2) + i in acc[..][T][i]
+  constexpr int kPieces = D::kWidth / 8;
+  const int row = t / kPieces, piece = t % kPieces, col = n0 + 8 * piece, n = a.cols - col;
+  auto part = [&](int s, int m) {
+    return a.partial + ((((size_t)s * gridDim.x + strip) * MT + m) * 16 + row) * D::kWidth + 8 * piece;
+  };
+  auto finish = [&](float* v, int m) {
+    if (n <= 0) return;
+    const Places where = places<false>(ep, (size_t)(16 * m + row), (size_t)col, 0, 0, 0);
+    Bias8 bias;
+    Old8<false> old;
+    load_bias(bias, ep, (size_t)col, n);
+    load_old<false>(old, ep, where, 0, n);
+    finish8<F16, false>(v, bias, old, ep, where, 0, n);
+  };
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    if (m) __syncthreads();
+    if constexpr (ALONG) {
+#pragma unroll
+      for (int T = 0; T < 4; T++) *reinterpret_cast<f32x4*>(&red[wave][c * kStride + 32 * (T >> 1) + 8 * q + 4 * (T & 1)]) = acc[m][T];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          *reinterpret_cast<f32x4*>(&red[wave][c * kStride + 8 * (4 * q + i) + 4 * h]) =
+              f32x4{acc[m][4 * h][i], acc[m][4 * h + 1][i], acc[m][4 * h + 2][i], acc[m][4 * h + 3][i]};
+    }
+    __syncthreads();
+    if (row < 16 && 16 * m + row < a.rows) {
+      float v[8];
+      __builtin_memcpy(v, &red[0][row * kStride + 8 * piece], 32);
+#pragma unroll
+      for (int w = 1; w < kFewWaves; w++) {
+        float x[8];
+        __builtin_memcpy(x, &red[w][row * kStride + 8 * piece], 32);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += x[e];
+      }
+      if (splits == 1) finish(v, m);
+      else store_through(part(split, m), v);
+    }
+  }
+  if (splits == 1) return;
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wavefront's partial sums have arrived
+  __syncthreads();
+  if (t == 0) arrived = __hip_atomic_fetch_add(a.counters + strip, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != (uint32_t)splits - 1u) return;
+  if (t == 0) __hip_atomic_store(a.counters + strip, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll 1
+  for (int m = 0; m < MT; m++) {
+    if (row < 16 && 16 * m + row < a.rows) {
+      float v[8];
+      load_through(v, part(0, m));
+#pragma unroll 4
+      for (int s = 1; s < splits; s++) {
+        float x[8];
+        load_through(x, part(s, m));
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += x[e];
+      }
+      finish(v, m);
+    }
+  }
+}
+
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
 // dz = dY * act'(pre), rounded to the operands' type into the workspace (rows of N rounded up to 8, zeros in the rest),
 // and fp32 sums over a chunk of rows of the unrounded dz.  Four wavefronts walk a chunk's rows, 512 columns wide.
@@ -913,6 +1112,7 @@ struct ccn_linear_plan {
   float* sums = nullptr;
   float* partial = nullptr;
   size_t partial_floats = 0;
+  uint32_t* counters = nullptr;   // arrivals per strip of the few-row kernels; zero between calls
 };
 
 namespace {
@@ -968,6 +1168,40 @@ int product_ring(LinProd& pr, const LinEpi& ep, bool out32, bool whole, int spli
   }
   if (whole) return launch_ring<F16, PA, QA, FR, FC, kOut16, true>(pr, ep, 1, s);
   return launch_ring<F16, PA, QA, FR, FC, kOut16, false>(pr, ep, 1, s);
+}
+
+// Up to kFewRows rows.
+template <bool F16, bool ALONG>
+int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint16_t* w, size_t ldw, int rows, int cols, int sum,
+                const LinEpi& ep, int cus, hipStream_t s) {
+  typedef Few<ALONG> D;
+  FewArgs a;
+  a.x = x;
+  a.w = w;
+  a.ldx = ldx;
+  a.ldw = ldw;
+  a.rows = rows;
+  a.cols = cols;
+  a.sum = sum;
+  a.partial = plan->partial;
+  a.counters = plan->counters;
+  const int strips = (cols + D::kWidth - 1) / D::kWidth, steps = (sum + D::kStep - 1) / D::kStep;
+  // a workgroup for every CU, each wavefront with a step at least
+  int splits = (cus + strips - 1) / strips;
+  if (splits > steps / kFewWaves) splits = steps / kFewWaves;
+  if (splits > kFewMaxSplits) splits = kFewMaxSplits;
+  if (splits < 1) splits = 1;
+  a.per_split = ((steps + splits - 1) / splits) * D::kStep;
+  splits = (sum + a.per_split - 1) / a.per_split;   // no empty split
+  const dim3 grid((unsigned)strips, (unsigned)splits), block(kFewWaves * kWave);
+  switch ((rows + 15) / 16) {
+    case 1: hipLaunchKernelGGL((linear_few_kernel<F16, 1, ALONG>), grid, block, 0, s, a, ep); break;
+    case 2: hipLaunchKernelGGL((linear_few_kernel<F16, 2, ALONG>), grid, block, 0, s, a, ep); break;
+    case 3: hipLaunchKernelGGL((linear_few_kernel<F16, 3, ALONG>), grid, block, 0, s, a, ep); break;
+    default: hipLaunchKernelGGL((linear_few_kernel<F16, 4, ALONG>), grid, block, 0, s, a, ep); break;
+  }
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
 }
 
 // One product.  read_r, read_c: see LinProd.
@@ -1051,6 +1285,7 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   if (pre) CCN_TRY(check16(pre, ldp, N));
   if (!aligned4(bias)) return CCN_EINVAL;
   const LinEpi ep{bias, resid, pre, Y, ldr, ldp, ldy, act, 0};
+  if (M <= kFewRows) return product_few<F16, false>(plan, X, ldx, W, ldw, M, N, K, ep, di->cu_count, as_stream(stream));
   return product<F16, true, false>(plan, X, ldx, M, W, ldw, N, M, N, K, ep, false, di->cu_count, as_stream(stream));
 }
 
@@ -1098,7 +1333,8 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const size_t ldg = act != CCN_ACT_NONE ? lddz : lddy;
   if (dX && M > 0) {
     const LinEpi ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
-    CCN_TRY((product<F16, true, true>(plan, g, ldg, M, W, ldw, K, M, K, N, ep, false, di->cu_count, s)));
+    if (M <= kFewRows) CCN_TRY((product_few<F16, true>(plan, g, ldg, W, ldw, M, K, N, ep, di->cu_count, s)));
+    else CCN_TRY((product<F16, true, true>(plan, g, ldg, M, W, ldw, K, M, K, N, ep, false, di->cu_count, s)));
   }
   if (dW) {
     const LinEpi ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
@@ -1117,6 +1353,7 @@ int ccn_linear_plan_destroy(ccn_linear_plan* plan) {
   if (plan->dz && hipFree(plan->dz) != hipSuccess) rc = CCN_EHIP;
   if (plan->sums && hipFree(plan->sums) != hipSuccess) rc = CCN_EHIP;
   if (plan->partial && hipFree(plan->partial) != hipSuccess) rc = CCN_EHIP;
+  if (plan->counters && hipFree(plan->counters) != hipSuccess) rc = CCN_EHIP;
   delete plan;
   return rc;
 }
@@ -1142,10 +1379,17 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   };
   const size_t need[3] = {floats(max_M, max_N, max_K), floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
   for (const size_t f : need) p->partial_floats = f > p->partial_floats ? f : p->partial_floats;
+  const size_t few_cols = ((size_t)(max_N > max_K ? max_N : max_K) + 127) & ~(size_t)127;
+  const size_t few = (size_t)kFewMaxSplits * few_cols * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
+  p->partial_floats = few > p->partial_floats ? few : p->partial_floats;
+  const size_t strips = few_cols / 64;
   const size_t lddz = ((size_t)max_N + 7) & ~(size_t)7;
   hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * lddz * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->counters, strips * sizeof(uint32_t));
+  if (e == hipSuccess) e = hipMemset(p->counters, 0, strips * sizeof(uint32_t));
+  if (e == hipSuccess) e = hipDeviceSynchronize();   // the zeros are there for calls on any stream
   if (e != hipSuccess) {
     ccn_linear_plan_destroy(p);
     return hip_fail(e);
