@@ -69,30 +69,34 @@ __device__ __forceinline__ void act_values(int act, float* v) {
     for (int e = 0; e < 8; e++) v[e] = fmaxf(v[e], -104.0f) * sigmoid(v[e]);
   }
 }
-__device__ __forceinline__ float act_slope(int act, float z0) {
-  const float z = fminf(fmaxf(z0, -104.0f), 104.0f);   // the slopes are 0 and 1 from there on
-  float r;
-  switch (act) {
-    case CCN_ACT_RELU: r = z > 0.0f ? 1.0f : 0.0f; break;
-    case CCN_ACT_GELU: {
-      float bell;
-      const float p = normal_cdf(z, &bell);
-      r = fmaf(z * kInvSqrt2Pi, bell, p);
-      break;
-    }
-    case CCN_ACT_GELU_TANH: {
-      const float s = gelu_tanh_gate(z);
-      r = fmaf(z * s * (1.0f - s) * (2.0f * kTanhC), fmaf(3.0f * kTanhA * z, z, 1.0f), s);
-      break;
-    }
-    case CCN_ACT_SILU: {
-      const float s = sigmoid(z);
-      r = s * fmaf(z, 1.0f - s, 1.0f);
-      break;
-    }
-    default: r = 1.0f;
+// g <- g * act'(z) for eight values.  Beyond +-104 the slopes are 0 and 1; a NaN in z stays one.
+template <class Slope> __device__ __forceinline__ void times_slope(const float* z, float* g, Slope slope) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float s = slope(__builtin_amdgcn_fmed3f(z[e], -104.0f, 104.0f));
+    g[e] *= z[e] != z[e] ? z[e] : s;
   }
-  return z0 != z0 ? z0 : r;
+}
+__device__ __forceinline__ void act_slopes(int act, const float* z, float* g) {
+  if (act == CCN_ACT_RELU) {
+    times_slope(z, g, [](float x) { return x > 0.0f ? 1.0f : 0.0f; });
+  } else if (act == CCN_ACT_GELU) {
+    times_slope(z, g, [](float x) {
+      float bell;
+      const float p = normal_cdf(x, &bell);
+      return fmaf(x * kInvSqrt2Pi, bell, p);
+    });
+  } else if (act == CCN_ACT_GELU_TANH) {
+    times_slope(z, g, [](float x) {
+      const float s = gelu_tanh_gate(x);
+      return fmaf(x * s * (1.0f - s) * (2.0f * kTanhC), fmaf(3.0f * kTanhA * x, x, 1.0f), s);
+    });
+  } else if (act == CCN_ACT_SILU) {
+    times_slope(z, g, [](float x) {
+      const float s = sigmoid(x);
+      return s * fmaf(x, 1.0f - s, 1.0f);
+    });
+  }
 }
 
 // ---- eight neighbouring elements of a row --------------------------------------------------------------------------------
@@ -802,24 +806,35 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
   }
 }
 
-// Adds the splits up in ascending order and finishes the output: eight columns of a row per thread.
+// Adds the splits of a product up and finishes the output.  2^shift lanes share a piece of eight columns: lane l adds the
+// splits l, l + 2^shift, ... in ascending order, then the lanes' sums are added pairwise (a fixed order for given sizes).
 template <bool F16, bool OUT32>
 __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __restrict__ partial, const int splits, const int rows,
-                                                             const int cols, const LinEpi ep) {
+                                                             const int cols, const int shift, const LinEpi ep) {
   const size_t ld = ((size_t)cols + 7) & ~(size_t)7, pieces = ld / 8;
-  const size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= pieces * (size_t)rows) return;
-  const size_t row = i / pieces, col = (i - row * pieces) * 8;
-  const float* p = partial + row * ld + col;
+  const size_t id = (size_t)blockIdx.x * kBlock + threadIdx.x, i = id >> shift;
+  const int lane = (int)(id & ((1u << shift) - 1u));
+  const bool live = i < pieces * (size_t)rows;
+  const size_t row = live ? i / pieces : 0, col = live ? (i - row * pieces) * 8 : 0;
+  const float* p = partial + ((size_t)lane * rows + row) * ld + col;
+  const size_t step = ((size_t)rows * ld) << shift;
   float v[8];
-  __builtin_memcpy(v, p, 32);
-  for (int s = 1; s < splits; s++) {
-    p += (size_t)rows * ld;
-    float x[8];
-    __builtin_memcpy(x, p, 32);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] += x[e];
+  for (int e = 0; e < 8; e++) v[e] = 0.0f;
+  if (live) {
+#pragma unroll 4
+    for (int s = lane; s < splits; s += 1 << shift) {
+      float x[8];
+      __builtin_memcpy(x, p, 32);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += x[e];
+      p += step;
+    }
   }
+  for (int k = 0; k < shift; k++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += __shfl_xor(v[e], 1 << k, kWave);
+  if (!live || lane) return;
   const int n = cols - (int)col;
   Bias8 bias;
   Old8<OUT32> old;
@@ -837,10 +852,11 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
 //                      8c .. 8c+7 and turns that 8 x 8 block over in registers: eight fragments of column 8c + j
 //   along (dX)         64 rows of W x 64 summed elements, fragments as they lie; row tiles are dealt so that a lane ends up
 //                      with eight neighbouring outputs
-// The four wavefronts of a workgroup take steps in turn and add up through LDS.  A strip whose sum is split over workgroups is
-// finished by the one that arrives last: partial sums go out and come back as relaxed agent-scope atomics (written through to
-// where the XCDs are coherent), complete (vmcnt 0) before the workgroup counts itself in; splits are added in ascending order
-// whoever does it.  The counter is back at zero when the call ends.
+// The four wavefronts of a workgroup take steps in turn and add up through LDS.  A strip whose sum is split over workgroups:
+// up to 16 rows, the workgroup that arrives last finishes it: partial sums go out and come back with the agent-scope bit (sc1:
+// written through to, and read from, where the XCDs are coherent), complete (vmcnt 0) before the workgroup counts itself in;
+// splits are added in ascending order whoever does it, and the counter is back at zero when the call ends.  With more rows one
+// workgroup would have too much to add (64 x 1024 x 1024: 17.9 us): the join kernel does it.
 constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16;
 template <bool ALONG> struct Few {
   static constexpr int kWidth = ALONG ? 64 : 128;   // outputs of a strip
@@ -853,24 +869,27 @@ struct FewArgs {
   size_t ldx, ldw;
   int rows, cols, sum;
   int per_split;        // a multiple of kStep
-  float* partial;       // [splits][strips][16*MT][kWidth]
+  float* partial;       // [splits][rows][cols rounded up to 8]
   uint32_t* counters;   // [strips], zero
 };
-__device__ __forceinline__ void store_through(float* p, const float* v) {
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    uint64_t x;
-    __builtin_memcpy(&x, v + 2 * e, 8);
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p) + e, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+constexpr int kAuxSc1 = 16;   // agent scope, in a gfx950 buffer instruction's cache policy
+struct Through {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ explicit Through(float* base) : rs(__builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7ffffffc, 0x00020000)) {}
+  __device__ __forceinline__ void store(uint32_t at, const float* v) const {
+    u32x4 lo, hi;
+    __builtin_memcpy(&lo, v, 16);
+    __builtin_memcpy(&hi, v + 4, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(lo, rs, at, 0, kAuxSc1);
+    __builtin_amdgcn_raw_buffer_store_b128(hi, rs, at + 16, 0, kAuxSc1);
   }
-}
-__device__ __forceinline__ void load_through(float* v, const float* p) {
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_memcpy(v + 2 * e, &x, 8);
+  __device__ __forceinline__ void load(float* v, uint32_t at) const {
+    const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, kAuxSc1));
+    const u32x4 hi = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 16, 0, kAuxSc1));
+    __builtin_memcpy(v, &lo, 16);
+    __builtin_memcpy(v + 4, &hi, 16);
   }
-}
+};
 template <bool F16> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -963,9 +982,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
   // along: 32*(T/2) + 8q + 4*(T%2) + i in acc[..][T][i]
   constexpr int kPieces = D::kWidth / 8;
   const int row = t / kPieces, piece = t % kPieces, col = n0 + 8 * piece, n = a.cols - col;
-  auto part = [&](int s, int m) {
-    return a.partial + ((((size_t)s * gridDim.x + strip) * MT + m) * 16 + row) * D::kWidth + 8 * piece;
-  };
+  const size_t ldp = ((size_t)a.cols + 7) & ~(size_t)7;
   auto finish = [&](float* v, int m) {
     if (n <= 0) return;
     const Places where = places<false>(ep, (size_t)(16 * m + row), (size_t)col, 0, 0, 0);
@@ -1000,42 +1017,50 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += x[e];
       }
-      if (splits == 1) finish(v, m);
-      else store_through(part(split, m), v);
+      if (splits == 1) {
+        finish(v, m);
+      } else if (n > 0) {
+        float* const at = a.partial + ((size_t)split * a.rows + 16 * m + row) * ldp + col;
+        if constexpr (MT == 1) Through(a.partial).store((uint32_t)((at - a.partial) * 4), v);
+        else __builtin_memcpy(at, v, 32);
+      }
     }
   }
-  if (splits == 1) return;
+  if (MT > 1 || splits == 1) return;
   __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wavefront's partial sums have arrived
   __syncthreads();
   if (t == 0) arrived = __hip_atomic_fetch_add(a.counters + strip, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (arrived != (uint32_t)splits - 1u) return;
   if (t == 0) __hip_atomic_store(a.counters + strip, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll 1
-  for (int m = 0; m < MT; m++) {
-    if (row < 16 && 16 * m + row < a.rows) {
-      float v[8];
-      load_through(v, part(0, m));
-#pragma unroll 4
-      for (int s = 1; s < splits; s++) {
-        float x[8];
-        load_through(x, part(s, m));
+  if (row < a.rows && n > 0) {
+    const Through through(a.partial);
+    const uint32_t at = (uint32_t)((row * ldp + col) * 4), step = (uint32_t)(a.rows * ldp * 4);
+    float x[kFewMaxSplits][8], v[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += x[e];
+    for (int s = 0; s < kFewMaxSplits; s++)
+      if (s < splits) through.load(x[s], at + s * step);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = x[0][e];
+#pragma unroll
+    for (int s = 1; s < kFewMaxSplits; s++)
+      if (s < splits) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += x[s][e];
       }
-      finish(v, m);
-    }
+    finish(v, 0);
   }
 }
 
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
 // dz = dY * act'(pre), rounded to the operands' type into the workspace (rows of N rounded up to 8, zeros in the rest),
-// and fp32 sums over a chunk of rows of the unrounded dz.  Four wavefronts walk a chunk's rows, 512 columns wide.
+// and fp32 sums over a chunk of rows of the unrounded dz.  Four wavefronts walk a chunk's rows, 512 columns wide, four rows in
+// flight each.  With one chunk the sums are db itself (`add`: added to it).
 template <bool F16>
 __global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __restrict__ dY, const size_t lddy,
                                                            const uint16_t* __restrict__ pre, const size_t ldp,
                                                            uint16_t* __restrict__ dz, const size_t lddz, float* __restrict__ sums,
-                                                           const int M, const int N, const int act, const int rows_per_chunk) {
+                                                           const int M, const int N, const int act, const int rows_per_chunk, const int add) {
   __shared__ float part[4][512 + 8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = (int)blockIdx.x * 512 + lane * 8, n = N - col;
@@ -1045,21 +1070,36 @@ __global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __res
 #pragma unroll
   for (int e = 0; e < 8; e++) s[e] = 0.0f;
   if (n > 0) {
-    for (int m = m0 + wave; m < m1; m += 4) {
-      float g[8];
-      unpack<F16>(load_piece(dY + (size_t)m * lddy + col, n), g);
-      if (act != CCN_ACT_NONE) {
-        float z[8];
-        unpack<F16>(load_piece(pre + (size_t)m * ldp + col, n), z);
+    constexpr int kRows = 4;   // rows in flight per wavefront
+    for (int m = m0 + wave; m < m1; m += 4 * kRows) {
+      u32x4 gv[kRows], zv[kRows];
 #pragma unroll
-        for (int e = 0; e < 8; e++) g[e] = e < n ? g[e] * act_slope(act, z[e]) : 0.0f;
-        if (dz) {
-          const u32x4 v = pack<F16>(g);
-          __builtin_memcpy(dz + (size_t)m * lddz + col, &v, 16);
+      for (int u = 0; u < kRows; u++) {
+        if (m + 4 * u < m1) {
+          gv[u] = load_piece(dY + (size_t)(m + 4 * u) * lddy + col, n);
+          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)(m + 4 * u) * ldp + col, n);
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) s[e] += g[e];
+      for (int u = 0; u < kRows; u++) {
+        if (m + 4 * u < m1) {
+          float g[8];
+          unpack<F16>(gv[u], g);
+          if (act != CCN_ACT_NONE) {
+            float z[8];
+            unpack<F16>(zv[u], z);
+            act_slopes(act, z, g);
+#pragma unroll
+            for (int e = 0; e < 8; e++) g[e] = e < n ? g[e] : 0.0f;
+          }
+          if (dz) {
+            const u32x4 v = pack<F16>(g);
+            __builtin_memcpy(dz + (size_t)(m + 4 * u) * lddz + col, &v, 16);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e++) s[e] += g[e];
+        }
+      }
     }
   }
   if (!sums) return;
@@ -1069,21 +1109,30 @@ __global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __res
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     const int c = threadIdx.x + 256 * h, at = (int)blockIdx.x * 512 + c;
-    if (at < N) sums[(size_t)blockIdx.y * N + at] = ((part[0][c] + part[1][c]) + part[2][c]) + part[3][c];
+    if (at < N) {
+      const float x = ((part[0][c] + part[1][c]) + part[2][c]) + part[3][c];
+      float* const o = sums + (size_t)blockIdx.y * N + at;
+      *o = add ? *o + x : x;
+    }
   }
 }
-// db[n] = (db[n] +) the sum of the chunks' sums: 64 columns per workgroup, each wavefront a quarter of the chunks.
-__global__ __launch_bounds__(kBlock) void linear_db_kernel(const float* __restrict__ sums, float* __restrict__ db, const int N,
-                                                           const int chunks, const int accumulate) {
-  __shared__ float part[4][kWave];
+// db[n] = (db[n] +) the sum of the chunks' sums: 64 columns per workgroup, each of 16 wavefronts every sixteenth chunk.
+constexpr int kDbWaves = 16;
+__global__ __launch_bounds__(kDbWaves * kWave) void linear_db_kernel(const float* __restrict__ sums, float* __restrict__ db, const int N,
+                                                                     const int chunks, const int accumulate) {
+  __shared__ float part[kDbWaves][kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * kWave + lane;
   float s = 0.0f;
-  if (c < N)
-    for (int k = wave; k < chunks; k += 4) s += sums[(size_t)k * N + c];
+  if (c < N) {
+#pragma unroll 8
+    for (int k = wave; k < chunks; k += kDbWaves) s += sums[(size_t)k * N + c];
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < N) {
-    const float x = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+    float x = part[0][lane];
+#pragma unroll
+    for (int w = 1; w < kDbWaves; w++) x += part[w][lane];
     db[c] = accumulate ? db[c] + x : x;
   }
 }
@@ -1141,10 +1190,13 @@ int launch_ring(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) 
   return CCN_OK;
 }
 template <bool F16, bool OUT32>
-int launch_join(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) {
-  const size_t threads = (size_t)pr.rows * (((size_t)pr.cols + 7) / 8);
-  hipLaunchKernelGGL((linear_join_kernel<F16, OUT32>), dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock), 0, s, pr.partial, splits,
-                     pr.rows, pr.cols, ep);
+int launch_join(const float* partial, int rows, int cols, int splits, const LinEpi& ep, hipStream_t s) {
+  const size_t pieces = (size_t)rows * (((size_t)cols + 7) / 8);
+  int shift = 0;   // lanes per piece: until there are 2^16 threads
+  while (shift < 4 && (2 << shift) <= splits && (pieces << shift) < 65536) shift++;
+  const size_t blocks = ((pieces << shift) + kBlock - 1) / kBlock;
+  if (blocks > 0x7fffffffull) return CCN_ERANGE;
+  hipLaunchKernelGGL((linear_join_kernel<F16, OUT32>), dim3((unsigned)blocks), dim3(kBlock), 0, s, partial, splits, rows, cols, shift, ep);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
@@ -1155,7 +1207,7 @@ int product_ring(LinProd& pr, const LinEpi& ep, bool out32, bool whole, int spli
   if constexpr (FR * FC < 16) {
     if (splits > 1) {
       CCN_TRY((launch_ring<F16, PA, QA, FR, FC, kOutPartial, true>(pr, ep, splits, s)));
-      return out32 ? launch_join<F16, true>(pr, ep, splits, s) : launch_join<F16, false>(pr, ep, splits, s);
+      return out32 ? launch_join<F16, true>(pr.partial, pr.rows, pr.cols, splits, ep, s) : launch_join<F16, false>(pr.partial, pr.rows, pr.cols, splits, ep, s);
     }
   }
   if (out32) {
@@ -1183,16 +1235,17 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   a.rows = rows;
   a.cols = cols;
   a.sum = sum;
-  a.partial = plan->partial;
   a.counters = plan->counters;
   const int strips = (cols + D::kWidth - 1) / D::kWidth, steps = (sum + D::kStep - 1) / D::kStep;
   // a workgroup for every CU, each wavefront with a step at least
   int splits = (cus + strips - 1) / strips;
   if (splits > steps / kFewWaves) splits = steps / kFewWaves;
+  if ((size_t)splits * (size_t)rows * (size_t)(cols + 7) > ((size_t)1 << 28)) splits = 1;   // 32-bit offsets into the partial sums
   if (splits > kFewMaxSplits) splits = kFewMaxSplits;
   if (splits < 1) splits = 1;
   a.per_split = ((steps + splits - 1) / splits) * D::kStep;
   splits = (sum + a.per_split - 1) / a.per_split;   // no empty split
+  a.partial = plan->partial;
   const dim3 grid((unsigned)strips, (unsigned)splits), block(kFewWaves * kWave);
   switch ((rows + 15) / 16) {
     case 1: hipLaunchKernelGGL((linear_few_kernel<F16, 1, ALONG>), grid, block, 0, s, a, ep); break;
@@ -1201,6 +1254,7 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
     default: hipLaunchKernelGGL((linear_few_kernel<F16, 4, ALONG>), grid, block, 0, s, a, ep); break;
   }
   CCN_HIP(hipGetLastError());
+  if (rows > 16 && splits > 1) return launch_join<F16, false>(a.partial, rows, cols, splits, ep, s);
   return CCN_OK;
 }
 
@@ -1246,7 +1300,7 @@ int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, int read_r, co
   if (splits > 1) {
     hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOutPartial>), grid, block, 0, s, pr, ep);
     CCN_HIP(hipGetLastError());
-    return out32 ? launch_join<F16, true>(pr, ep, splits, s) : launch_join<F16, false>(pr, ep, splits, s);
+    return out32 ? launch_join<F16, true>(pr.partial, pr.rows, pr.cols, splits, ep, s) : launch_join<F16, false>(pr.partial, pr.rows, pr.cols, splits, ep, s);
   }
   if (out32) {
     if constexpr (!PA && !QA) hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut32>), grid, block, 0, s, pr, ep);
@@ -1314,19 +1368,24 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const bool want_dz = act != CCN_ACT_NONE && (dX || dW);
   const size_t lddz = ((size_t)plan->max_n + 7) & ~(size_t)7;
   int chunks = 0;
+  bool done = false;   // db is there
   if (M > 0 && (want_dz || db)) {
     const int strips = (N + 511) / 512;
-    // rows per chunk: enough workgroups for the whole chip, at least four rows for each wavefront
+    // rows per chunk: four workgroups for every CU, at least one row for each wavefront; up to 32 rows one chunk, which needs no
+    // second kernel
     int per = (int)(((size_t)M * strips + 4 * (size_t)di->cu_count - 1) / (4 * (size_t)di->cu_count));
-    if (per < 16) per = 16;
+    if (per < 4) per = 4;
     if ((M + per - 1) / per > kMaxChunks) per = (M + kMaxChunks - 1) / kMaxChunks;
+    if (M <= 32) per = M;
     chunks = (M + per - 1) / per;
+    done = chunks == 1;
+    float* const sums = !db ? nullptr : done ? db : plan->sums;
     hipLaunchKernelGGL((linear_dz_kernel<F16>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp,
-                       want_dz ? plan->dz : nullptr, lddz, db ? plan->sums : nullptr, M, N, act, per);
+                       want_dz ? plan->dz : nullptr, lddz, sums, M, N, act, per, done ? accumulate : 0);
     CCN_HIP(hipGetLastError());
   }
-  if (db) {
-    hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kBlock), 0, s, plan->sums, db, N, chunks, accumulate);
+  if (db && !done) {
+    hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kDbWaves * kWave), 0, s, plan->sums, db, N, chunks, accumulate);
     CCN_HIP(hipGetLastError());
   }
   const uint16_t* const g = act != CCN_ACT_NONE ? plan->dz : dY;
