@@ -10,6 +10,7 @@
 // 16-byte reads, an "across" tile through the transposing ds_read_b64_tr_b16.
 #include "ccn_common.hpp"
 
+#include <cmath>
 #include <new>
 #include <type_traits>
 
@@ -244,6 +245,8 @@ __device__ __forceinline__ void tile_of(uint32_t b, int tiles_r, int tiles_c, in
   tc = (int)(in / h);
 }
 
+enum { kOut16 = 0, kOut32 = 1, kOutPartial = 2 };   // what a tile leaves: a 16-bit or an fp32 output, or a split's fp32 sums
+
 struct LinProd {
   const uint16_t* p;   // row operand
   const uint16_t* q;   // column operand
@@ -251,184 +254,13 @@ struct LinProd {
   int rows, cols, sum;
   int read_r, read_c;  // rows or columns of the operands that may be read: rows, cols, or for an "across" operand that many rounded up to 8
   int tiles_r, tiles_c;
-  int per_split;       // summed elements per split (a multiple of kGK)
+  int per_split;       // summed elements per split (a multiple of 64)
   float* partial;      // [splits][rows][cols rounded up to 8] when splits > 1
-};
-
-// ---- any shape, any alignment -----------------------------------------------------------------------------------------
-// 128 x 128 tiles, 64 summed elements per step, four wavefronts of 64 x 64 (2 x 2 blocks of v_mfma_f32_32x32x16).  The
-// pieces of step k+1 travel from memory to registers while step k is multiplied from LDS.  Tiles at the edge read the
-// last row again instead of one behind it (its results are not stored); pieces that cross the end of a row, and steps
-// that cross the end of the sum, are filled with zeros, on both operands (0 * inf would not be 0).
-constexpr int kGT = 128, kGK = 64;
-constexpr int kGTile = kGT * kGK * 2;      // bytes of one operand's step
-constexpr int kGCStride = 64 + 4;          // floats per row of a wavefront's 32 x 64 piece of the output
-constexpr int kGLds = (2 * kGTile > 4 * 32 * kGCStride * 4) ? 2 * kGTile : 4 * 32 * kGCStride * 4;
-
-enum { kOut16 = 0, kOut32 = 1, kOutPartial = 2 };
-
-template <bool ALONG> struct GSide {
-  // thread t stages pieces j = 0..3: along: row t/8 + 32j, piece t%8 of the step;  across: step row t/16 + 16j, piece t%16
-  const uint16_t* base[4];
-  int edge;   // across: valid elements of this thread's piece
-  __device__ __forceinline__ void init(const uint16_t* p, size_t ld, int o0, int outer, int t) {
-    if constexpr (ALONG) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int r = o0 + (t >> 3) + 32 * j;
-        base[j] = p + (size_t)(r < outer ? r : outer - 1) * ld + 8 * (t & 7);
-      }
-      edge = 8;
-    } else {
-      const int c = o0 + 8 * (t & 15);
-#pragma unroll
-      for (int j = 0; j < 4; j++) base[j] = p + (size_t)((t >> 4) + 16 * j) * ld + c;
-      edge = outer - c;
-    }
-  }
-  __device__ __forceinline__ void fetch(u32x4* v, size_t ld, int k, int sum, int t, bool whole) const {
-    const size_t off = ALONG ? (size_t)k : (size_t)k * ld;
-    if (whole) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) __builtin_memcpy(&v[j], base[j] + off, 16);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int n = ALONG ? sum - k - 8 * (t & 7) : (k + (t >> 4) + 16 * j < sum ? edge : 0);
-        v[j] = load_piece(base[j] + off, n);
-      }
-    }
-  }
-  static __device__ __forceinline__ int swz(int row) { return (row & 7) ^ ((row >> 3) & 7); }
-  static __device__ __forceinline__ void put(uint8_t* lds, const u32x4* v, int t) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if constexpr (ALONG) {
-        const int row = (t >> 3) + 32 * j;
-        *reinterpret_cast<u32x4*>(lds + row * 128 + (((t & 7) ^ swz(row)) << 4)) = v[j];
-      } else {
-        const int k = (t >> 4) + 16 * j;
-        *reinterpret_cast<u32x4*>(lds + k * 256 + (((t & 15) ^ (4 * (k & 3))) << 4)) = v[j];
-      }
-    }
-  }
-  // fragment f (32 rows or columns), summed elements 16*ks + 8*(lane/32) .. +7 of row or column 32*f + lane%32
-  static __device__ __forceinline__ s16x8 frag(const uint8_t* lds, int f, int ks, int lane) {
-    const int li = lane & 31, lh = lane >> 5;
-    if constexpr (ALONG) {
-      const int row = 32 * f + li;
-      return *reinterpret_cast<const s16x8*>(lds + row * 128 + (((2 * ks + lh) ^ swz(row)) << 4));
-    } else {
-      const int a16 = lane & 15, g2 = (lane >> 4) & 1;
-      const int at = ((lh * 8 + (a16 >> 2)) * 16 + ((2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2)))) * 16 + 8 * (a16 & 1);
-      const uint8_t* p = lds + (at ^ (f * 64)) + ks * 4096;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 1024));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  }
 };
 
 template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <bool F16, bool PA, bool QA, int OUT>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 4)))
-void linear_tile128_kernel(const LinProd pr, const LinEpi ep) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kGLds];
-  uint8_t* const lp = lds;
-  uint8_t* const lq = lds + kGTile;
-  int tr, tc;
-  tile_of(blockIdx.x, pr.tiles_r, pr.tiles_c, tr, tc);
-  const int r0 = tr * kGT, c0 = tc * kGT;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wr = wave >> 1, wc = wave & 1, li = lane & 31, lh = lane >> 5;
-  const int k_begin = (int)blockIdx.y * pr.per_split;
-  const int k_end = pr.sum - k_begin < pr.per_split ? pr.sum : k_begin + pr.per_split;
-  const bool pin = PA || r0 + kGT <= pr.rows, qin = QA || c0 + kGT <= pr.cols;
-
-  GSide<PA> sp;
-  GSide<QA> sq;
-  sp.init(pr.p, pr.ldp, r0, pr.rows, t);
-  sq.init(pr.q, pr.ldq, c0, pr.cols, t);
-  f32x16 acc[2][2];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
-#pragma unroll
-  for (int a = 0; a < 2; a++)
-#pragma unroll
-    for (int b = 0; b < 2; b++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) acc[a][b][i] = 0.0f;
-
-  u32x4 vp[4], vq[4];
-  auto fetch = [&](int k) {
-    const bool whole = k + kGK <= k_end;
-    sp.fetch(vp, pr.ldp, k, k_end, t, whole && pin);
-    sq.fetch(vq, pr.ldq, k, k_end, t, whole && qin);
-  };
-  if (k_begin < k_end) fetch(k_begin);
-  for (int k = k_begin; k < k_end; k += kGK) {
-    __syncthreads();   // everybody has read the step before
-    GSide<PA>::put(lp, vp, t);
-    GSide<QA>::put(lq, vq, t);
-    if (k + kGK < k_end) fetch(k + kGK);
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 4; ks++) {
-      s16x8 fp[2], fq[2];
-#pragma unroll
-      for (int f = 0; f < 2; f++) {
-        fq[f] = GSide<QA>::frag(lq, 2 * wc + f, ks, lane);
-        fp[f] = GSide<PA>::frag(lp, 2 * wr + f, ks, lane);
-      }
-#pragma unroll
-      for (int a = 0; a < 2; a++)
-#pragma unroll
-        for (int b = 0; b < 2; b++) acc[a][b] = mfma32<F16>(fq[a], fp[b], acc[a][b]);
-    }
-  }
-  __syncthreads();   // LDS becomes four private pieces of the output
-  float* const cw = reinterpret_cast<float*>(lds) + wave * (32 * kGCStride);
-  const int r8 = lane >> 3, c8 = lane & 7;
-  const int col = c0 + 64 * wc + 8 * c8, n = pr.cols - col;
-  const int row0 = r0 + 64 * wr + r8;   // piece i of 8 is row row0 + 8*i
-  const int pieces = n > 0 ? (pr.rows - row0 + 7) >> 3 : 0;   // those inside the matrix
-  const Places where = places<OUT == kOut32>(ep, (size_t)(r0 + 64 * wr), (size_t)(c0 + 64 * wc), r8, 8 * c8, 8);
-  Bias8 bias;
-  if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)col, n);
-#pragma unroll
-  for (int b = 0; b < 2; b++) {
-    Old8<OUT == kOut32> old[4];
-    if constexpr (OUT != kOutPartial) {
-#pragma unroll
-      for (int s = 0; s < 4; s++)
-        if (4 * b + s < pieces) load_old<OUT == kOut32>(old[s], ep, where, 4 * b + s, n);
-    }
-#pragma unroll
-    for (int a = 0; a < 2; a++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const f32x4 v = {acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
-        *reinterpret_cast<f32x4*>(cw + li * kGCStride + 32 * a + 8 * i + 4 * lh) = v;
-      }
-    __builtin_amdgcn_wave_barrier();   // a wavefront's LDS operations complete in order
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      float v[8];
-      __builtin_memcpy(v, cw + (8 * s + r8) * kGCStride + 8 * c8, 32);
-      if (4 * b + s < pieces) {
-        if constexpr (OUT == kOutPartial) {
-          const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
-          float* const o = pr.partial + ((size_t)blockIdx.y * pr.rows + row0 + 8 * (4 * b + s)) * ld + col;
-          __builtin_memcpy(o, v, 32);
-        } else {
-          finish8<F16, OUT == kOut32>(v, bias, old[s], ep, where, 4 * b + s, n);
-        }
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
 }
 
 // ---- 16-byte aligned operands: tiles on a ring of direct-to-LDS stages -------------------------------------------------------
@@ -844,6 +676,36 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
   finish8<F16, OUT32>(v, bias, old, ep, where, 0, n);
 }
 
+// ---- operands whose rows are not made of aligned 16-byte pieces --------------------------------------------------------------
+// A copy with aligned rows, zeros behind each row's end: the ring then runs on it.  It costs a launch and two passes over the
+// operand at the memory's rate, less than matrix instructions fed from unaligned loads through registers lose at any size (129 x
+// 129 x 129: 11.1 instead of 11.8 us, 777 x 1537 x 2049: 27 instead of 57, 2049 x 2049 x 2049: 54 instead of 90).
+struct PackJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  size_t ld, ldd;   // ldd: a multiple of 8
+  int rows, cols;
+};
+constexpr int kPackRows = 16;
+__global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, const PackJob b) {
+  const PackJob& job = blockIdx.z ? b : a;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = ((int)blockIdx.x * kWave + lane) * 8;
+  if (col >= job.cols) return;
+  for (int r0 = (int)blockIdx.y * kPackRows; r0 < job.rows; r0 += (int)gridDim.y * kPackRows) {
+    u32x4 v[kPackRows / 4];
+#pragma unroll
+    for (int u = 0; u < kPackRows / 4; u++) {
+      const int r = r0 + 4 * u + wave;
+      if (r < job.rows) v[u] = load_piece(job.src + (size_t)r * job.ld + col, job.cols - col);
+    }
+#pragma unroll
+    for (int u = 0; u < kPackRows / 4; u++) {
+      const int r = r0 + 4 * u + wave;
+      if (r < job.rows) *reinterpret_cast<u32x4*>(job.dst + (size_t)r * job.ldd + col) = v[u];
+    }
+  }
+}
+
 // ---- few rows: the weights are read once, at the memory's rate ---------------------------------------------------------------
 // Up to 64 rows (16*MT): what counts is reading W, and every wavefront keeps 8 KiB of it in flight beside the 8 KiB it works on.
 // W goes from memory to registers and from there into v_mfma_f32_16x16x32, whose row operand it is; X (16 rows of it per
@@ -1139,7 +1001,7 @@ __global__ __launch_bounds__(kDbWaves * kWave) void linear_db_kernel(const float
 
 constexpr size_t kMaxLd = (size_t)1 << 22;
 constexpr int kMaxChunks = 256;      // row chunks of the column sums
-constexpr size_t kMaxSplitTiles = 1024;   // tiles x splits of a split product, which bounds the partial sums' workspace
+constexpr int kMaxSplits = 16;
 
 #define CCN_TRY(expr)                  \
   do {                                 \
@@ -1147,6 +1009,7 @@ constexpr size_t kMaxSplitTiles = 1024;   // tiles x splits of a split product, 
     if (_rc != CCN_OK) return _rc;     \
   } while (0)
 
+inline size_t round8(size_t n) { return (n + 7) & ~(size_t)7; }
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -1158,6 +1021,8 @@ struct ccn_linear_plan {
   int device = -1;
   int max_m = 0, max_n = 0, max_k = 0;
   uint16_t* dz = nullptr;
+  uint16_t* px = nullptr;    // aligned copies of X and W
+  uint16_t* pw = nullptr;
   float* sums = nullptr;
   float* partial = nullptr;
   size_t partial_floats = 0;
@@ -1166,14 +1031,15 @@ struct ccn_linear_plan {
 
 namespace {
 
-// How often a product is split along its sum: few tiles leave CUs idle; a split has at least two steps.
-int splits_for(int tiles, int sum, int cus) {
-  if (tiles >= cus || sum < 4 * kGK) return 1;
-  int s = (2 * cus) / tiles;
-  const int most = sum / (2 * kGK);
-  if (s > most) s = most;
-  if ((size_t)s * (size_t)tiles > kMaxSplitTiles) s = (int)(kMaxSplitTiles / (size_t)tiles);
-  return s < 1 ? 1 : s;
+// A 16-bit matrix as the products take it.  extent: columns that may be read (its width, or that rounded up to 8).
+struct Operand {
+  const uint16_t* p;
+  size_t ld;
+  int rows, extent;
+};
+// Whether the ring can fetch it: aligned 16-byte pieces, and as a sum's rows ("across") only whole ones.
+bool ring_fetches(const Operand& o, bool along) {
+  return aligned16(o.p) && o.ld % 8 == 0 && o.ld <= kRMaxLd && (along || o.extent % 8 == 0);
 }
 
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
@@ -1258,56 +1124,79 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   return CCN_OK;
 }
 
-// One product.  read_r, read_c: see LinProd.
+// How a product runs on the ring, by estimated time.  Measured in us (4096 x 4096 x 4096 and smaller): a step of 64 summed
+// elements takes a CU 0.42 with one 128 x 128 tile on it, 1.06 with two, 1.6 with a 256 x 256 tile; 3.5 or 8 go into the first
+// loads and the output; a split adds 1.8 for the join kernel and 0.4 per MB of partial sums, written and read.
+//   rows x sum x cols        256 x 256    128 x 128, splits 1 / 2 / 4 / 8
+//   256 x 4096 x 4096        74.1         33.0 / 23.6 / 21.7 / 27.3
+//   1024 x 8192 x 1024       132.8        54.1 / 35.7 / 28.9 / 34.8
+//   1024 x 1024 x 1024       30.2         12.2 / 13.1 / 15.1 / 20.5
+//   2048 x 4096 x 4096       77.7         71.2 / 110.7
+//   4096 x 4096 x 4096       110.9        134.2
+struct RingPlan {
+  bool large;
+  int splits;
+};
+RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus) {
+  const auto tiles = [&](int edge) { return (double)((rows + edge - 1) / edge) * (double)((cols + edge - 1) / edge); };
+  const double steps = (double)((sum + 63) / 64), t128 = tiles(128), t256 = tiles(256);
+  const size_t each = (size_t)rows * round8((size_t)cols);
+  RingPlan best{true, 1};
+  double least = 8.0 + 1.6 * steps * std::ceil(t256 / cus);
+  for (int s = 1; s <= kMaxSplits; s++) {
+    if (s > 1 && (s * 2.0 > steps || (double)s * t128 > 2.0 * cus || (size_t)s * each > partial_floats)) break;
+    const double deep = std::ceil(s * t128 / cus);
+    double t = 3.5 + std::ceil(steps / s) * (deep < 2.0 ? 0.42 : 0.53 * deep);
+    if (s > 1) t += 1.8 + 0.4e-6 * 4.0 * (double)s * (double)each;
+    if (t < least) {
+      least = t;
+      best = RingPlan{false, s};
+    }
+  }
+  return best;
+}
+
+// One product of operands that the ring can fetch: C [rows x cols].
 template <bool F16, bool PA, bool QA>
-int product(ccn_linear_plan* plan, const uint16_t* p, size_t ldp, int read_r, const uint16_t* q, size_t ldq, int read_c, int rows, int cols,
-            int sum, const LinEpi& ep, bool out32, int cus, hipStream_t s) {
+int product(ccn_linear_plan* plan, const Operand& p, const Operand& q, int rows, int cols, int sum, const LinEpi& ep, bool out32, int cus,
+            hipStream_t s) {
   LinProd pr;
-  pr.p = p;
-  pr.q = q;
-  pr.ldp = ldp;
-  pr.ldq = ldq;
+  pr.p = p.p;
+  pr.q = q.p;
+  pr.ldp = p.ld;
+  pr.ldq = q.ld;
   pr.rows = rows;
   pr.cols = cols;
   pr.sum = sum;
-  pr.read_r = read_r;
-  pr.read_c = read_c;
+  pr.read_r = PA ? rows : p.extent;
+  pr.read_c = QA ? cols : q.extent;
   pr.partial = plan->partial;
-  const auto tiles = [&](int edge) { return (size_t)((rows + edge - 1) / edge) * (size_t)((cols + edge - 1) / edge); };
-  if (tiles(128) > 0x7fffffffull) return CCN_ERANGE;
-  const auto aligned = [](const void* x, size_t ld, int size) {
+  if ((size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128) > 0x7fffffffull) return CCN_ERANGE;
+  const auto whole_rows = [](const void* x, size_t ld, int size) {
     return aligned16(x) && ld % (size_t)(16 / size) == 0 && ld * (size_t)size <= 2 * kRMaxLd;
   };
-  // how the sum is split when there are few tiles of 128 x 128
-  int splits = splits_for((int)tiles(128), sum, cus);
-  const size_t each = (size_t)rows * (((size_t)cols + 7) & ~(size_t)7);
-  if ((size_t)splits * each > plan->partial_floats) splits = (int)(plan->partial_floats / each);
-  if (splits < 2) splits = 1;
-  const int steps = (sum + kGK - 1) / kGK;
-  pr.per_split = ((steps + splits - 1) / splits) * kGK;
-  if (splits > 1) splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
-  if (pr.per_split < kGK) pr.per_split = kGK;
-  if (aligned(p, ldp, 2) && aligned(q, ldq, 2) && (PA || read_r % 8 == 0) && (QA || read_c % 8 == 0)) {
-    const bool whole = cols % 8 == 0 && aligned(ep.out, ep.ldo, out32 ? 4 : 2) && (!ep.resid || aligned(ep.resid, ep.ldr, 2)) &&
-                       (!ep.pre || aligned(ep.pre, ep.ldp, 2));
-    // large tiles where they occupy half of the CUs at least
-    if (2 * tiles(256) >= (size_t)cus && sum >= 4 * kRK) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
-    return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, splits, s);
+  const bool whole = cols % 8 == 0 && whole_rows(ep.out, ep.ldo, out32 ? 4 : 2) && (!ep.resid || whole_rows(ep.resid, ep.ldr, 2)) &&
+                     (!ep.pre || whole_rows(ep.pre, ep.ldp, 2));
+  RingPlan how = choose_ring(rows, cols, sum, plan->partial_floats, cus);
+  const int steps = (sum + 63) / 64;
+  pr.per_split = 64 * ((steps + how.splits - 1) / how.splits);
+  if (how.splits > 1) how.splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
+  if (how.large) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
+  return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, how.splits, s);
+}
+
+// Aligned copies of up to two operands into the plan (nullptr: none).
+int pack(const Operand* a, int a_cols, uint16_t* a_to, const Operand* b, int b_cols, uint16_t* b_to, hipStream_t s) {
+  const auto job = [](const Operand* o, int cols, uint16_t* to) { return o ? PackJob{o->p, to, o->ld, round8((size_t)cols), o->rows, cols} : PackJob{}; };
+  PackJob x = job(a, a_cols, a_to), y = job(b, b_cols, b_to);
+  if (!a) {
+    x = y;
+    y = PackJob{};
   }
-  pr.tiles_r = (rows + kGT - 1) / kGT;
-  pr.tiles_c = (cols + kGT - 1) / kGT;
-  const dim3 grid((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits), block(kBlock);
-  if (splits > 1) {
-    hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOutPartial>), grid, block, 0, s, pr, ep);
-    CCN_HIP(hipGetLastError());
-    return out32 ? launch_join<F16, true>(pr.partial, pr.rows, pr.cols, splits, ep, s) : launch_join<F16, false>(pr.partial, pr.rows, pr.cols, splits, ep, s);
-  }
-  if (out32) {
-    if constexpr (!PA && !QA) hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut32>), grid, block, 0, s, pr, ep);
-    else return CCN_EINVAL;
-  } else {
-    hipLaunchKernelGGL((linear_tile128_kernel<F16, PA, QA, kOut16>), grid, block, 0, s, pr, ep);
-  }
+  const int cols = x.cols > y.cols ? x.cols : y.cols, rows = x.rows > y.rows ? x.rows : y.rows;
+  const int gy = (rows + kPackRows - 1) / kPackRows;
+  const dim3 grid((unsigned)((cols + 511) / 512), (unsigned)(gy < 65535 ? gy : 65535), a && b ? 2u : 1u);
+  hipLaunchKernelGGL(linear_pack_kernel, grid, dim3(kBlock), 0, s, x, y);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
@@ -1339,8 +1228,16 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   if (pre) CCN_TRY(check16(pre, ldp, N));
   if (!aligned4(bias)) return CCN_EINVAL;
   const LinEpi ep{bias, resid, pre, Y, ldr, ldp, ldy, act, 0};
-  if (M <= kFewRows) return product_few<F16, false>(plan, X, ldx, W, ldw, M, N, K, ep, di->cu_count, as_stream(stream));
-  return product<F16, true, false>(plan, X, ldx, M, W, ldw, N, M, N, K, ep, false, di->cu_count, as_stream(stream));
+  hipStream_t s = as_stream(stream);
+  if (M <= kFewRows) return product_few<F16, false>(plan, X, ldx, W, ldw, M, N, K, ep, di->cu_count, s);
+  Operand x{X, ldx, M, K}, w{W, ldw, K, N};
+  const bool cx = !ring_fetches(x, true), cw = !ring_fetches(w, false);
+  if (cx || cw) {
+    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
+    if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
+    if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
+  }
+  return product<F16, true, false>(plan, x, w, M, N, K, ep, false, di->cu_count, s);
 }
 
 template <bool F16>
@@ -1365,8 +1262,11 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
     if (dW) CCN_TRY(check16(X, ldx, K));
   }
   hipStream_t s = as_stream(stream);
-  const bool want_dz = act != CCN_ACT_NONE && (dX || dW);
-  const size_t lddz = ((size_t)plan->max_n + 7) & ~(size_t)7;
+  // dz goes to the workspace when there is an activation, and when dY is not laid out as the ring wants it
+  Operand g{dY, lddy, M, N};
+  const bool few = M <= kFewRows;   // dX by the kernel for few rows, which takes anything
+  const bool want_dz = M > 0 && (act != CCN_ACT_NONE ? dX || dW : (dW && !ring_fetches(g, false)) || (dX && !few && !ring_fetches(g, true)));
+  if (want_dz) g = Operand{plan->dz, round8((size_t)plan->max_n), M, (int)round8((size_t)N)};
   int chunks = 0;
   bool done = false;   // db is there
   if (M > 0 && (want_dz || db)) {
@@ -1381,24 +1281,28 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
     done = chunks == 1;
     float* const sums = !db ? nullptr : done ? db : plan->sums;
     hipLaunchKernelGGL((linear_dz_kernel<F16>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp,
-                       want_dz ? plan->dz : nullptr, lddz, sums, M, N, act, per, done ? accumulate : 0);
+                       want_dz ? plan->dz : nullptr, g.ld, sums, M, N, act, per, done ? accumulate : 0);
     CCN_HIP(hipGetLastError());
   }
   if (db && !done) {
     hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kDbWaves * kWave), 0, s, plan->sums, db, N, chunks, accumulate);
     CCN_HIP(hipGetLastError());
   }
-  const uint16_t* const g = act != CCN_ACT_NONE ? plan->dz : dY;
-  const size_t ldg = act != CCN_ACT_NONE ? lddz : lddy;
+  // operands that the ring cannot fetch: W along its rows for dX, X and dz across them for dW
+  Operand x{X, ldx, M, K}, w{W, ldw, K, N};
+  const bool cw = dX && !few && !ring_fetches(w, true), cx = dW && M > 0 && !ring_fetches(x, false);
+  const LinEpi dx_ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
+  const LinEpi dw_ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
+  if (cw || cx) {
+    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
+    if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
+    if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
+  }
   if (dX && M > 0) {
-    const LinEpi ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
-    if (M <= kFewRows) CCN_TRY((product_few<F16, true>(plan, g, ldg, W, ldw, M, K, N, ep, di->cu_count, s)));
-    else CCN_TRY((product<F16, true, true>(plan, g, ldg, M, W, ldw, K, M, K, N, ep, false, di->cu_count, s)));
+    if (few) CCN_TRY((product_few<F16, true>(plan, g.p, g.ld, W, ldw, M, K, N, dx_ep, di->cu_count, s)));
+    else CCN_TRY((product<F16, true, true>(plan, g, w, M, K, N, dx_ep, false, di->cu_count, s)));
   }
-  if (dW) {
-    const LinEpi ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
-    CCN_TRY((product<F16, false, false>(plan, X, ldx, K, g, ldg, g == plan->dz ? (N + 7) & ~7 : N, K, N, M, ep, dw32, di->cu_count, s)));
-  }
+  if (dW) CCN_TRY((product<F16, false, false>(plan, x, g, K, N, M, dw_ep, dw32, di->cu_count, s)));
   return CCN_OK;
 }
 
@@ -1410,6 +1314,8 @@ int ccn_linear_plan_destroy(ccn_linear_plan* plan) {
   if (!plan) return CCN_OK;
   int rc = CCN_OK;
   if (plan->dz && hipFree(plan->dz) != hipSuccess) rc = CCN_EHIP;
+  if (plan->px && hipFree(plan->px) != hipSuccess) rc = CCN_EHIP;
+  if (plan->pw && hipFree(plan->pw) != hipSuccess) rc = CCN_EHIP;
   if (plan->sums && hipFree(plan->sums) != hipSuccess) rc = CCN_EHIP;
   if (plan->partial && hipFree(plan->partial) != hipSuccess) rc = CCN_EHIP;
   if (plan->counters && hipFree(plan->counters) != hipSuccess) rc = CCN_EHIP;
@@ -1430,11 +1336,11 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   p->max_m = max_M;
   p->max_n = max_N;
   p->max_k = max_K;
-  // a split product has at most kMaxSplitTiles tiles x splits, and a split at least two steps
-  auto floats = [](int rows, int cols, int sum) {
-    const size_t tiles = (size_t)((rows + kGT - 1) / kGT) * (size_t)((cols + kGT - 1) / kGT);
-    const size_t most = tiles * (size_t)(sum / (2 * kGK) + 1);
-    return (most < kMaxSplitTiles ? most : kMaxSplitTiles) * (size_t)(kGT * kGT);
+  // A split product has at most two 128 x 128 tiles on every CU, over all its splits, and two steps of 64 in each split.
+  auto floats = [&](int rows, int cols, int sum) {
+    const size_t tiles = (size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128);
+    const size_t most = tiles * (size_t)(sum / 128 + 1), cap = 2 * (size_t)di->cu_count;
+    return (most < cap ? most : cap) * (size_t)(128 * 128);
   };
   const size_t need[3] = {floats(max_M, max_N, max_K), floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
   for (const size_t f : need) p->partial_floats = f > p->partial_floats ? f : p->partial_floats;
@@ -1442,8 +1348,9 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t few = (size_t)kFewMaxSplits * few_cols * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
   p->partial_floats = few > p->partial_floats ? few : p->partial_floats;
   const size_t strips = few_cols / 64;
-  const size_t lddz = ((size_t)max_N + 7) & ~(size_t)7;
-  hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * lddz * sizeof(uint16_t));
+  hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * round8((size_t)max_N) * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * round8((size_t)max_K) * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, (size_t)max_K * round8((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->counters, strips * sizeof(uint32_t));
