@@ -265,22 +265,27 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f
 
 // ---- 16-byte aligned operands: tiles on a ring of direct-to-LDS stages -------------------------------------------------------
 // A 256-thread workgroup owns a tile of (64*FR) x (64*FC), its four wavefronts a quarter each, FR x FC blocks of 32 x 32.
-// The operands travel from memory to LDS directly, into a ring of four stages of 32 summed elements; requests of 1 KiB are
+// The operands travel from memory to LDS directly, into a ring of four stages of RK summed elements; requests of 1 KiB are
 // spread between the matrix instructions, and one is waited for three steps after it was made.  An "along" stage holds rows
-// of 64 bytes, the 16-byte pieces swizzled by (row/4)%4; an "across" stage 32 rows as in memory, swizzled by 4*(k%4).  Tiles
-// at the edge read the last row or the last 8 columns again (results not stored); a sum that is no multiple of 32 ends with
-// a step loaded through registers with zeros behind the end.
-//   4 x 4   256 x 256, one wavefront per SIMD (256 accumulators each, in the accumulation half of the register file), one
-//           workgroup per CU: per 16 summed elements a wavefront reads eight fragments for sixteen matrix instructions
-//   2 x 2   128 x 128, two workgroups per CU: four fragments for four matrix instructions, for outputs of few large tiles
-constexpr int kRK = 32;                      // summed elements per stage
+// of 2*RK bytes, the 16-byte pieces swizzled so that the 32 rows of a fragment meet no bank twice; an "across" stage RK rows as
+// in memory, swizzled by 4*(k%4).  Tiles at the edge read the last row or the last 8 columns again (results not stored); a
+// sum that is no multiple of RK ends with a step loaded through registers with zeros behind the end.  One workgroup per CU.
+//   4 x 4   256 x 256, RK 32: 256 accumulators per lane, in the accumulation half of the register file; per 16 summed elements a
+//           wavefront reads eight fragments for sixteen matrix instructions
+//   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  What bounds it is the 64 bytes a clock that L2 gives a CU, so an
+//           "along" request covers whole 128-byte lines (RK 32, two workgroups per CU: half of every line fetched is wasted, and
+//           it does not matter how many wavefronts share the CU)
 constexpr size_t kRMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
+constexpr int kStages = 4;
 template <int FR, int FC> struct Ring {
+  static constexpr int RK = FR == 4 ? 32 : 64;
+  static constexpr int kRounds = RK / 16;
   static constexpr int kRows = 64 * FR, kCols = 64 * FC;
-  static constexpr int kSideP = kRows * kRK * 2, kSideQ = kCols * kRK * 2, kStage = kSideP + kSideQ;
+  static constexpr int kSideP = kRows * RK * 2, kSideQ = kCols * RK * 2, kStage = kSideP + kSideQ;
   static constexpr int kCStride = 32 * FC + 4;   // floats per row of a wavefront's 32 x (32*FC) piece of the output
-  static constexpr int kLds = 4 * kStage > 4 * 32 * kCStride * 4 ? 4 * kStage : 4 * 32 * kCStride * 4;
-  static constexpr int kPerStep = FR + FC;       // requests of a wavefront per step
+  static constexpr int kLds = kStages * kStage;  // the output's pieces fit in there too
+  static constexpr int kPerStep = (FR + FC) * RK / 32;   // requests of a wavefront per step
+  static_assert(kLds >= 4 * 32 * kCStride * 4, "output pieces");
 };
 
 __device__ __forceinline__ u32x4 descriptor(const void* base) {   // no stride; the offsets used below stay inside the matrix
@@ -295,53 +300,55 @@ __device__ __forceinline__ void load_to_lds(u32x4 rs, uint32_t lds_addr, uint32_
 }
 constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
 
-// One operand of F 64-row (or 64-column) bands.
-template <bool ALONG, int F> struct RSide {
-  static constexpr int kOuter = 64 * F;
-  static constexpr int kRowBytes = kOuter * 2;             // across: one summed element
-  static constexpr int kLanes = kRowBytes / 16;            // across: lanes per summed element (32 or 16)
-  static constexpr int kPer = 64 / kLanes;                 // across: summed elements per request (2 or 4)
+// One operand of F 64-row (or 64-column) bands, RK summed elements at a time.
+template <bool ALONG, int F, int RK> struct RSide {
+  static constexpr int kOuter = 64 * F, kRequests = F * RK / 32;   // of a wavefront, per stage
+  static constexpr int kRowBytes = ALONG ? 2 * RK : 2 * kOuter;    // a row of the stage: one outer index, or one summed element
+  static constexpr int kLanes = kRowBytes / 16, kPer = 64 / kLanes;   // lanes per row, rows per request
   const uint16_t* base;   // along: the tile's first row;  across: its first column
-  uint32_t voff[F], soff0, soffj;
+  uint32_t voff[ALONG ? kRequests : 1], soff0, soffj;
   size_t ld;
-  // wavefront w makes requests j = 0..F-1 of a stage: along: rows 16*(w + 4j) .. +15;  across: summed elements
-  // kPer*(w + 4j) .. +kPer-1.  outer: rows, or columns that may be read (a multiple of 8)
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (!ALONG) return 4 * (row & 3);
+    else return RK == 32 ? (row >> 2) & 3 : (row & 7) ^ ((row >> 3) & 7);
+  }
+  // wavefront w makes requests j of a stage: its rows kPer*(w + 4j) .. +kPer-1.  outer: rows, or columns that may be read (a
+  // multiple of 8)
   __device__ __forceinline__ void init(const uint16_t* p, size_t ld_, int o0, int outer, int lane, int wave) {
     ld = ld_;
+    const int in = lane / kLanes, slot = lane % kLanes;
     if constexpr (ALONG) {
       base = p + (size_t)o0 * ld;
       const int last = outer - 1 - o0;
 #pragma unroll
-      for (int j = 0; j < F; j++) {
-        const int r = 16 * (wave + 4 * j) + (lane >> 2);
-        voff[j] = (uint32_t)(r < last ? r : last) * (uint32_t)(ld * 2) + 16u * (uint32_t)((lane & 3) ^ ((lane >> 4) & 3));
+      for (int j = 0; j < kRequests; j++) {
+        const int r = kPer * (wave + 4 * j) + in;
+        voff[j] = (uint32_t)(r < last ? r : last) * (uint32_t)(ld * 2) + 16u * (uint32_t)(slot ^ swizzle(r));
       }
       soff0 = soffj = 0;
     } else {
       base = p + o0;
-      const int kr = lane / kLanes, k4 = kPer == 4 ? kr : 2 * (wave & 1) + kr;   // (kPer*(w + 4j) + kr) % 4
-      const int c = 8 * ((lane % kLanes) ^ (4 * k4)), last = outer - 8 - o0;
-      voff[0] = (uint32_t)kr * (uint32_t)(ld * 2) + 2u * (uint32_t)(c < last ? c : last);
+      const int c = 8 * (slot ^ swizzle(kPer * wave + in)), last = outer - 8 - o0;   // (a multiple of 4 rows from j to j + 1)
+      voff[0] = (uint32_t)in * (uint32_t)(ld * 2) + 2u * (uint32_t)(c < last ? c : last);
       soff0 = (uint32_t)(kPer * wave) * (uint32_t)(ld * 2);
       soffj = (uint32_t)(4 * kPer) * (uint32_t)(ld * 2);
     }
   }
   __device__ __forceinline__ void request(uint32_t lds_addr, int step, int j) const {
-    if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (kRK * 2));
-    else load_to_lds(descriptor(base + (size_t)step * kRK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
+    if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (RK * 2));
+    else load_to_lds(descriptor(base + (size_t)step * RK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
   }
-  // the summed elements from `k` on, `left` < 32 of them, through registers
+  // the summed elements from `k` on, `left` < RK of them, through registers
   __device__ __forceinline__ void put_tail(uint8_t* lds, int k, int left, int o0, int outer, int t) const {
 #pragma unroll
-    for (int i = 0; i < F; i++) {
-      const int id = t + 256 * i;
+    for (int i = 0; i < kRequests; i++) {
+      const int id = t + 256 * i, row = id / kLanes, c = 8 * ((id % kLanes) ^ swizzle(row));
       u32x4 v;
       if constexpr (ALONG) {
-        const int row = id >> 2, c = 8 * ((id & 3) ^ ((row >> 2) & 3)), last = outer - 1 - o0;
+        const int last = outer - 1 - o0;
         v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c);
       } else {
-        const int kr = id / kLanes, c = 8 * ((id % kLanes) ^ (4 * (kr & 3)));
-        v = load_piece(base + (size_t)(k + kr) * ld + c, kr < left ? outer - o0 - c : 0);
+        v = load_piece(base + (size_t)(k + row) * ld + c, row < left ? outer - o0 - c : 0);
       }
       *reinterpret_cast<u32x4*>(lds + id * 16) = v;
     }
@@ -349,14 +356,14 @@ template <bool ALONG, int F> struct RSide {
   // fragment f: 32 rows or columns from 32*f of this wavefront's half of the tile, 16 summed elements from 16*ks on
   static __device__ __forceinline__ int address(int half, int lane) {
     const int li = lane & 31, lh = lane >> 5;
-    if constexpr (ALONG) return (32 * F * half + li) * 64;
+    if constexpr (ALONG) return (32 * F * half + li) * kRowBytes;
     const int a16 = lane & 15, g2 = (lane >> 4) & 1;
     return (lh * 8 + (a16 >> 2)) * kRowBytes + (((4 * F * half + 2 * g2 + ((a16 >> 1) & 1)) ^ (4 * (a16 >> 2))) * 16) + 8 * (a16 & 1);
   }
   static __device__ __forceinline__ s16x8 frag(const uint8_t* lds, int at, int f, int ks, int lane) {
     if constexpr (ALONG) {
-      const int li = lane & 31, lh = lane >> 5;
-      return *reinterpret_cast<const s16x8*>(lds + at + f * 2048 + (((2 * ks + lh) ^ ((li >> 2) & 3)) << 4));
+      const int li = lane & 31, lh = lane >> 5;   // a half of the tile is a multiple of 64 rows: it does not change the swizzle
+      return *reinterpret_cast<const s16x8*>(lds + at + f * 32 * kRowBytes + (((2 * ks + lh) ^ swizzle(32 * f + li)) << 4));
     } else {
       const uint8_t* p = lds + (at ^ (f * 64)) + ks * (16 * kRowBytes);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
@@ -440,25 +447,23 @@ template <bool OUT32> struct AnyPieces {
   }
 };
 
-// OUT: kOut16, kOut32 or kOutPartial.  WHOLE: every piece of an output row is inside it and 16-byte aligned.
+// One tile.  OUT: kOut16, kOut32 or kOutPartial.  WHOLE: every piece of an output row is inside it and 16-byte aligned.
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(FR * FC == 16 ? 1 : 2, FR * FC == 16 ? 1 : 2)))
-void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
+__device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, const uint32_t tile, const int split, uint8_t* const lds_ring) {
   typedef Ring<FR, FC> R;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
+  constexpr int RK = R::RK;
   int tr, tc;
-  tile_of(blockIdx.x, pr.tiles_r, pr.tiles_c, tr, tc);
+  tile_of(tile, pr.tiles_r, pr.tiles_c, tr, tc);
   const int r0 = tr * R::kRows, c0 = tc * R::kCols;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);   // a scalar: it goes into descriptors
   const int wr = wave >> 1, wc = wave & 1, li = lane & 31, lh = lane >> 5;
-  // this split's steps: first .. first + nk, and the elements behind the last whole step
-  const int first = OUT == kOutPartial ? (int)blockIdx.y * (pr.per_split / kRK) : 0;
-  const int k_begin = first * kRK;
+  // this split's whole steps, and the elements behind them
+  const int k_begin = OUT == kOutPartial ? split * pr.per_split : 0, first = k_begin / RK;
   const int k_end = OUT == kOutPartial && pr.sum - k_begin > pr.per_split ? k_begin + pr.per_split : pr.sum;
-  const int nk = (k_end - k_begin) / kRK, left = (k_end - k_begin) - nk * kRK;
+  const int nk = (k_end - k_begin) / RK, left = (k_end - k_begin) - nk * RK;
 
-  RSide<PA, FR> sp;
-  RSide<QA, FC> sq;
+  RSide<PA, FR, RK> sp;
+  RSide<QA, FC, RK> sq;
   sp.init(pr.p, pr.ldp, r0, pr.read_r, lane, wave);
   sq.init(pr.q, pr.ldq, c0, pr.read_c, lane, wave);
   typedef __attribute__((address_space(3))) void* lds_void_ptr;
@@ -466,9 +471,9 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
   // request j of step `kt` (past the end: the last step's again, unused), into stage `stage`
   auto request_p = [&](int stage, int kt, int j) { sp.request(lds0 + stage * R::kStage, first + (kt < nk ? kt : nk - 1), j); };
   auto request_q = [&](int stage, int kt, int j) { sq.request(lds0 + stage * R::kStage + R::kSideP, first + (kt < nk ? kt : nk - 1), j); };
-  const int pat = RSide<PA, FR>::address(wr, lane), qat = RSide<QA, FC>::address(wc, lane);
-  auto read_p = [&](int stage, int f, int ks) { return RSide<PA, FR>::frag(lds_ring + stage * R::kStage, pat, f, ks, lane); };
-  auto read_q = [&](int stage, int f, int ks) { return RSide<QA, FC>::frag(lds_ring + stage * R::kStage + R::kSideP, qat, f, ks, lane); };
+  const int pat = sp.address(wr, lane), qat = sq.address(wc, lane);
+  auto read_p = [&](int stage, int f, int ks) { return sp.frag(lds_ring + stage * R::kStage, pat, f, ks, lane); };
+  auto read_q = [&](int stage, int f, int ks) { return sq.frag(lds_ring + stage * R::kStage + R::kSideP, qat, f, ks, lane); };
 
   f32x16 acc[FC][FR];   // [column block][row block]: register 4*i+e is row 32*rb + li, column 32*cb + 8*i + 4*lh + e
 #pragma unroll
@@ -479,17 +484,17 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
       for (int i = 0; i < 16; i++) acc[a][b][i] = 0.0f;
 
   // A round of 16 summed elements multiplies from fragment set `set` while the fragments of the next round are read into the
-  // other set from (stage rbuf, half rks), in the order in which that round needs them; between the matrix instructions half
-  // of the requests for step `lkt` go out.  Every piece is pinned in place: the order is the schedule.
-  // Odd steps make their two halves of the requests in the other order: a request of an "along" operand touches half of every
-  // 128-byte line, and the other half then follows one round later, while the line is still in L1 (dX of 8192 x 8192 x 4096:
-  // 430 -> 412 us).
+  // other set from (stage rbuf, sixteen rks), in the order in which that round needs them; between the matrix instructions part
+  // `part` (of kRounds) of the requests for step `lkt` goes out.  Every piece is pinned in place: the order is the schedule.
   s16x8 fq[2][FC], fp[2][FR];
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
-  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int first_half) {
-    const int o = set ^ 1, half = first_half ^ (lstage & 1);
+  auto round = [&](int set, int rbuf, int rks, int lstage, int lkt, int part) {
+    const int o = set ^ 1;
     auto m = [&](int rb, int cb) { acc[cb][rb] = mfma32<F16>(fq[set][cb], fp[set][rb], acc[cb][rb]); };
     if constexpr (FR == 4 && FC == 4) {
+      // Odd steps make their two parts in the other order: a request of an "along" operand touches half of every 128-byte line,
+      // and the other half then follows one round later, while the line is still in L1 (dX of 8192 x 8192 x 4096: 430 -> 412 us).
+      const int half = part ^ (lstage & 1);
       fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
       fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
       fq[o][1] = read_q(rbuf, 1, rks); m(0, 2); pin();
@@ -514,19 +519,20 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
       static_assert(FR == 2 && FC == 2, "a schedule is written out for 4 x 4 and 2 x 2 blocks");
       fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
       fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
-      request_p(lstage, lkt, half); pin();
+      request_p(lstage, lkt, part); pin();
       fq[o][1] = read_q(rbuf, 1, rks); m(1, 0); pin();
       fp[o][1] = read_p(rbuf, 1, rks); m(1, 1); pin();
-      request_q(lstage, lkt, half); pin();
+      request_q(lstage, lkt, part); pin();
     }
   };
   // Step kt multiplies from stage kt%4:
-  //   round 0   reads the second half of this step's fragments; second half of the requests for step kt+3
-  //   barrier   every wavefront waits for its own requests for step kt+1 (those of two newer steps stay in flight) and for
-  //             its LDS reads, then for the others: stage (kt+1)%4 is complete, nobody reads stage kt%4 any more
-  //   round 1   reads the first half of step kt+1; first half of the requests for step kt+4, into stage kt%4
+  //   all rounds but the last   read the next sixteen of this step; parts 1.. of the requests for step kt+3
+  //   barrier      every wavefront waits for its own requests for step kt+1 (those of two newer steps stay in flight) and for
+  //                its LDS reads, then for the others: stage (kt+1)%4 is complete, nobody reads stage kt%4 any more
+  //   last round   reads the first sixteen of step kt+1; part 0 of the requests for step kt+4, into stage kt%4
   auto step = [&](int st, int kt) {
-    round(0, st, 1, (st + 3) & 3, kt + 3, 1);
+#pragma unroll
+    for (int i = 0; i + 1 < R::kRounds; i++) round(i & 1, st, i + 1, (st + 3) & 3, kt + 3, i + 1);
     __builtin_amdgcn_s_waitcnt(waitcnt(2 * R::kPerStep, 0));
     __builtin_amdgcn_s_barrier();
     pin();
@@ -535,13 +541,16 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
   if (nk > 0) {
 #pragma unroll
     for (int st = 0; st < 4; st++) {
-      // stage 3 is odd: its first half is the second half of the rows
+      // of stage 3 part 0 only (with 4 x 4 blocks that is the second half of the rows: the stage is odd)
+      constexpr int kp = decltype(sp)::kRequests, kq = decltype(sq)::kRequests;
 #pragma unroll
-      for (int j = st < 3 ? 0 : FR / 2; j < FR; j++) request_p(st, st, j);
+      for (int j = 0; j < kp; j++)
+        if (st < 3 || (R::kRounds == 2 ? j >= kp / 2 : j < kp / R::kRounds)) request_p(st, st, j);
 #pragma unroll
-      for (int j = st < 3 ? 0 : FC / 2; j < FC; j++) request_q(st, st, j);
+      for (int j = 0; j < kq; j++)
+        if (st < 3 || (R::kRounds == 2 ? j >= kq / 2 : j < kq / R::kRounds)) request_q(st, st, j);
     }
-    __builtin_amdgcn_s_waitcnt(waitcnt(5 * R::kPerStep / 2, 0));   // the requests for step 0 have landed
+    __builtin_amdgcn_s_waitcnt(waitcnt(2 * R::kPerStep + R::kPerStep / R::kRounds, 0));   // the requests for step 0 have landed
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int f = 0; f < FC; f++) fq[0][f] = read_q(0, f, 0);
@@ -561,11 +570,11 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
     __builtin_amdgcn_s_barrier();                // ... everywhere, before the stages are written to
   }
   if (left) {
-    sp.put_tail(lds_ring, k_begin + nk * kRK, left, r0, pr.read_r, t);
-    sq.put_tail(lds_ring + R::kSideP, k_begin + nk * kRK, left, c0, pr.read_c, t);
+    sp.put_tail(lds_ring, k_end - left, left, r0, pr.read_r, t);
+    sq.put_tail(lds_ring + R::kSideP, k_end - left, left, c0, pr.read_c, t);
     __syncthreads();
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
+    for (int ks = 0; ks < R::kRounds; ks++) {
 #pragma unroll
       for (int f = 0; f < FC; f++) fq[0][f] = read_q(0, f, ks);
 #pragma unroll
@@ -624,7 +633,7 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
         if constexpr (OUT == kOutPartial) {
           if (i < pieces) {
             const size_t ld = ((size_t)pr.cols + 7) & ~(size_t)7;
-            f32x4* const o = reinterpret_cast<f32x4*>(pr.partial + ((size_t)blockIdx.y * pr.rows + (row_first + lr + kStep * i)) * ld + col_first + 8 * lc);
+            f32x4* const o = reinterpret_cast<f32x4*>(pr.partial + ((size_t)split * pr.rows + (row_first + lr + kStep * i)) * ld + col_first + 8 * lc);
             o[0] = f32x4{v[u][0], v[u][1], v[u][2], v[u][3]};
             o[1] = f32x4{v[u][4], v[u][5], v[u][6], v[u][7]};
           }
@@ -636,6 +645,13 @@ void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
+  ring_tile<F16, PA, QA, FR, FC, OUT, WHOLE>(pr, ep, blockIdx.x, (int)blockIdx.y, lds_ring);
 }
 
 // Adds the splits of a product up and finishes the output.  2^shift lanes share a piece of eight columns: lane l adds the
@@ -1045,11 +1061,9 @@ bool ring_fetches(const Operand& o, bool along) {
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
 int launch_ring(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) {
   constexpr int kLds = Ring<FR, FC>::kLds;
-  if (kLds > 64 * 1024) {
-    static const hipError_t attr = hipFuncSetAttribute((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>,
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (attr != hipSuccess) return hip_fail(attr);
-  }
+  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attr != hipSuccess) return hip_fail(attr);
   hipLaunchKernelGGL((linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>), dim3((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits),
                      dim3(kBlock), kLds, s, pr, ep);
   CCN_HIP(hipGetLastError());
