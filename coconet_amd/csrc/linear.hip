@@ -272,6 +272,7 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f
 // sum that is no multiple of RK ends with a step loaded through registers with zeros behind the end.  One workgroup per CU.
 //   4 x 4   256 x 256, RK 32: 256 accumulators per lane, in the accumulation half of the register file; per 16 summed elements a
 //           wavefront reads eight fragments for sixteen matrix instructions
+//   4 x 2   256 x 128, RK 32: six fragments for eight
 //   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  What bounds it is the 64 bytes a clock that L2 gives a CU, so an
 //           "along" request covers whole 128-byte lines (RK 32, two workgroups per CU: half of every line fetched is wasted, and
 //           it does not matter how many wavefronts share the CU)
@@ -515,8 +516,21 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
       m(3, 2); pin();
       m(3, 3); pin();
       request_q(lstage, lkt, 2 * half + 1); pin();
+    } else if constexpr (FR == 4) {
+      const int half = part ^ (lstage & 1);   // as above
+      fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
+      fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
+      request_p(lstage, lkt, 2 * half); pin();
+      fq[o][1] = read_q(rbuf, 1, rks); m(1, 0); pin();
+      fp[o][1] = read_p(rbuf, 1, rks); m(1, 1); pin();
+      request_p(lstage, lkt, 2 * half + 1); pin();
+      fp[o][2] = read_p(rbuf, 2, rks); m(2, 0); pin();
+      m(2, 1); pin();
+      request_q(lstage, lkt, half); pin();
+      fp[o][3] = read_p(rbuf, 3, rks); m(3, 0); pin();
+      m(3, 1); pin();
     } else {
-      static_assert(FR == 2 && FC == 2, "a schedule is written out for 4 x 4 and 2 x 2 blocks");
+      static_assert(FR == 2 && FC == 2, "a schedule is written out for 4 x 4, 4 x 2 and 2 x 2 blocks");
       fq[o][0] = read_q(rbuf, 0, rks); m(0, 0); pin();
       fp[o][0] = read_p(rbuf, 0, rks); m(0, 1); pin();
       request_p(lstage, lkt, part); pin();
@@ -541,7 +555,7 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
   if (nk > 0) {
 #pragma unroll
     for (int st = 0; st < 4; st++) {
-      // of stage 3 part 0 only (with 4 x 4 blocks that is the second half of the rows: the stage is odd)
+      // of stage 3 part 0 only (with two rounds that is the second half of the rows: the stage is odd)
       constexpr int kp = decltype(sp)::kRequests, kq = decltype(sq)::kRequests;
 #pragma unroll
       for (int j = 0; j < kp; j++)
@@ -1084,7 +1098,7 @@ template <bool F16, bool PA, bool QA, int FR, int FC>
 int product_ring(LinProd& pr, const LinEpi& ep, bool out32, bool whole, int splits, hipStream_t s) {
   pr.tiles_r = (pr.rows + 64 * FR - 1) / (64 * FR);
   pr.tiles_c = (pr.cols + 64 * FC - 1) / (64 * FC);
-  if constexpr (FR * FC < 16) {
+  if constexpr (FR == 2) {
     if (splits > 1) {
       CCN_TRY((launch_ring<F16, PA, QA, FR, FC, kOutPartial, true>(pr, ep, splits, s)));
       return out32 ? launch_join<F16, true>(pr.partial, pr.rows, pr.cols, splits, ep, s) : launch_join<F16, false>(pr.partial, pr.rows, pr.cols, splits, ep, s);
@@ -1147,24 +1161,30 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
 //   1024 x 1024 x 1024       30.2         12.2 / 13.1 / 15.1 / 20.5
 //   2048 x 4096 x 4096       77.7         71.2 / 110.7
 //   4096 x 4096 x 4096       110.9        134.2
+enum RingTile { kTile256, kTile256x128, kTile128 };
 struct RingPlan {
-  bool large;
+  RingTile tile;
   int splits;
 };
 RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus) {
-  const auto tiles = [&](int edge) { return (double)((rows + edge - 1) / edge) * (double)((cols + edge - 1) / edge); };
-  const double steps = (double)((sum + 63) / 64), t128 = tiles(128), t256 = tiles(256);
+  const auto tiles = [&](int r, int c) { return (double)((rows + r - 1) / r) * (double)((cols + c - 1) / c); };
+  const double steps = (double)((sum + 63) / 64), t128 = tiles(128, 128);
   const size_t each = (size_t)rows * round8((size_t)cols);
-  RingPlan best{true, 1};
-  double least = 8.0 + 1.6 * steps * std::ceil(t256 / cus);
+  RingPlan best{kTile256, 1};
+  double least = 8.0 + 1.6 * steps * std::ceil(tiles(256, 256) / cus);
+  const double half = 6.0 + 0.9 * steps * std::ceil(tiles(256, 128) / cus);
+  if (half < least) {
+    least = half;
+    best.tile = kTile256x128;
+  }
   for (int s = 1; s <= kMaxSplits; s++) {
     if (s > 1 && (s * 2.0 > steps || (double)s * t128 > 2.0 * cus || (size_t)s * each > partial_floats)) break;
     const double deep = std::ceil(s * t128 / cus);
-    double t = 3.5 + std::ceil(steps / s) * (deep < 2.0 ? 0.42 : 0.53 * deep);
+    double t = 5.0 + std::ceil(steps / s) * (deep < 2.0 ? 0.40 : 0.5 * deep);
     if (s > 1) t += 1.8 + 0.4e-6 * 4.0 * (double)s * (double)each;
     if (t < least) {
       least = t;
-      best = RingPlan{false, s};
+      best = RingPlan{kTile128, s};
     }
   }
   return best;
@@ -1195,7 +1215,8 @@ int product(ccn_linear_plan* plan, const Operand& p, const Operand& q, int rows,
   const int steps = (sum + 63) / 64;
   pr.per_split = 64 * ((steps + how.splits - 1) / how.splits);
   if (how.splits > 1) how.splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
-  if (how.large) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
+  if (how.tile == kTile256) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
+  if (how.tile == kTile256x128) return product_ring<F16, PA, QA, 4, 2>(pr, ep, out32, whole, 1, s);
   return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, how.splits, s);
 }
 
