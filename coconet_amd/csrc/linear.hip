@@ -945,49 +945,49 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
 }
 
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
-// dz = dY * act'(pre), rounded to the operands' type into the workspace (rows of N rounded up to 8, zeros in the rest),
-// and fp32 sums over a chunk of rows of the unrounded dz.  Four wavefronts walk a chunk's rows, 512 columns wide, four rows in
-// flight each.  With one chunk the sums are db itself (`add`: added to it).
-template <bool F16>
-__global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __restrict__ dY, const size_t lddy,
-                                                           const uint16_t* __restrict__ pre, const size_t ldp,
-                                                           uint16_t* __restrict__ dz, const size_t lddz, float* __restrict__ sums,
-                                                           const int M, const int N, const int act, const int rows_per_chunk, const int add) {
-  __shared__ float part[4][512 + 8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = (int)blockIdx.x * 512 + lane * 8, n = N - col;
+// dz = dY * act'(pre), rounded to the operands' type into the workspace (aligned rows, zeros up to a multiple of 8 columns), and
+// fp32 sums over a chunk of rows of the unrounded dz.  LANES lanes share a row's strip of 8*LANES columns, a workgroup of WAVES
+// wavefronts works on WAVES * 64/LANES rows at a time, ROWS times that in flight.
+//   64, 4, 4     many rows: a strip of 512 columns, chunks of rows over the chip, linear_db_kernel adds the chunks up
+//   16, 16, 1    up to 64 rows, all at once: one chunk, its sums are db itself (`add`: added to it)
+template <bool F16, int LANES, int WAVES, int ROWS>
+__global__ __launch_bounds__(WAVES * kWave) void linear_dz_kernel(const uint16_t* __restrict__ dY, const size_t lddy,
+                                                                  const uint16_t* __restrict__ pre, const size_t ldp,
+                                                                  uint16_t* __restrict__ dz, const size_t lddz, float* __restrict__ sums,
+                                                                  const int M, const int N, const int act, const int rows_per_chunk,
+                                                                  const int add) {
+  constexpr int kPass = WAVES * (kWave / LANES), kWidth = 8 * LANES;
+  __shared__ float part[WAVES][kWidth + 8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, piece = lane % LANES;
+  const int col = (int)blockIdx.x * kWidth + piece * 8, n = N - col;
   const int m0 = (int)blockIdx.y * rows_per_chunk;
   const int m1 = M - m0 < rows_per_chunk ? M : m0 + rows_per_chunk;
   float s[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) s[e] = 0.0f;
   if (n > 0) {
-    constexpr int kRows = 4;   // rows in flight per wavefront
-    for (int m = m0 + wave; m < m1; m += 4 * kRows) {
-      u32x4 gv[kRows], zv[kRows];
+    for (int m = m0 + wave * (kWave / LANES) + lane / LANES; m < m1; m += ROWS * kPass) {
+      u32x4 gv[ROWS], zv[ROWS];
 #pragma unroll
-      for (int u = 0; u < kRows; u++) {
-        if (m + 4 * u < m1) {
-          gv[u] = load_piece(dY + (size_t)(m + 4 * u) * lddy + col, n);
-          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)(m + 4 * u) * ldp + col, n);
+      for (int u = 0; u < ROWS; u++) {
+        const int r = m + u * kPass;
+        if (r < m1) {
+          gv[u] = load_piece(dY + (size_t)r * lddy + col, n);
+          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)r * ldp + col, n);
         }
       }
 #pragma unroll
-      for (int u = 0; u < kRows; u++) {
-        if (m + 4 * u < m1) {
+      for (int u = 0; u < ROWS; u++) {
+        const int r = m + u * kPass;
+        if (r < m1) {
           float g[8];
           unpack<F16>(gv[u], g);
-          if (act != CCN_ACT_NONE) {
+          if (act != CCN_ACT_NONE) {   // (behind the row's end dY and pre are zeros, and so is the product)
             float z[8];
             unpack<F16>(zv[u], z);
             act_slopes(act, z, g);
-#pragma unroll
-            for (int e = 0; e < 8; e++) g[e] = e < n ? g[e] : 0.0f;
           }
-          if (dz) {
-            const u32x4 v = pack<F16>(g);
-            __builtin_memcpy(dz + (size_t)(m + 4 * u) * lddz + col, &v, 16);
-          }
+          if (dz) *reinterpret_cast<u32x4*>(dz + (size_t)r * lddz + col) = pack<F16>(g);
 #pragma unroll
           for (int e = 0; e < 8; e++) s[e] += g[e];
         }
@@ -996,37 +996,73 @@ __global__ __launch_bounds__(kBlock) void linear_dz_kernel(const uint16_t* __res
   }
   if (!sums) return;
 #pragma unroll
-  for (int e = 0; e < 8; e++) part[wave][lane * 8 + e] = s[e];
-  __syncthreads();
+  for (int off = LANES; off < kWave; off <<= 1)
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const int c = threadIdx.x + 256 * h, at = (int)blockIdx.x * 512 + c;
+    for (int e = 0; e < 8; e++) s[e] += __shfl_xor(s[e], off, kWave);
+  if (lane < LANES) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) part[wave][piece * 8 + e] = s[e];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < kWidth; c += WAVES * kWave) {
+    const int at = (int)blockIdx.x * kWidth + c;
     if (at < N) {
-      const float x = ((part[0][c] + part[1][c]) + part[2][c]) + part[3][c];
+      float x = part[0][c];
+#pragma unroll
+      for (int w = 1; w < WAVES; w++) x += part[w][c];
       float* const o = sums + (size_t)blockIdx.y * N + at;
       *o = add ? *o + x : x;
     }
   }
 }
-// db[n] = (db[n] +) the sum of the chunks' sums: 64 columns per workgroup, each of 16 wavefronts every sixteenth chunk.
-constexpr int kDbWaves = 16;
-__global__ __launch_bounds__(kDbWaves * kWave) void linear_db_kernel(const float* __restrict__ sums, float* __restrict__ db, const int N,
-                                                                     const int chunks, const int accumulate) {
-  __shared__ float part[kDbWaves][kWave];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * kWave + lane;
+// db[n] = (db[n] +) the sum of the chunks' sums: 64 columns per workgroup of WAVES wavefronts, each every WAVES-th chunk.
+struct DbArgs {
+  const float* sums;
+  float* db;
+  int cols, chunks, accumulate;
+};
+template <int WAVES> __device__ __forceinline__ void add_chunks(const DbArgs& a, const int block, float* const part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = block * kWave + lane;
   float s = 0.0f;
-  if (c < N) {
+  if (c < a.cols) {
 #pragma unroll 8
-    for (int k = wave; k < chunks; k += kDbWaves) s += sums[(size_t)k * N + c];
+    for (int k = wave; k < a.chunks; k += WAVES) s += a.sums[(size_t)k * a.cols + c];
   }
-  part[wave][lane] = s;
+  part[wave * kWave + lane] = s;
   __syncthreads();
-  if (wave == 0 && c < N) {
-    float x = part[0][lane];
+  if (wave == 0 && c < a.cols) {
+    float x = part[lane];
 #pragma unroll
-    for (int w = 1; w < kDbWaves; w++) x += part[w][lane];
-    db[c] = accumulate ? db[c] + x : x;
+    for (int w = 1; w < WAVES; w++) x += part[w * kWave + lane];
+    a.db[c] = a.accumulate ? a.db[c] + x : x;
   }
+}
+constexpr int kDbWaves = 16;
+__global__ __launch_bounds__(kDbWaves * kWave) void linear_db_kernel(const DbArgs a) {
+  __shared__ float part[kDbWaves * kWave];
+  add_chunks<kDbWaves>(a, (int)blockIdx.x, part);
+}
+
+// Both products of a backward pass, and db, in one launch: the tiles of small ones run side by side on CUs that one product alone
+// would leave idle, and two launches are saved.  The product with the longer sum is dealt out first.
+struct PairArgs {
+  LinProd x, w;    // dX, dW
+  LinEpi ex, ew;
+  DbArgs db;
+  int nx, nw, w_first;   // tiles of each; the workgroups behind them are db's
+};
+template <bool F16, bool OUT32, bool WHOLE>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1))) void linear_pair_kernel(const PairArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
+  const int b = (int)blockIdx.x;
+  if (b >= a.nx + a.nw) {
+    add_chunks<kBlock / kWave>(a.db, b - a.nx - a.nw, reinterpret_cast<float*>(lds_ring));
+    return;
+  }
+  if (a.w_first ? b >= a.nw : b < a.nx)
+    ring_tile<F16, true, true, 2, 2, kOut16, WHOLE>(a.x, a.ex, (uint32_t)(a.w_first ? b - a.nw : b), 0, lds_ring);
+  else
+    ring_tile<F16, false, false, 2, 2, OUT32 ? kOut32 : kOut16, WHOLE>(a.w, a.ew, (uint32_t)(a.w_first ? b : b - a.nx), 0, lds_ring);
 }
 
 constexpr size_t kMaxLd = (size_t)1 << 22;
@@ -1165,35 +1201,27 @@ enum RingTile { kTile256, kTile256x128, kTile128 };
 struct RingPlan {
   RingTile tile;
   int splits;
+  double us;
 };
 RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus) {
   const auto tiles = [&](int r, int c) { return (double)((rows + r - 1) / r) * (double)((cols + c - 1) / c); };
   const double steps = (double)((sum + 63) / 64), t128 = tiles(128, 128);
   const size_t each = (size_t)rows * round8((size_t)cols);
-  RingPlan best{kTile256, 1};
-  double least = 8.0 + 1.6 * steps * std::ceil(tiles(256, 256) / cus);
+  RingPlan best{kTile256, 1, 8.0 + 1.6 * steps * std::ceil(tiles(256, 256) / cus)};
   const double half = 6.0 + 0.9 * steps * std::ceil(tiles(256, 128) / cus);
-  if (half < least) {
-    least = half;
-    best.tile = kTile256x128;
-  }
+  if (half < best.us) best = RingPlan{kTile256x128, 1, half};
   for (int s = 1; s <= kMaxSplits; s++) {
     if (s > 1 && (s * 2.0 > steps || (double)s * t128 > 2.0 * cus || (size_t)s * each > partial_floats)) break;
     const double deep = std::ceil(s * t128 / cus);
     double t = 5.0 + std::ceil(steps / s) * (deep < 2.0 ? 0.40 : 0.5 * deep);
     if (s > 1) t += 1.8 + 0.4e-6 * 4.0 * (double)s * (double)each;
-    if (t < least) {
-      least = t;
-      best = RingPlan{kTile128, s};
-    }
+    if (t < best.us) best = RingPlan{kTile128, s, t};
   }
   return best;
 }
 
-// One product of operands that the ring can fetch: C [rows x cols].
-template <bool F16, bool PA, bool QA>
-int product(ccn_linear_plan* plan, const Operand& p, const Operand& q, int rows, int cols, int sum, const LinEpi& ep, bool out32, int cus,
-            hipStream_t s) {
+// A product of operands that the ring can fetch: C [rows x cols].
+LinProd make_product(const ccn_linear_plan* plan, const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum) {
   LinProd pr;
   pr.p = p.p;
   pr.q = q.p;
@@ -1202,22 +1230,40 @@ int product(ccn_linear_plan* plan, const Operand& p, const Operand& q, int rows,
   pr.rows = rows;
   pr.cols = cols;
   pr.sum = sum;
-  pr.read_r = PA ? rows : p.extent;
-  pr.read_c = QA ? cols : q.extent;
+  pr.read_r = p_along ? rows : p.extent;
+  pr.read_c = q_along ? cols : q.extent;
+  pr.tiles_r = (rows + 127) / 128;
+  pr.tiles_c = (cols + 127) / 128;
+  pr.per_split = 0;
   pr.partial = plan->partial;
-  if ((size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128) > 0x7fffffffull) return CCN_ERANGE;
-  const auto whole_rows = [](const void* x, size_t ld, int size) {
+  return pr;
+}
+// Whether every piece of the output's rows (and of what is read or written beside it) is inside its row and 16-byte aligned.
+bool whole_pieces(const LinEpi& ep, int cols, bool out32) {
+  const auto ok = [](const void* x, size_t ld, int size) {
     return aligned16(x) && ld % (size_t)(16 / size) == 0 && ld * (size_t)size <= 2 * kRMaxLd;
   };
-  const bool whole = cols % 8 == 0 && whole_rows(ep.out, ep.ldo, out32 ? 4 : 2) && (!ep.resid || whole_rows(ep.resid, ep.ldr, 2)) &&
-                     (!ep.pre || whole_rows(ep.pre, ep.ldp, 2));
-  RingPlan how = choose_ring(rows, cols, sum, plan->partial_floats, cus);
-  const int steps = (sum + 63) / 64;
+  return cols % 8 == 0 && ok(ep.out, ep.ldo, out32 ? 4 : 2) && (!ep.resid || ok(ep.resid, ep.ldr, 2)) && (!ep.pre || ok(ep.pre, ep.ldp, 2));
+}
+template <bool F16, bool PA, bool QA>
+int run_product(LinProd& pr, const LinEpi& ep, bool out32, RingPlan how, hipStream_t s) {
+  if ((size_t)pr.tiles_r * (size_t)pr.tiles_c > 0x7fffffffull) return CCN_ERANGE;
+  const bool whole = whole_pieces(ep, pr.cols, out32);
+  const int steps = (pr.sum + 63) / 64;
   pr.per_split = 64 * ((steps + how.splits - 1) / how.splits);
-  if (how.splits > 1) how.splits = (sum + pr.per_split - 1) / pr.per_split;   // no empty split
+  if (how.splits > 1) how.splits = (pr.sum + pr.per_split - 1) / pr.per_split;   // no empty split
   if (how.tile == kTile256) return product_ring<F16, PA, QA, 4, 4>(pr, ep, out32, whole, 1, s);
   if (how.tile == kTile256x128) return product_ring<F16, PA, QA, 4, 2>(pr, ep, out32, whole, 1, s);
   return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, how.splits, s);
+}
+template <bool F16, bool OUT32, bool WHOLE> int launch_pair(const PairArgs& a, hipStream_t s) {
+  constexpr int kLds = Ring<2, 2>::kLds;
+  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_pair_kernel<F16, OUT32, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attr != hipSuccess) return hip_fail(attr);
+  const int blocks = a.nx + a.nw + (a.db.db ? (a.db.cols + kWave - 1) / kWave : 0);
+  hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE>), dim3((unsigned)blocks), dim3(kBlock), kLds, s, a);
+  CCN_HIP(hipGetLastError());
+  return CCN_OK;
 }
 
 // Aligned copies of up to two operands into the plan (nullptr: none).
@@ -1272,7 +1318,8 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
     if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
     if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
   }
-  return product<F16, true, false>(plan, x, w, M, N, K, ep, false, di->cu_count, s);
+  LinProd pr = make_product(plan, x, true, w, false, M, N, K);
+  return run_product<F16, true, false>(pr, ep, false, choose_ring(M, N, K, plan->partial_floats, di->cu_count), s);
 }
 
 template <bool F16>
@@ -1303,26 +1350,26 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const bool want_dz = M > 0 && (act != CCN_ACT_NONE ? dX || dW : (dW && !ring_fetches(g, false)) || (dX && !few && !ring_fetches(g, true)));
   if (want_dz) g = Operand{plan->dz, round8((size_t)plan->max_n), M, (int)round8((size_t)N)};
   int chunks = 0;
-  bool done = false;   // db is there
+  bool db_left = db != nullptr;
   if (M > 0 && (want_dz || db)) {
-    const int strips = (N + 511) / 512;
-    // rows per chunk: four workgroups for every CU, at least one row for each wavefront; up to 32 rows one chunk, which needs no
-    // second kernel
-    int per = (int)(((size_t)M * strips + 4 * (size_t)di->cu_count - 1) / (4 * (size_t)di->cu_count));
-    if (per < 4) per = 4;
-    if ((M + per - 1) / per > kMaxChunks) per = (M + kMaxChunks - 1) / kMaxChunks;
-    if (M <= 32) per = M;
-    chunks = (M + per - 1) / per;
-    done = chunks == 1;
-    float* const sums = !db ? nullptr : done ? db : plan->sums;
-    hipLaunchKernelGGL((linear_dz_kernel<F16>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp,
-                       want_dz ? plan->dz : nullptr, g.ld, sums, M, N, act, per, done ? accumulate : 0);
+    uint16_t* const to = want_dz ? plan->dz : nullptr;
+    if (few) {
+      hipLaunchKernelGGL((linear_dz_kernel<F16, 16, 16, 1>), dim3((unsigned)((N + 127) / 128)), dim3(16 * kWave), 0, s, dY, lddy, pre, ldp, to, g.ld,
+                         db, M, N, act, M, accumulate);
+      db_left = false;
+    } else {
+      // rows per chunk: four workgroups for every CU, at least one row for each wavefront
+      const int strips = (N + 511) / 512;
+      int per = (int)(((size_t)M * strips + 4 * (size_t)di->cu_count - 1) / (4 * (size_t)di->cu_count));
+      if (per < 4) per = 4;
+      if ((M + per - 1) / per > kMaxChunks) per = (M + kMaxChunks - 1) / kMaxChunks;
+      chunks = (M + per - 1) / per;
+      hipLaunchKernelGGL((linear_dz_kernel<F16, 64, 4, 4>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp, to, g.ld,
+                         db ? plan->sums : nullptr, M, N, act, per, 0);
+    }
     CCN_HIP(hipGetLastError());
   }
-  if (db && !done) {
-    hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kDbWaves * kWave), 0, s, plan->sums, db, N, chunks, accumulate);
-    CCN_HIP(hipGetLastError());
-  }
+  const DbArgs dba{plan->sums, db_left ? db : nullptr, N, chunks, accumulate};
   // operands that the ring cannot fetch: W along its rows for dX, X and dz across them for dW
   Operand x{X, ldx, M, K}, w{W, ldw, K, N};
   const bool cw = dX && !few && !ring_fetches(w, true), cx = dW && M > 0 && !ring_fetches(x, false);
@@ -1333,11 +1380,39 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
     if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
     if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
   }
-  if (dX && M > 0) {
-    if (few) CCN_TRY((product_few<F16, true>(plan, g.p, g.ld, W, ldw, M, K, N, dx_ep, di->cu_count, s)));
-    else CCN_TRY((product<F16, true, true>(plan, g, w, M, K, N, dx_ep, false, di->cu_count, s)));
+  RingPlan hx{}, hw{};
+  LinProd px{}, pw{};
+  const bool ring_dx = dX && M > 0 && !few;
+  if (ring_dx) {
+    px = make_product(plan, g, true, w, true, M, K, N);
+    hx = choose_ring(M, K, N, plan->partial_floats, di->cu_count);
   }
-  if (dW) CCN_TRY((product<F16, false, false>(plan, x, g, K, N, M, dw_ep, dw32, di->cu_count, s)));
+  if (dW) {
+    pw = make_product(plan, x, false, g, false, K, N, M);
+    hw = choose_ring(K, N, M, plan->partial_floats, di->cu_count);
+  }
+  if (ring_dx && dW) {
+    // Side by side, if that is estimated to be faster than one after the other (3 us for what is between two launches): as long as
+    // the longer sum, and as all steps dealt over the CUs.
+    const double sx = (N + 63) / 64, sw = (M + 63) / 64;
+    const double tx = (double)px.tiles_r * px.tiles_c, tw = (double)pw.tiles_r * pw.tiles_c;
+    double longest = sx > sw ? sx : sw;
+    const double dealt = (tx * sx + tw * sw) / di->cu_count;
+    if (dealt > longest) longest = dealt;
+    if (5.0 + 0.5 * longest < hx.us + hw.us + (db_left ? 6.0 : 3.0) && tx + tw < 1e6) {
+      const PairArgs a{px, pw, dx_ep, dw_ep, dba, (int)tx, (int)tw, sw > sx ? 1 : 0};
+      const bool whole = whole_pieces(dx_ep, K, false) && whole_pieces(dw_ep, N, dw32);
+      if (dw32) return whole ? launch_pair<F16, true, true>(a, s) : launch_pair<F16, true, false>(a, s);
+      return whole ? launch_pair<F16, false, true>(a, s) : launch_pair<F16, false, false>(a, s);
+    }
+  }
+  if (db_left) {
+    hipLaunchKernelGGL(linear_db_kernel, dim3((unsigned)((N + kWave - 1) / kWave)), dim3(kDbWaves * kWave), 0, s, dba);
+    CCN_HIP(hipGetLastError());
+  }
+  if (ring_dx) CCN_TRY((run_product<F16, true, true>(px, dx_ep, false, hx, s)));
+  else if (dX && M > 0) CCN_TRY((product_few<F16, true>(plan, g.p, g.ld, W, ldw, M, K, N, dx_ep, di->cu_count, s)));
+  if (dW) CCN_TRY((run_product<F16, false, false>(pw, dw_ep, dw32, hw, s)));
   return CCN_OK;
 }
 
