@@ -103,11 +103,20 @@ __device__ __forceinline__ void act_slopes(int act, const float* z, float* g) {
 // ---- eight neighbouring elements of a row --------------------------------------------------------------------------------
 // gfx950 loads and stores 16 bytes at any 2-byte aligned address; `n` is how many of the eight are there (behind a row's
 // end they are neither read nor written).
-__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, int n) {
+// A piece that ends with its row is loaded as the row's last 16 bytes and shifted down: one load, where loads of single
+// elements under conditions would wait for each other.  back: elements of the row in front of p.
+__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, int n, int back) {
   u32x4 v = {0u, 0u, 0u, 0u};
-  if (n >= 8) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
+  if (n <= 0) return v;
+  const int s = n >= 8 ? 0 : 8 - n;
+  if (s <= back) {
+    __builtin_memcpy(&v, p - s, 16);
+    if (s) {
+      if (s & 4) v = u32x4{v[2], v[3], 0u, 0u};
+      if (s & 2) v = u32x4{v[1], v[2], v[3], 0u};
+      if (s & 1) v = u32x4{(v[0] >> 16) | (v[1] << 16), (v[1] >> 16) | (v[2] << 16), (v[2] >> 16) | (v[3] << 16), v[3] >> 16};
+    }
+  } else {   // a row of fewer than eight elements
 #pragma unroll
     for (int e = 0; e < 7; e++)
       if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
@@ -186,7 +195,7 @@ __device__ __forceinline__ Places places(const LinEpi& ep, size_t row0, size_t c
 template <bool OUT32> struct Old8 { u32x4 r; };        // the residual
 template <> struct Old8<true> { float d[8]; };         // what is added to
 template <bool OUT32>
-__device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, const Places& w, int i, int n) {
+__device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, const Places& w, int i, int n, int back) {
   if constexpr (OUT32) {
     if (!ep.accumulate) return;
     const float* const o = reinterpret_cast<const float*>(w.out + i * w.sout + w.vout);
@@ -198,7 +207,7 @@ __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, const
         if (e < n) x.d[e] = o[e];
     }
   } else {
-    if (ep.resid) x.r = load_piece(reinterpret_cast<const uint16_t*>(w.res + i * w.sres + w.vres), n);
+    if (ep.resid) x.r = load_piece(reinterpret_cast<const uint16_t*>(w.res + i * w.sres + w.vres), n, back);
   }
 }
 template <bool F16, bool OUT32>
@@ -255,6 +264,7 @@ struct LinProd {
   int read_r, read_c;  // rows or columns of the operands that may be read: rows, cols, or for an "across" operand that many rounded up to 8
   int tiles_r, tiles_c;
   int per_split;       // summed elements per split (a multiple of 64)
+  int brief;           // the sum is short: no ring
   float* partial;      // [splits][rows][cols rounded up to 8] when splits > 1
 };
 
@@ -284,9 +294,10 @@ template <int FR, int FC> struct Ring {
   static constexpr int kRows = 64 * FR, kCols = 64 * FC;
   static constexpr int kSideP = kRows * RK * 2, kSideQ = kCols * RK * 2, kStage = kSideP + kSideQ;
   static constexpr int kCStride = 32 * FC + 4;   // floats per row of a wavefront's 32 x (32*FC) piece of the output
-  static constexpr int kLds = kStages * kStage;  // the output's pieces fit in there too
+  static constexpr int kLds = kStages * kStage;
+  static constexpr int kPieces = 4 * 32 * kCStride * 4, kBriefLds = kStage > kPieces ? kStage : kPieces;   // one stage, then the output's pieces
   static constexpr int kPerStep = (FR + FC) * RK / 32;   // requests of a wavefront per step
-  static_assert(kLds >= 4 * 32 * kCStride * 4, "output pieces");
+  static_assert(kLds >= kPieces, "output pieces");
 };
 
 __device__ __forceinline__ u32x4 descriptor(const void* base) {   // no stride; the offsets used below stay inside the matrix
@@ -339,7 +350,7 @@ template <bool ALONG, int F, int RK> struct RSide {
     if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (RK * 2));
     else load_to_lds(descriptor(base + (size_t)step * RK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
   }
-  // the summed elements from `k` on, `left` < RK of them, through registers
+  // the summed elements from `k` on, `left` of them (RK are used), through registers
   __device__ __forceinline__ void put_tail(uint8_t* lds, int k, int left, int o0, int outer, int t) const {
 #pragma unroll
     for (int i = 0; i < kRequests; i++) {
@@ -347,9 +358,9 @@ template <bool ALONG, int F, int RK> struct RSide {
       u32x4 v;
       if constexpr (ALONG) {
         const int last = outer - 1 - o0;
-        v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c);
+        v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c, k + c);
       } else {
-        v = load_piece(base + (size_t)(k + row) * ld + c, row < left ? outer - o0 - c : 0);
+        v = load_piece(base + (size_t)(k + row) * ld + c, row < left ? outer - o0 - c : 0, o0 + c);
       }
       *reinterpret_cast<u32x4*>(lds + id * 16) = v;
     }
@@ -398,7 +409,7 @@ template <bool OUT32> struct WholePieces {
     sres = (uint32_t)step * (uint32_t)ep.ldr * 2;
     spre = (uint32_t)step * (uint32_t)ep.ldp * 2;
   }
-  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i, int) const {
+  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i) const {
     if constexpr (OUT32) {
       if (!ep.accumulate) return;
       const u32x4 lo = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(out, vout, i * sout, 0));
@@ -409,7 +420,7 @@ template <bool OUT32> struct WholePieces {
       if (ep.resid) x.r = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(res, vres, i * sres, 0));
     }
   }
-  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i, int) const {
+  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i) const {
     if constexpr (OUT32) {
       if (ep.accumulate) {
 #pragma unroll
@@ -437,16 +448,59 @@ template <bool OUT32> struct WholePieces {
     }
   }
 };
-// The same interface for rows that may start anywhere and end inside a piece.
+// The same interface for rows that may start anywhere (pieces inside the row; what is behind the last one: edge_elements).
 template <bool OUT32> struct AnyPieces {
   Places w;
   __device__ __forceinline__ AnyPieces(const LinEpi& ep, size_t row0, size_t col0, int lr, int lc, int step)
       : w(places<OUT32>(ep, row0, col0, lr, lc, step)) {}
-  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i, int n) const { ccn::load_old<OUT32>(x, ep, w, i, n); }
-  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i, int n) const {
-    finish8<F16, OUT32>(v, bias, old, ep, w, i, n);
+  __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, int i) const { ccn::load_old<OUT32>(x, ep, w, i, 8, 0); }
+  template <bool F16> __device__ __forceinline__ void finish(float* v, const Bias8& bias, const Old8<OUT32>& old, const LinEpi& ep, int i) const {
+    finish8<F16, OUT32>(v, bias, old, ep, w, i, 8);
   }
 };
+// The last `n` (1..7) columns of 32 rows of an output whose width is no multiple of 8, an element per lane and turn: at(row, e)
+// gives the finished sum.  rows: how many of the 32 are inside the matrix.
+template <bool F16, bool OUT32, class At>
+__device__ __forceinline__ void edge_elements(const LinEpi& ep, size_t row0, size_t col, int n, int rows, int lane, At at) {
+  constexpr int kTurns = 4;   // 7 * 32 elements at most
+  const uint32_t magic = 65536u / (uint32_t)n + 1u;   // i / n for i < 224
+  float v[kTurns], old[kTurns], bias[kTurns];
+  size_t r[kTurns], c[kTurns];
+  bool on[kTurns];
+#pragma unroll
+  for (int u = 0; u < kTurns; u++) {
+    const uint32_t i = (uint32_t)(lane + kWave * u), q = (i * magic) >> 16, e = i - q * (uint32_t)n;
+    on[u] = (int)q < rows;
+    r[u] = row0 + q;
+    c[u] = col + e;
+    v[u] = old[u] = bias[u] = 0.0f;
+    if (on[u]) {
+      v[u] = at((int)q, (int)e);
+      if constexpr (OUT32) {
+        if (ep.accumulate) old[u] = static_cast<const float*>(ep.out)[r[u] * ep.ldo + c[u]];
+      } else {
+        if (ep.bias) bias[u] = ep.bias[c[u]];
+        if (ep.resid) old[u] = half_in<F16>(ep.resid[r[u] * ep.ldr + c[u]]);
+      }
+    }
+  }
+  if constexpr (OUT32) {
+#pragma unroll
+    for (int u = 0; u < kTurns; u++)
+      if (on[u]) static_cast<float*>(ep.out)[r[u] * ep.ldo + c[u]] = old[u] + v[u];
+  } else {
+    float x[8];   // as the pieces compute them
+#pragma unroll
+    for (int u = 0; u < 8; u++) x[u] = u < kTurns ? v[u & 3] + bias[u & 3] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < kTurns; u++)
+      if (on[u] && ep.pre) ep.pre[r[u] * ep.ldp + c[u]] = half_out<F16>(x[u]);
+    act_values(ep.act, x);
+#pragma unroll
+    for (int u = 0; u < kTurns; u++)
+      if (on[u]) static_cast<uint16_t*>(ep.out)[r[u] * ep.ldo + c[u]] = half_out<F16>(ep.resid ? x[u] + old[u] : x[u]);
+  }
+}
 
 // One tile.  OUT: kOut16, kOut32 or kOutPartial.  WHOLE: every piece of an output row is inside it and 16-byte aligned.
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
@@ -461,7 +515,8 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
   // this split's whole steps, and the elements behind them
   const int k_begin = OUT == kOutPartial ? split * pr.per_split : 0, first = k_begin / RK;
   const int k_end = OUT == kOutPartial && pr.sum - k_begin > pr.per_split ? k_begin + pr.per_split : pr.sum;
-  const int nk = (k_end - k_begin) / RK, left = (k_end - k_begin) - nk * RK;
+  // (a short sum goes through registers altogether: it needs a quarter of the LDS, and four workgroups share a CU)
+  const int nk = pr.brief ? 0 : (k_end - k_begin) / RK;
 
   RSide<PA, FR, RK> sp;
   RSide<QA, FC, RK> sq;
@@ -583,9 +638,9 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
     __builtin_amdgcn_s_waitcnt(waitcnt(0, 0));   // the last reads of LDS and the last (unused) loads into it are done
     __builtin_amdgcn_s_barrier();                // ... everywhere, before the stages are written to
   }
-  if (left) {
-    sp.put_tail(lds_ring, k_end - left, left, r0, pr.read_r, t);
-    sq.put_tail(lds_ring + R::kSideP, k_end - left, left, c0, pr.read_c, t);
+  for (int k = k_begin + nk * RK; k < k_end; k += RK) {
+    sp.put_tail(lds_ring, k, k_end - k, r0, pr.read_r, t);
+    sq.put_tail(lds_ring + R::kSideP, k, k_end - k, c0, pr.read_c, t);
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < R::kRounds; ks++) {
@@ -609,15 +664,17 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
   const int lr = lane / kLanesPerRow, lc = lane % kLanesPerRow;
   const int row_first = r0 + 32 * FR * wr, col_first = c0 + 32 * FC * wc;
   const int n = pr.cols - (col_first + 8 * lc);
-  const int pieces = n > 0 ? (pr.rows - (row_first + lr) + kStep - 1) / kStep : 0;   // piece i is row row_first + lr + kStep*i
+  // piece i is row row_first + lr + kStep*i; those inside the matrix (a split's sums lie in rows of whole pieces)
+  const int pieces = n >= (OUT == kOutPartial ? 1 : 8) ? (pr.rows - (row_first + lr) + kStep - 1) / kStep : 0;
+  const int edge = WHOLE || OUT == kOutPartial ? 0 : pr.cols & 7, edge_at = pr.cols - edge - col_first;
   typedef std::conditional_t<WHOLE, WholePieces<kO32>, AnyPieces<kO32>> Where;
   const Where where(ep, (size_t)row_first, (size_t)col_first, lr, 8 * lc, kStep);
   Bias8 bias;
-  if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)(col_first + 8 * lc), n);
+  if constexpr (OUT == kOut16) load_bias(bias, ep, (size_t)(col_first + 8 * lc), n >= 8 ? 8 : 0);
   Old8<kO32> old[kAhead];
   auto fetch_old = [&](int u, int i) {
     if constexpr (OUT != kOutPartial) {
-      if (i < pieces && i < kPieces) where.load_old(old[u], ep, i, n);
+      if (i < pieces && i < kPieces) where.load_old(old[u], ep, i);
     }
   };
 #pragma unroll
@@ -652,17 +709,22 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
             o[1] = f32x4{v[u][4], v[u][5], v[u][6], v[u][7]};
           }
         } else {
-          if (i < pieces) where.template finish<F16>(v[u], bias, old[u], ep, i, n);
+          if (i < pieces) where.template finish<F16>(v[u], bias, old[u], ep, i);
           fetch_old(u, i + kAhead);
         }
       }
+    }
+    if constexpr (!WHOLE && OUT != kOutPartial) {
+      if (edge && edge_at >= 0 && edge_at < 32 * FC)
+        edge_elements<F16, kO32>(ep, (size_t)(row_first + 32 * b), (size_t)(col_first + edge_at), edge, pr.rows - (row_first + 32 * b) < 32 ? pr.rows - (row_first + 32 * b) : 32, lane,
+                                 [&](int r, int e) { return cw[r * R::kCStride + (edge_at >> 1) + (e & 3) + (e >> 2) * 16 * FC]; });
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
 
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(FR == 4 ? 1 : 2, FR == 4 ? 1 : 4)))
 void linear_ring_kernel(const LinProd pr, const LinEpi ep) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
   ring_tile<F16, PA, QA, FR, FC, OUT, WHOLE>(pr, ep, blockIdx.x, (int)blockIdx.y, lds_ring);
@@ -702,7 +764,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
   Old8<OUT32> old;
   const Places where = places<OUT32>(ep, row, col, 0, 0, 0);
   load_bias(bias, ep, col, n);
-  load_old<OUT32>(old, ep, where, 0, n);
+  load_old<OUT32>(old, ep, where, 0, n, (int)col);
   finish8<F16, OUT32>(v, bias, old, ep, where, 0, n);
 }
 
@@ -726,7 +788,7 @@ __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, co
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
       const int r = r0 + 4 * u + wave;
-      if (r < job.rows) v[u] = load_piece(job.src + (size_t)r * job.ld + col, job.cols - col);
+      if (r < job.rows) v[u] = load_piece(job.src + (size_t)r * job.ld + col, job.cols - col, col);
     }
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
@@ -825,14 +887,15 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
     for (int i = 0; i < 8; i++) {
       const uint16_t* const p = ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw;
       if (whole) __builtin_memcpy(&s.w[i], p, 16);
-      else s.w[i] = load_piece(p, ALONG ? k_end - (k + 32 * (i & 1) + 8 * q) : (k + 8 * q + i < k_end ? a.cols - (n0 + 8 * c) : 0));
+      else s.w[i] = load_piece(p, ALONG ? k_end - (k + 32 * (i & 1) + 8 * q) : (k + 8 * q + i < k_end ? a.cols - (n0 + 8 * c) : 0),
+                               ALONG ? k + 32 * (i & 1) + 8 * q : n0 + 8 * c);
     }
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
       for (int h = 0; h < (ALONG ? 2 : 1); h++) {
         if (whole) __builtin_memcpy(&s.x[m][h], xp[m] + k + 32 * h, 16);
-        else s.x[m][h] = load_piece(xp[m] + k + 32 * h, k_end - (k + 32 * h + 8 * q));
+        else s.x[m][h] = load_piece(xp[m] + k + 32 * h, k_end - (k + 32 * h + 8 * q), k + 32 * h + 8 * q);
       }
   };
   f32x4 acc[MT][D::kAcc];
@@ -881,7 +944,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
     Bias8 bias;
     Old8<false> old;
     load_bias(bias, ep, (size_t)col, n);
-    load_old<false>(old, ep, where, 0, n);
+    load_old<false>(old, ep, where, 0, n, col);
     finish8<F16, false>(v, bias, old, ep, where, 0, n);
   };
 #pragma unroll
@@ -972,8 +1035,8 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_dz_kernel(const uint16_t
       for (int u = 0; u < ROWS; u++) {
         const int r = m + u * kPass;
         if (r < m1) {
-          gv[u] = load_piece(dY + (size_t)r * lddy + col, n);
-          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)r * ldp + col, n);
+          gv[u] = load_piece(dY + (size_t)r * lddy + col, n, col);
+          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)r * ldp + col, n, col);
         }
       }
 #pragma unroll
@@ -1052,7 +1115,7 @@ struct PairArgs {
   int nx, nw, w_first;   // tiles of each; the workgroups behind them are db's
 };
 template <bool F16, bool OUT32, bool WHOLE>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(1, 1))) void linear_pair_kernel(const PairArgs a) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 4))) void linear_pair_kernel(const PairArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
   const int b = (int)blockIdx.x;
   if (b >= a.nx + a.nw) {
@@ -1114,8 +1177,9 @@ int launch_ring(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) 
   static const hipError_t attr = hipFuncSetAttribute((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>,
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   if (attr != hipSuccess) return hip_fail(attr);
+  const int lds = pr.brief ? Ring<FR, FC>::kBriefLds : kLds;
   hipLaunchKernelGGL((linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>), dim3((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits),
-                     dim3(kBlock), kLds, s, pr, ep);
+                     dim3(kBlock), lds, s, pr, ep);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
@@ -1220,8 +1284,14 @@ RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus
   return best;
 }
 
-// A product of operands that the ring can fetch: C [rows x cols].
-LinProd make_product(const ccn_linear_plan* plan, const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum) {
+// Whether a product does without the ring: short sums (`brief`), where there are more tiles than CUs (four workgroups then share a
+// CU: 65 x 4096 x 4096, dW: 48 instead of 33 us of a whole backward pass), or where an operand would have to be copied first.
+bool brief_product(const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum, int cus) {
+  if (sum > 192) return false;
+  return (size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128) > (size_t)cus || !ring_fetches(p, p_along) || !ring_fetches(q, q_along);
+}
+// A product whose operands the ring can fetch (or a brief one): C [rows x cols].
+LinProd make_product(const ccn_linear_plan* plan, const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum, int cus) {
   LinProd pr;
   pr.p = p.p;
   pr.q = q.p;
@@ -1235,6 +1305,7 @@ LinProd make_product(const ccn_linear_plan* plan, const Operand& p, bool p_along
   pr.tiles_r = (rows + 127) / 128;
   pr.tiles_c = (cols + 127) / 128;
   pr.per_split = 0;
+  pr.brief = brief_product(p, p_along, q, q_along, rows, cols, sum, cus) ? 1 : 0;
   pr.partial = plan->partial;
   return pr;
 }
@@ -1260,8 +1331,9 @@ template <bool F16, bool OUT32, bool WHOLE> int launch_pair(const PairArgs& a, h
   constexpr int kLds = Ring<2, 2>::kLds;
   static const hipError_t attr = hipFuncSetAttribute((const void*)linear_pair_kernel<F16, OUT32, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   if (attr != hipSuccess) return hip_fail(attr);
+  const int lds = a.x.brief && a.w.brief ? Ring<2, 2>::kBriefLds : kLds;
   const int blocks = a.nx + a.nw + (a.db.db ? (a.db.cols + kWave - 1) / kWave : 0);
-  hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE>), dim3((unsigned)blocks), dim3(kBlock), kLds, s, a);
+  hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE>), dim3((unsigned)blocks), dim3(kBlock), lds, s, a);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
 }
@@ -1313,12 +1385,12 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   if (M <= kFewRows) return product_few<F16, false>(plan, X, ldx, W, ldw, M, N, K, ep, di->cu_count, s);
   Operand x{X, ldx, M, K}, w{W, ldw, K, N};
   const bool cx = !ring_fetches(x, true), cw = !ring_fetches(w, false);
-  if (cx || cw) {
+  if ((cx || cw) && !brief_product(x, true, w, false, M, N, K, di->cu_count)) {
     CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
     if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
     if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
   }
-  LinProd pr = make_product(plan, x, true, w, false, M, N, K);
+  LinProd pr = make_product(plan, x, true, w, false, M, N, K, di->cu_count);
   return run_product<F16, true, false>(pr, ep, false, choose_ring(M, N, K, plan->partial_floats, di->cu_count), s);
 }
 
@@ -1347,7 +1419,11 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   // dz goes to the workspace when there is an activation, and when dY is not laid out as the ring wants it
   Operand g{dY, lddy, M, N};
   const bool few = M <= kFewRows;   // dX by the kernel for few rows, which takes anything
-  const bool want_dz = M > 0 && (act != CCN_ACT_NONE ? dX || dW : (dW && !ring_fetches(g, false)) || (dX && !few && !ring_fetches(g, true)));
+  Operand x{X, ldx, M, K}, w{W, ldw, K, N};
+  const bool brief_dx = dX && !few && brief_product(g, true, w, true, M, K, N, di->cu_count);
+  const bool brief_dw = dW && brief_product(x, false, g, false, K, N, M, di->cu_count);
+  const bool want_dz = M > 0 && (act != CCN_ACT_NONE ? dX || dW
+                                                     : (dW && !brief_dw && !ring_fetches(g, false)) || (dX && !few && !brief_dx && !ring_fetches(g, true)));
   if (want_dz) g = Operand{plan->dz, round8((size_t)plan->max_n), M, (int)round8((size_t)N)};
   int chunks = 0;
   bool db_left = db != nullptr;
@@ -1371,8 +1447,7 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   }
   const DbArgs dba{plan->sums, db_left ? db : nullptr, N, chunks, accumulate};
   // operands that the ring cannot fetch: W along its rows for dX, X and dz across them for dW
-  Operand x{X, ldx, M, K}, w{W, ldw, K, N};
-  const bool cw = dX && !few && !ring_fetches(w, true), cx = dW && M > 0 && !ring_fetches(x, false);
+  const bool cw = dX && M > 0 && !few && !brief_dx && !ring_fetches(w, true), cx = dW && M > 0 && !brief_dw && !ring_fetches(x, false);
   const LinEpi dx_ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
   const LinEpi dw_ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
   if (cw || cx) {
@@ -1384,11 +1459,11 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   LinProd px{}, pw{};
   const bool ring_dx = dX && M > 0 && !few;
   if (ring_dx) {
-    px = make_product(plan, g, true, w, true, M, K, N);
+    px = make_product(plan, g, true, w, true, M, K, N, di->cu_count);
     hx = choose_ring(M, K, N, plan->partial_floats, di->cu_count);
   }
   if (dW) {
-    pw = make_product(plan, x, false, g, false, K, N, M);
+    pw = make_product(plan, x, false, g, false, K, N, M, di->cu_count);
     hw = choose_ring(K, N, M, plan->partial_floats, di->cu_count);
   }
   if (ring_dx && dW) {
