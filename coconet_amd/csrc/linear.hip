@@ -103,24 +103,28 @@ __device__ __forceinline__ void act_slopes(int act, const float* z, float* g) {
 // ---- eight neighbouring elements of a row --------------------------------------------------------------------------------
 // gfx950 loads and stores 16 bytes at any 2-byte aligned address; `n` is how many of the eight are there (behind a row's
 // end they are neither read nor written).
-// A piece that ends with its row is loaded as the row's last 16 bytes and shifted down: one load, where loads of single
-// elements under conditions would wait for each other.  back: elements of the row in front of p.
-__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, int n, int back) {
+// Loading is done in two steps, so that many loads can be in flight before the first is looked at: fetch_piece reads the piece at
+// column `col` of a row of `len` elements, or the row's last 16 bytes where the piece would cross (or lie behind) the end;
+// trim_piece then shifts the `n` = len - col elements down and puts zeros behind them (n <= 0: zeros).
+__device__ __forceinline__ u32x4 fetch_piece(const uint16_t* row, int col, int len) {
   u32x4 v = {0u, 0u, 0u, 0u};
-  if (n <= 0) return v;
-  const int s = n >= 8 ? 0 : 8 - n;
-  if (s <= back) {
-    __builtin_memcpy(&v, p - s, 16);
-    if (s) {
-      if (s & 4) v = u32x4{v[2], v[3], 0u, 0u};
-      if (s & 2) v = u32x4{v[1], v[2], v[3], 0u};
-      if (s & 1) v = u32x4{(v[0] >> 16) | (v[1] << 16), (v[1] >> 16) | (v[2] << 16), (v[2] >> 16) | (v[3] << 16), v[3] >> 16};
-    }
-  } else {   // a row of fewer than eight elements
+  if (len >= 8) {   // uniform
+    const int at = len - 8;
+    __builtin_memcpy(&v, row + (col < at ? col : at), 16);
+  } else {
 #pragma unroll
     for (int e = 0; e < 7; e++)
-      if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+      if (e < len) v[e >> 1] |= (uint32_t)row[e] << (16 * (e & 1));   // trimmed to what is there already
   }
+  return v;
+}
+__device__ __forceinline__ u32x4 trim_piece(u32x4 v, int n, int len) {
+  if (__ballot(n < 8) == 0) return v;
+  const int s = n >= 8 || len < 8 ? 0 : 8 - n;   // (a row of fewer than 8 elements is one piece, loaded unshifted)
+  if (s & 4) v = u32x4{v[2], v[3], 0u, 0u};
+  if (s & 2) v = u32x4{v[1], v[2], v[3], 0u};
+  if (s & 1) v = u32x4{(v[0] >> 16) | (v[1] << 16), (v[1] >> 16) | (v[2] << 16), (v[2] >> 16) | (v[3] << 16), v[3] >> 16};
+  if (n <= 0) v = u32x4{0u, 0u, 0u, 0u};
   return v;
 }
 __device__ __forceinline__ void store_piece(uint16_t* p, const u32x4 v, int n) {
@@ -207,7 +211,7 @@ __device__ __forceinline__ void load_old(Old8<OUT32>& x, const LinEpi& ep, const
         if (e < n) x.d[e] = o[e];
     }
   } else {
-    if (ep.resid) x.r = load_piece(reinterpret_cast<const uint16_t*>(w.res + i * w.sres + w.vres), n, back);
+    if (ep.resid) x.r = trim_piece(fetch_piece(reinterpret_cast<const uint16_t*>(w.res + i * w.sres + w.vres) - back, back, back + n), n, back + n);
   }
 }
 template <bool F16, bool OUT32>
@@ -350,19 +354,25 @@ template <bool ALONG, int F, int RK> struct RSide {
     if constexpr (ALONG) load_to_lds(descriptor(base), lds_addr + j * 4096, voff[j], (uint32_t)step * (RK * 2));
     else load_to_lds(descriptor(base + (size_t)step * RK * ld), lds_addr + j * 4096, voff[0], soff0 + j * soffj);
   }
-  // the summed elements from `k` on, `left` of them (RK are used), through registers
-  __device__ __forceinline__ void put_tail(uint8_t* lds, int k, int left, int o0, int outer, int t) const {
+  // the summed elements from `k` on, `left` of them (RK are used), through registers.  outer: as for init
+  struct Held { u32x4 v[kRequests]; };
+  __device__ __forceinline__ void hold(Held& h, int k, int left, int o0, int outer, int t) const {
 #pragma unroll
     for (int i = 0; i < kRequests; i++) {
       const int id = t + 256 * i, row = id / kLanes, c = 8 * ((id % kLanes) ^ swizzle(row));
-      u32x4 v;
       if constexpr (ALONG) {
         const int last = outer - 1 - o0;
-        v = load_piece(base + (size_t)(row < last ? row : last) * ld + k + c, left - c, k + c);
+        h.v[i] = fetch_piece(base + (size_t)(row < last ? row : last) * ld, k + c, k + left);
       } else {
-        v = load_piece(base + (size_t)(k + row) * ld + c, row < left ? outer - o0 - c : 0, o0 + c);
+        h.v[i] = fetch_piece(base - o0 + (size_t)(k + (row < left ? row : left - 1)) * ld, o0 + c, outer);
       }
-      *reinterpret_cast<u32x4*>(lds + id * 16) = v;
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* lds, const Held& h, int k, int left, int o0, int outer, int t) const {
+#pragma unroll
+    for (int i = 0; i < kRequests; i++) {
+      const int id = t + 256 * i, row = id / kLanes, c = 8 * ((id % kLanes) ^ swizzle(row));
+      *reinterpret_cast<u32x4*>(lds + id * 16) = ALONG ? trim_piece(h.v[i], left - c, k + left) : trim_piece(h.v[i], row < left ? outer - o0 - c : 0, outer);
     }
   }
   // fragment f: 32 rows or columns from 32*f of this wavefront's half of the tile, 16 summed elements from 16*ks on
@@ -639,11 +649,16 @@ __device__ __forceinline__ void ring_tile(const LinProd& pr, const LinEpi& ep, c
     __builtin_amdgcn_s_barrier();                // ... everywhere, before the stages are written to
   }
   for (int k = k_begin + nk * RK; k < k_end; k += RK) {
-    sp.put_tail(lds_ring, k, k_end - k, r0, pr.read_r, t);
-    sq.put_tail(lds_ring + R::kSideP, k, k_end - k, c0, pr.read_c, t);
+    typename decltype(sp)::Held hp;
+    typename decltype(sq)::Held hq;
+    sp.hold(hp, k, k_end - k, r0, pr.read_r, t);
+    sq.hold(hq, k, k_end - k, c0, pr.read_c, t);
+    sp.put(lds_ring, hp, k, k_end - k, r0, pr.read_r, t);
+    sq.put(lds_ring + R::kSideP, hq, k, k_end - k, c0, pr.read_c, t);
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < R::kRounds; ks++) {
+      if (k + 16 * ks >= k_end) break;
 #pragma unroll
       for (int f = 0; f < FC; f++) fq[0][f] = read_q(0, f, ks);
 #pragma unroll
@@ -788,12 +803,12 @@ __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, co
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
       const int r = r0 + 4 * u + wave;
-      if (r < job.rows) v[u] = load_piece(job.src + (size_t)r * job.ld + col, job.cols - col, col);
+      if (r < job.rows) v[u] = fetch_piece(job.src + (size_t)r * job.ld, col, job.cols);
     }
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
       const int r = r0 + 4 * u + wave;
-      if (r < job.rows) *reinterpret_cast<u32x4*>(job.dst + (size_t)r * job.ldd + col) = v[u];
+      if (r < job.rows) *reinterpret_cast<u32x4*>(job.dst + (size_t)r * job.ldd + col) = trim_piece(v[u], job.cols - col, job.cols);
     }
   }
 }
@@ -882,21 +897,32 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
     u32x4 w[8], x[MT][ALONG ? 2 : 1];
   };
   auto fetch = [&](Step& s, int k) {
-    const bool whole = inside && k + D::kStep <= k_end;
+    if (inside && k + D::kStep <= k_end) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint16_t* const p = ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw;
-      if (whole) __builtin_memcpy(&s.w[i], p, 16);
-      else s.w[i] = load_piece(p, ALONG ? k_end - (k + 32 * (i & 1) + 8 * q) : (k + 8 * q + i < k_end ? a.cols - (n0 + 8 * c) : 0),
-                               ALONG ? k + 32 * (i & 1) + 8 * q : n0 + 8 * c);
+      for (int i = 0; i < 8; i++) __builtin_memcpy(&s.w[i], ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw, 16);
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < (ALONG ? 2 : 1); h++) __builtin_memcpy(&s.x[m][h], xp[m] + k + 32 * h, 16);
+      return;
     }
+    // a step at an edge: the last rows and pieces again, trimmed to zeros behind the end of the sum
+    auto row_of = [&](int i) { return k + 8 * q + i < k_end ? k + 8 * q + i : k_end - 1; };   // across
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      s.w[i] = ALONG ? fetch_piece(wp[i >> 1] - 8 * q, k + 32 * (i & 1) + 8 * q, k_end) : fetch_piece(a.w + (size_t)row_of(i) * a.ldw, n0 + 8 * c, a.cols);
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int h = 0; h < (ALONG ? 2 : 1); h++) {
-        if (whole) __builtin_memcpy(&s.x[m][h], xp[m] + k + 32 * h, 16);
-        else s.x[m][h] = load_piece(xp[m] + k + 32 * h, k_end - (k + 32 * h + 8 * q), k + 32 * h + 8 * q);
-      }
+      for (int h = 0; h < (ALONG ? 2 : 1); h++) s.x[m][h] = fetch_piece(xp[m] - 8 * q, k + 32 * h + 8 * q, k_end);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      s.w[i] = ALONG ? trim_piece(s.w[i], k_end - (k + 32 * (i & 1) + 8 * q), k_end)
+                     : trim_piece(s.w[i], k + 8 * q + i < k_end ? a.cols - (n0 + 8 * c) : 0, a.cols);
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int h = 0; h < (ALONG ? 2 : 1); h++) s.x[m][h] = trim_piece(s.x[m][h], k_end - (k + 32 * h + 8 * q), k_end);
   };
   f32x4 acc[MT][D::kAcc];
 #pragma unroll
@@ -1035,8 +1061,8 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_dz_kernel(const uint16_t
       for (int u = 0; u < ROWS; u++) {
         const int r = m + u * kPass;
         if (r < m1) {
-          gv[u] = load_piece(dY + (size_t)r * lddy + col, n, col);
-          if (act != CCN_ACT_NONE) zv[u] = load_piece(pre + (size_t)r * ldp + col, n, col);
+          gv[u] = fetch_piece(dY + (size_t)r * lddy, col, N);
+          if (act != CCN_ACT_NONE) zv[u] = fetch_piece(pre + (size_t)r * ldp, col, N);
         }
       }
 #pragma unroll
@@ -1044,10 +1070,10 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_dz_kernel(const uint16_t
         const int r = m + u * kPass;
         if (r < m1) {
           float g[8];
-          unpack<F16>(gv[u], g);
+          unpack<F16>(trim_piece(gv[u], n, N), g);
           if (act != CCN_ACT_NONE) {   // (behind the row's end dY and pre are zeros, and so is the product)
             float z[8];
-            unpack<F16>(zv[u], z);
+            unpack<F16>(trim_piece(zv[u], n, N), z);
             act_slopes(act, z, g);
           }
           if (dz) *reinterpret_cast<u32x4*>(dz + (size_t)r * lddz + col) = pack<F16>(g);
@@ -1139,6 +1165,9 @@ constexpr int kMaxSplits = 16;
   } while (0)
 
 inline size_t round8(size_t n) { return (n + 7) & ~(size_t)7; }
+// Rows of the plan's own matrices start on cache lines: requests of 128 bytes that straddle two of them cost a fifth of a product's
+// time (777 x 1536 x 2048 15.0 us, 777 x 1544 x 2048 18.7).
+inline size_t pitch(size_t n) { return (n + 63) & ~(size_t)63; }
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -1340,7 +1369,7 @@ template <bool F16, bool OUT32, bool WHOLE> int launch_pair(const PairArgs& a, h
 
 // Aligned copies of up to two operands into the plan (nullptr: none).
 int pack(const Operand* a, int a_cols, uint16_t* a_to, const Operand* b, int b_cols, uint16_t* b_to, hipStream_t s) {
-  const auto job = [](const Operand* o, int cols, uint16_t* to) { return o ? PackJob{o->p, to, o->ld, round8((size_t)cols), o->rows, cols} : PackJob{}; };
+  const auto job = [](const Operand* o, int cols, uint16_t* to) { return o ? PackJob{o->p, to, o->ld, pitch((size_t)cols), o->rows, cols} : PackJob{}; };
   PackJob x = job(a, a_cols, a_to), y = job(b, b_cols, b_to);
   if (!a) {
     x = y;
@@ -1387,8 +1416,8 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   const bool cx = !ring_fetches(x, true), cw = !ring_fetches(w, false);
   if ((cx || cw) && !brief_product(x, true, w, false, M, N, K, di->cu_count)) {
     CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
-    if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
-    if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
+    if (cx) x = Operand{plan->px, pitch((size_t)K), M, (int)round8((size_t)K)};
+    if (cw) w = Operand{plan->pw, pitch((size_t)N), K, (int)round8((size_t)N)};
   }
   LinProd pr = make_product(plan, x, true, w, false, M, N, K, di->cu_count);
   return run_product<F16, true, false>(pr, ep, false, choose_ring(M, N, K, plan->partial_floats, di->cu_count), s);
@@ -1424,7 +1453,7 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const bool brief_dw = dW && brief_product(x, false, g, false, K, N, M, di->cu_count);
   const bool want_dz = M > 0 && (act != CCN_ACT_NONE ? dX || dW
                                                      : (dW && !brief_dw && !ring_fetches(g, false)) || (dX && !few && !brief_dx && !ring_fetches(g, true)));
-  if (want_dz) g = Operand{plan->dz, round8((size_t)plan->max_n), M, (int)round8((size_t)N)};
+  if (want_dz) g = Operand{plan->dz, pitch((size_t)N), M, (int)round8((size_t)N)};
   int chunks = 0;
   bool db_left = db != nullptr;
   if (M > 0 && (want_dz || db)) {
@@ -1452,8 +1481,8 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const LinEpi dw_ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
   if (cw || cx) {
     CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
-    if (cx) x = Operand{plan->px, round8((size_t)K), M, (int)round8((size_t)K)};
-    if (cw) w = Operand{plan->pw, round8((size_t)N), K, (int)round8((size_t)N)};
+    if (cx) x = Operand{plan->px, pitch((size_t)K), M, (int)round8((size_t)K)};
+    if (cw) w = Operand{plan->pw, pitch((size_t)N), K, (int)round8((size_t)N)};
   }
   RingPlan hx{}, hw{};
   LinProd px{}, pw{};
@@ -1533,9 +1562,9 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t few = (size_t)kFewMaxSplits * few_cols * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
   p->partial_floats = few > p->partial_floats ? few : p->partial_floats;
   const size_t strips = few_cols / 64;
-  hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * round8((size_t)max_N) * sizeof(uint16_t));
-  if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * round8((size_t)max_K) * sizeof(uint16_t));
-  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, (size_t)max_K * round8((size_t)max_N) * sizeof(uint16_t));
+  hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * pitch((size_t)max_N) * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * pitch((size_t)max_K) * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, (size_t)max_K * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->counters, strips * sizeof(uint32_t));
