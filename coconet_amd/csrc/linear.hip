@@ -1033,6 +1033,102 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
   }
 }
 
+// Up to 4 rows, forward: strips of 32 columns and no split of the sum over workgroups, whose joining costs as long as the reading of
+// a small W (1 x 1024 x 8192: 8.0 us).  A wavefront's step is 128 summed elements x 32 columns: lane (kr, c2) = (lane/4, lane%4)
+// loads rows 8kr .. 8kr+7 of columns 8*c2 .. and turns the 8 x 8 block over as above.  One v_mfma_f32_16x16x32 then has the four
+// column groups of four different eights of summed elements (h = kr%4) as its rows, and four rows of X with the same four eights
+// as its columns: of its 16 x 16 results the 4 x 4 blocks with equal h are sums, the others are dropped.  The wavefronts of a
+// workgroup take steps in turn; two neighbouring strips, which share every cache line of W, are dealt to one XCD.
+constexpr int kOneRows = 4, kOneWidth = 32, kOneStep = 128, kOneSum = 2048;
+template <bool F16, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void linear_one_kernel(const FewArgs a, const LinEpi ep) {
+  __shared__ __attribute__((aligned(16))) float red[WAVES * 4][kOneRows * kOneWidth + 4];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), kr = lane >> 2, c2 = lane & 3;
+  const int b = (int)blockIdx.x, full = (int)gridDim.x & ~15;
+  const int strip = b < full ? (b & ~15) + 2 * (b & 7) + ((b >> 3) & 1) : b;
+  const int n0 = strip * kOneWidth;
+  const uint16_t* const xrow = a.x + (size_t)(c2 < a.rows ? c2 : a.rows - 1) * a.ldx;
+  const bool inside = n0 + kOneWidth <= a.cols;
+  struct Step { u32x4 w[8], x; };
+  auto fetch = [&](Step& s, int k) {
+    const int k8 = k + 8 * kr;
+    if (inside && k + kOneStep <= a.sum) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) __builtin_memcpy(&s.w[i], a.w + (size_t)(k8 + i) * a.ldw + n0 + 8 * c2, 16);
+      __builtin_memcpy(&s.x, xrow + k8, 16);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) s.w[i] = fetch_piece(a.w + (size_t)(k8 + i < a.sum ? k8 + i : a.sum - 1) * a.ldw, n0 + 8 * c2, a.cols);
+    s.x = fetch_piece(xrow, k8, a.sum);
+#pragma unroll
+    for (int i = 0; i < 8; i++) s.w[i] = trim_piece(s.w[i], k8 + i < a.sum ? a.cols - (n0 + 8 * c2) : 0, a.cols);
+    s.x = trim_piece(s.x, a.sum - k8, a.sum);
+  };
+  f32x4 acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[e] = __builtin_amdgcn_perm(s.w[2 * e + 1][j >> 1], s.w[2 * e][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+      acc[j] = mfma16<F16>(f, s.x, acc[j]);
+    }
+  };
+  {
+    constexpr int kTurn = WAVES * kOneStep;
+    Step s0, s1;
+    int k = wave * kOneStep;
+    if (k < a.sum) fetch(s0, k);
+    for (; k < a.sum; k += 2 * kTurn) {
+      if (k + kTurn < a.sum) fetch(s1, k + kTurn);
+      multiply(s0);
+      if (k + 2 * kTurn < a.sum) fetch(s0, k + 2 * kTurn);
+      if (k + kTurn < a.sum) multiply(s1);
+    }
+  }
+  // lane (h, h', m) = (lane/16, lane/4%4, lane%4) with h == h' holds row m, columns 8i + j, in acc[j][i]
+  const int h = lane >> 4, m = lane & 3;
+  if (h == ((lane >> 2) & 3)) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+        *reinterpret_cast<f32x4*>(&red[wave * 4 + h][m * kOneWidth + 8 * i + 4 * u]) =
+            f32x4{acc[4 * u][i], acc[4 * u + 1][i], acc[4 * u + 2][i], acc[4 * u + 3][i]};
+  }
+  __syncthreads();
+  // 128 sums of 4*WAVES: four threads each, then one
+  const int at = t & 127, part = t >> 7;
+  constexpr int kParts = WAVES / 2;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4 * WAVES / kParts; i++) s += red[part * (4 * WAVES / kParts) + i][at];
+  __syncthreads();
+  red[part][at] = s;
+  __syncthreads();
+  const int row = t >> 2, col = n0 + 8 * (t & 3), n = a.cols - col;
+  if (t < 16 && row < a.rows && n > 0) {
+    float v[8];
+    __builtin_memcpy(v, &red[0][8 * t], 32);
+#pragma unroll
+    for (int p = 1; p < kParts; p++) {
+      float x[8];
+      __builtin_memcpy(x, &red[p][8 * t], 32);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += x[e];
+    }
+    const Places where = places<false>(ep, (size_t)row, (size_t)col, 0, 0, 0);
+    Bias8 bias;
+    Old8<false> old;
+    load_bias(bias, ep, (size_t)col, n);
+    load_old<false>(old, ep, where, 0, n, col);
+    finish8<F16, false>(v, bias, old, ep, where, 0, n);
+  }
+}
+
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
 // dz = dY * act'(pre), rounded to the operands' type into the workspace (aligned rows, zeros up to a multiple of 8 columns), and
 // fp32 sums over a chunk of rows of the unrounded dz.  LANES lanes share a row's strip of 8*LANES columns, a workgroup of WAVES
@@ -1259,6 +1355,17 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   a.cols = cols;
   a.sum = sum;
   a.counters = plan->counters;
+  if constexpr (!ALONG) {
+    // (one row, us with this kernel / with the other: 1024 x 1024 4.8 / 5.9, 2048 x 1024 6.6 / 7.0, 1024 x 8192 6.5 / 8.5, but
+    // 4096 x 1024 8.8 / 7.5 and 4096 x 4096 13.8 / 10.8: a CU alone reads a long strip too slowly)
+    const int narrow = (cols + kOneWidth - 1) / kOneWidth;
+    if (rows <= kOneRows && sum <= kOneSum) {
+      if (narrow >= cus) hipLaunchKernelGGL((linear_one_kernel<F16, 8>), dim3((unsigned)narrow), dim3(8 * kWave), 0, s, a, ep);
+      else hipLaunchKernelGGL((linear_one_kernel<F16, 16>), dim3((unsigned)narrow), dim3(16 * kWave), 0, s, a, ep);
+      CCN_HIP(hipGetLastError());
+      return CCN_OK;
+    }
+  }
   const int strips = (cols + D::kWidth - 1) / D::kWidth, steps = (sum + D::kStep - 1) / D::kStep;
   // a workgroup for every CU, each wavefront with a step at least
   int splits = (cus + strips - 1) / strips;
