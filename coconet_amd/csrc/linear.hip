@@ -1133,7 +1133,7 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_one_kernel(const FewArgs
 // dz = dY * act'(pre), rounded to the operands' type into the workspace (aligned rows, zeros up to a multiple of 8 columns), and
 // fp32 sums over a chunk of rows of the unrounded dz.  LANES lanes share a row's strip of 8*LANES columns, a workgroup of WAVES
 // wavefronts works on WAVES * 64/LANES rows at a time, ROWS times that in flight.
-//   64, 4, 4     many rows: a strip of 512 columns, chunks of rows over the chip, linear_db_kernel adds the chunks up
+//   64, 4, 2     many rows (8192 x 4096, gelu_tanh: 45 us; 48 with four in flight): a strip of 512 columns, chunks of rows over the chip, linear_db_kernel adds the chunks up
 //   16, 16, 1    up to 64 rows, all at once: one chunk, its sums are db itself (`add`: added to it)
 template <bool F16, int LANES, int WAVES, int ROWS>
 __global__ __launch_bounds__(WAVES * kWave) void linear_dz_kernel(const uint16_t* __restrict__ dY, const size_t lddy,
@@ -1576,7 +1576,7 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
       if (per < 4) per = 4;
       if ((M + per - 1) / per > kMaxChunks) per = (M + kMaxChunks - 1) / kMaxChunks;
       chunks = (M + per - 1) / per;
-      hipLaunchKernelGGL((linear_dz_kernel<F16, 64, 4, 4>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp, to, g.ld,
+      hipLaunchKernelGGL((linear_dz_kernel<F16, 64, 4, 2>), dim3((unsigned)strips, (unsigned)chunks), dim3(kBlock), 0, s, dY, lddy, pre, ldp, to, g.ld,
                          db ? plan->sums : nullptr, M, N, act, per, 0);
     }
     CCN_HIP(hipGetLastError());
