@@ -10,6 +10,7 @@
 // 16-byte reads, an "across" tile through the transposing ds_read_b64_tr_b16.
 #include "ccn_common.hpp"
 
+#include <atomic>
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -1008,7 +1009,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
     }
   }
   if (MT > 1 || splits == 1) return;
-  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wavefront's partial sums have arrived
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's partial sums have arrived
   __syncthreads();
   if (t == 0) arrived = __hip_atomic_fetch_add(a.counters + strip, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
@@ -1296,12 +1297,21 @@ bool ring_fetches(const Operand& o, bool along) {
   return aligned16(o.p) && o.ld % 8 == 0 && o.ld <= kRMaxLd && (along || o.extent % 8 == 0);
 }
 
+// More than 64 KiB of dynamic LDS have to be asked for, once for every kernel and device.
+int allow_lds(const void* kernel, int bytes, std::atomic<uint32_t>& devices) {
+  int dev = -1;
+  CCN_HIP(hipGetDevice(&dev));
+  if (dev < 0 || dev > 31) return CCN_ENODEV;
+  if (devices.load(std::memory_order_relaxed) >> dev & 1u) return CCN_OK;
+  CCN_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  devices.fetch_or(1u << dev, std::memory_order_relaxed);
+  return CCN_OK;
+}
 template <bool F16, bool PA, bool QA, int FR, int FC, int OUT, bool WHOLE>
 int launch_ring(const LinProd& pr, const LinEpi& ep, int splits, hipStream_t s) {
   constexpr int kLds = Ring<FR, FC>::kLds;
-  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (attr != hipSuccess) return hip_fail(attr);
+  static std::atomic<uint32_t> devices{0};
+  CCN_TRY(allow_lds((const void*)linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>, kLds, devices));
   const int lds = pr.brief ? Ring<FR, FC>::kBriefLds : kLds;
   hipLaunchKernelGGL((linear_ring_kernel<F16, PA, QA, FR, FC, OUT, WHOLE>), dim3((unsigned)(pr.tiles_r * pr.tiles_c), (unsigned)splits),
                      dim3(kBlock), lds, s, pr, ep);
@@ -1465,8 +1475,8 @@ int run_product(LinProd& pr, const LinEpi& ep, bool out32, RingPlan how, hipStre
 }
 template <bool F16, bool OUT32, bool WHOLE> int launch_pair(const PairArgs& a, hipStream_t s) {
   constexpr int kLds = Ring<2, 2>::kLds;
-  static const hipError_t attr = hipFuncSetAttribute((const void*)linear_pair_kernel<F16, OUT32, WHOLE>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (attr != hipSuccess) return hip_fail(attr);
+  static std::atomic<uint32_t> devices{0};
+  CCN_TRY(allow_lds((const void*)linear_pair_kernel<F16, OUT32, WHOLE>, kLds, devices));
   const int lds = a.x.brief && a.w.brief ? Ring<2, 2>::kBriefLds : kLds;
   const int blocks = a.nx + a.nw + (a.db.db ? (a.db.cols + kWave - 1) / kWave : 0);
   hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE>), dim3((unsigned)blocks), dim3(kBlock), lds, s, a);
@@ -1648,7 +1658,7 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   if (!out) return CCN_EINVAL;
   *out = nullptr;
   if (max_M < 1 || max_N < 1 || max_K < 1) return CCN_EINVAL;
-  if ((size_t)max_N > kMaxLd || (size_t)max_K > kMaxLd) return CCN_ERANGE;
+  if ((size_t)max_N > kRMaxLd || (size_t)max_K > kRMaxLd || max_M > (1 << 30)) return CCN_ERANGE;
   const DeviceInfo* di = nullptr;
   CCN_TRY(current_device_info(&di));
   ccn_linear_plan* const p = new (std::nothrow) ccn_linear_plan();

@@ -313,9 +313,11 @@ int  ccn_matmul_f16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, in
  *
  *      X, W, resid, Y, pre, dY, dX: bf16 (_bf16) or IEEE-half (_f16) bit patterns, row-major; ld*: elements from one row to
  *      the next (at least the row's length).  bias, db: fp32.  dW: the operands' type, or fp32 (dw_type CCN_TYPE_F32).
- *      Any M >= 0, N >= 1, K >= 1, any alignment that the element type allows (fp32 arrays 4 bytes, 16-bit ones 2): whole
- *      rows of 16-byte pieces on the fast kernels, everything else on the same matrix cores at a lower rate.  M = 0 (an
- *      empty batch): forward writes nothing; backward writes zero gradients, or leaves them when accumulating.
+ *      Any M >= 0, N >= 1, K >= 1 (N, K up to 2^21), any alignment that the element type allows (fp32 arrays 4 bytes, 16-bit
+ *      ones 2).  Operands with 16-byte aligned rows (ld a multiple of 8; the width too, of W in forward and of X in backward)
+ *      are read as they lie; the call first copies others into the plan, two passes over them.  Up to 64 rows (serving) the
+ *      weights are read once, as they lie.  M = 0 (an empty batch): forward writes nothing; backward writes zero gradients,
+ *      or leaves them when accumulating.
  *      Products are accumulated in fp32 on the matrix cores, Y is computed from the fp32 z, every output is rounded to
  *      nearest even once.  dz is rounded to the operands' type before the two products when there is an activation (the
  *      matrix cores take 16-bit operands); db is summed in fp32 from the unrounded dz.  Sums run in a fixed order: the
@@ -327,10 +329,11 @@ int  ccn_matmul_f16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, in
  *      Y may be resid itself (same address and ld); otherwise outputs must not overlap inputs or each other.
  *      Rows and columns outside the matrices (the padding of a row) are neither read for the result nor written.
  *
- *      A plan owns the workspace (dz, partial sums) for calls of up to max_M x max_N x max_K; one plan serves any number of
- *      layers of up to that size.  Calls on one plan must be ordered (one stream, or events), also calls replayed from
- *      recordings.  Every call on a plan can be recorded.  CCN_ERANGE: a size beyond the plan's, or rows too long for
- *      32-bit addressing inside a tile (ld > 2^22). ---- */
+ *      A plan owns the workspace for calls of up to max_M x max_N x max_K: dz and aligned copies of X and W (2 bytes for each
+ *      of their elements, rows rounded up to 64) and up to 128 MiB of partial sums; one plan serves any number of layers of up
+ *      to that size.  Calls on one plan must be ordered (one stream, or events), also calls replayed from
+ *      recordings.  Every call on a plan can be recorded.  CCN_ERANGE: a size beyond the plan's, N or K of a plan beyond 2^21
+ *      or M beyond 2^30, ld beyond 2^22. ---- */
 #define CCN_ACT_NONE      0
 #define CCN_ACT_RELU      1
 #define CCN_ACT_GELU      2

@@ -20,7 +20,8 @@ def test_linear_refusals():
     for dims in ((0, 8, 8), (8, 0, 8), (8, 8, -1)):
         assert lib.ccn_linear_plan_create(*dims, C.byref(plan)) == capi.CCN_EINVAL and not plan.value
     assert lib.ccn_linear_plan_create(8, 8, 8, None) == capi.CCN_EINVAL
-    assert lib.ccn_linear_plan_create(8, (1 << 22) + 1, 8, C.byref(plan)) == capi.CCN_ERANGE
+    for dims in ((8, (1 << 21) + 1, 8), (8, 8, (1 << 21) + 1), ((1 << 30) + 1, 8, 8)):
+        assert lib.ccn_linear_plan_create(*dims, C.byref(plan)) == capi.CCN_ERANGE
     assert lib.ccn_linear_plan_destroy(None) == capi.CCN_OK
     for t in ("bf16", "f16"):
         assert getattr(lib, "ccn_linear_" + t)(None, 0x1000, 8, 0x1000, 8, None, None, 0, 0x1000, 8, None, 0, 8, 8, 8, 0, None) == capi.CCN_EINVAL

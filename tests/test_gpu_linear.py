@@ -116,6 +116,7 @@ def forward_case(ccn, M, N, K, act, half, bias=True, resid=True, keep=True, pad=
 
 SHAPES = [(1, 1, 1), (1, 8, 8), (1, 64, 1024), (1, 8192, 1024), (2, 257, 63), (3, 130, 4099), (5, 2049, 515), (15, 1000, 333), (16, 4096, 2048), (17, 72, 4096),
           (31, 777, 129), (32, 512, 64), (33, 520, 1030), (48, 1024, 4096), (64, 640, 8192), (65, 128, 64), (127, 129, 65), (128, 128, 128), (129, 255, 1),
+          (3, 1000, 130), (4, 33, 2047), (4, 7, 5), (100, 5, 300), (100, 300, 5), (300, 3, 5), (70, 7, 200),
           (255, 256, 32), (256, 264, 40), (300, 301, 302), (512, 512, 1024), (777, 1025, 513), (1000, 2056, 1032), (2048, 1024, 96)]
 
 
@@ -141,7 +142,8 @@ def test_forward_strides_and_alignments(ccn, M, N, K, pad, shift):
     forward_case(ccn, M, N, K, "gelu", True, pad=pad, shift=shift)
 
 
-@pytest.mark.parametrize("M,N,K,half", [(4096, 4096, 256, False), (4096, 4104, 136, True), (4100, 4096, 520, False), (8192, 2048, 1024, False), (3000, 6000, 1000, True)])
+@pytest.mark.parametrize("M,N,K,half", [(4096, 4096, 256, False), (4096, 4104, 136, True), (4100, 4096, 520, False), (8192, 2048, 1024, False), (3000, 6000, 1000, True),
+                                         (2048, 4096, 1024, False), (2040, 4000, 1000, True), (2000, 4001, 1003, False)])
 def test_forward_large(ccn, M, N, K, half):
     forward_case(ccn, M, N, K, "gelu_tanh", half, resid=True, keep=True)
 
@@ -243,7 +245,8 @@ def backward_case(ccn, M, N, K, act, half, dw32=False, accumulate=False, pad=0, 
 
 
 BSHAPES = [(1, 1, 1), (1, 64, 128), (2, 513, 70), (7, 130, 1031), (16, 1024, 512), (33, 65, 129), (64, 256, 256), (128, 128, 128), (130, 257, 131), (255, 1000, 72),
-           (256, 512, 1024), (515, 264, 2049), (1001, 515, 1025), (2048, 256, 256), (4097, 136, 200)]
+           (256, 512, 1024), (515, 264, 2049), (1001, 515, 1025), (2048, 256, 256), (4097, 136, 200),
+           (300, 3, 5), (100, 5, 300), (500, 300, 5), (1000, 6, 40), (20, 2100, 2060), (190, 2100, 2053)]
 
 
 @pytest.mark.parametrize("M,N,K", BSHAPES)
@@ -275,7 +278,8 @@ def test_backward_parts(ccn, want):
     backward_case(ccn, 150, 264, 136, "none", False, want=want)
 
 
-@pytest.mark.parametrize("M,N,K,act,half", [(4096, 4096, 4096, "gelu", False), (8192, 2048, 2056, "none", False), (4100, 4104, 4096, "relu", True)])
+@pytest.mark.parametrize("M,N,K,act,half", [(4096, 4096, 4096, "gelu", False), (8192, 2048, 2056, "none", False), (4100, 4104, 4096, "relu", True),
+                                              (1024, 4096, 2048, "none", False), (1000, 4090, 2040, "none", True), (1000, 4001, 2003, "silu", False)])
 def test_backward_large(ccn, M, N, K, act, half):
     backward_case(ccn, M, N, K, act, half, dw32=act == "none")
 
