@@ -29,6 +29,7 @@ namespace ccn {
 constexpr int kAwBlock = 256;          // elements of one scale
 constexpr int kAwLane = kAwBlock / kWave;   // 4 elements of a block per lane: every access of a wavefront is one contiguous piece
 constexpr int kAwGroupShift = 5;       // blocks per entry of the coarse table: 32
+constexpr uint32_t kAwGridX = 1u << 25;   // workgroups in a row of the grid: 2^31 of the 2^32 - 1 threads that a launch may have there
 constexpr float kE4m3Max = 448.0f, kE4m3Tiny = 0.001953125f;
 constexpr float kAwFlush = 7.888609052210118e-31f;   // 2^-100: a block whose largest |m| is below it is held as zeros
 
@@ -305,7 +306,7 @@ int adamw_sync_table(ccn_adamw_plan* p, const void* const* g, int P, float* cons
 
 template <int G, int CAP>
 int adamw_launch(const ccn_adamw_plan* p, const AdamwArgs& a, const AdamwPrm& k, hipStream_t s) {
-  const uint32_t gx = a.blocks < 0x40000000u ? a.blocks : 0x40000000u;
+  const uint32_t gx = a.blocks < kAwGridX ? a.blocks : kAwGridX;
   const dim3 grid(gx, (a.blocks + gx - 1) / gx);
   // Wavefronts kept resident per CU, by a request for LDS that the kernel never touches (0: as many as fit, 32).  GB/s at
   // 2^26 elements with no cap / 24 / 20 / 16 / 13 wavefronts: fp32 moments and fp32 gradients 6095 / 6199 / 6391 / 6465 /
@@ -448,7 +449,7 @@ int adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int b
     if (counts[b] == 0) continue;
     if (counts[b] > ((size_t)1 << 48)) return CCN_ERANGE;
     const uint64_t nb = ((uint64_t)counts[b] + kAwBlock - 1) / kAwBlock;
-    if (blocks + nb >= 0xffffffffull) return CCN_ERANGE;   // block numbers are 32-bit
+    if (blocks + nb > 0x80000000ull) return CCN_ERANGE;   // block numbers are 32-bit, also those of a grid's last row
     const uint32_t i = (uint32_t)bufs.size();
     bufs.push_back(AdamwBuf{(uint64_t)counts[b], (uint32_t)blocks, decay ? decay[b] : 1.0f});
     first.push_back((uint32_t)blocks);

@@ -1380,8 +1380,8 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   // a workgroup for every CU, each wavefront with a step at least
   int splits = (cus + strips - 1) / strips;
   if (splits > steps / kFewWaves) splits = steps / kFewWaves;
-  if ((size_t)splits * (size_t)rows * (size_t)(cols + 7) > ((size_t)1 << 28)) splits = 1;   // 32-bit offsets into the partial sums
   if (splits > kFewMaxSplits) splits = kFewMaxSplits;
+  if ((size_t)(splits > 1 ? splits : 0) * (size_t)rows * round8((size_t)cols) > plan->partial_floats) splits = 1;
   if (splits < 1) splits = 1;
   a.per_split = ((steps + splits - 1) / splits) * D::kStep;
   splits = (sum + a.per_split - 1) / a.per_split;   // no empty split
@@ -1676,7 +1676,9 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t need[3] = {floats(max_M, max_N, max_K), floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
   for (const size_t f : need) p->partial_floats = f > p->partial_floats ? f : p->partial_floats;
   const size_t few_cols = ((size_t)(max_N > max_K ? max_N : max_K) + 127) & ~(size_t)127;
-  const size_t few = (size_t)kFewMaxSplits * few_cols * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
+  // A split sum of few rows has fewer than two workgroups for every CU, over all its splits, of up to 128 outputs each.
+  const size_t few_most = (size_t)kFewMaxSplits * few_cols, few_cap = 2 * (size_t)di->cu_count * 128;
+  const size_t few = (few_most < few_cap ? few_most : few_cap) * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
   p->partial_floats = few > p->partial_floats ? few : p->partial_floats;
   const size_t strips = few_cols / 64;
   hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * pitch((size_t)max_N) * sizeof(uint16_t));

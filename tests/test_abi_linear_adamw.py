@@ -40,6 +40,8 @@ def test_adamw_refusals():
     assert lib.ccn_adamw_plan_create(counts, None, 2, 32, None) == capi.CCN_EINVAL
     huge = (C.c_size_t * 1)(1 << 62)
     assert lib.ccn_adamw_plan_create(huge, None, 1, 32, C.byref(plan)) == capi.CCN_ERANGE and not plan.value
+    many = (C.c_size_t * 3)(1 << 38, 1 << 38, 1)      # 2^31 blocks and one more
+    assert lib.ccn_adamw_plan_create(many, None, 3, 32, C.byref(plan)) == capi.CCN_ERANGE and not plan.value
     assert lib.ccn_adamw_plan_destroy(None) == capi.CCN_OK
     assert lib.ccn_adamw_plan_sizes(None, None, None) == capi.CCN_EINVAL
     tbl = (C.c_void_p * 4)(*([0x1000] * 4))

@@ -392,3 +392,38 @@ def test_refusals(ccn):
     empty.step(empty.tables([[None, None]], [None, None]), None, None, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, overflow_flag=c.flag)
     torch.cuda.synchronize()
     assert c.flag.item() == 0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_offsets_past_32_bits(ccn, bits):
+    """More blocks than a row of the grid takes (2^33 elements; 2^24 with fp32 moments: 2^32): tensors with the same
+    values end alike, whichever their place."""
+    each, n = (1 << 30, 8) if bits == 8 else (1 << 29, 8)
+    counts = [each] * n + [1000]
+    need = sum(counts) * (4 + (2 if bits == 8 else 8)) + 2 * each
+    if torch.cuda.mem_get_info()[0] < need + (8 << 30):
+        pytest.skip("not enough memory free")
+    g = torch.randn(each, device=DEV, generator=gen(3)).bfloat16()
+    first = torch.randn(each, device=DEV, generator=gen(4))
+    w = [first.clone() for _ in range(n)] + [first[:1000].clone()]
+    plan = ccn.AdamWPlan(counts, bits=bits)
+    m = torch.zeros(plan.elems, device=DEV, dtype=torch.uint8 if bits == 8 else torch.float32)
+    v = torch.zeros_like(m)
+    scales = torch.zeros(2 * plan.blocks, device=DEV) if bits == 8 else None
+    h = HYPER
+    plan.step(plan.tables([[g] * n + [g[:1000]]], w), m, v, h["lr"], h["beta1"], h["beta2"], h["eps"], h["wd"], 1, scales=scales, g_type="bf16")
+    torch.cuda.synchronize()
+    assert not torch.equal(w[0], first)
+    for i in range(1, n):
+        assert torch.equal(w[i], w[0]), i
+        assert torch.equal(m[i * each:(i + 1) * each], m[:each]) and torch.equal(v[i * each:(i + 1) * each], v[:each]), i
+    assert torch.equal(w[n], w[0][:1000]) and torch.equal(m[n * each:][:512], m[:512])
+    plan.close()
+    # the first tensor alone, as the other tests check it
+    plan = ccn.AdamWPlan([each], bits=bits)
+    m1, v1 = torch.zeros_like(m[:each]), torch.zeros_like(m[:each])
+    s1 = torch.zeros(2 * plan.blocks, device=DEV) if bits == 8 else None
+    plan.step(plan.tables([[g]], [first]), m1, v1, h["lr"], h["beta1"], h["beta2"], h["eps"], h["wd"], 1, scales=s1, g_type="bf16")
+    torch.cuda.synchronize()
+    assert torch.equal(first, w[0]) and torch.equal(m1, m[:each]) and torch.equal(v1, v[:each])
+    plan.close()

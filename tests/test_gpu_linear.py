@@ -334,6 +334,32 @@ def test_empty_batch(ccn):
     plan.close()
 
 
+@pytest.mark.parametrize("M,N,K", [(2112, 136, 200), (40, 136, 2112), (3, 136, 2048), (2100, 129, 201)])
+def test_rows_far_apart(ccn, M, N, K):
+    """Rows 2^21 elements apart: offsets inside the matrices pass 2^32, inside a tile 2^30."""
+    g, ld, rows = gen(M), 1 << 21, max(M, K)
+    big = [torch.empty(rows * ld, device=DEV, dtype=torch.bfloat16) for _ in range(4)]
+    far = [b.view(rows, ld) for b in big]
+    X, W, G, R = matrix(g, M, K, False), matrix(g, K, N, False, 0.1), matrix(g, M, N, False), matrix(g, M, N, False)
+    b = torch.randn(N, device=DEV, generator=g)
+    plan = ccn.LinearPlan(M, N, K)
+    y, pre = (torch.empty(M, N, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    dx, dw, db, db2 = torch.empty_like(X, memory_format=torch.contiguous_format), torch.empty(K, N, device=DEV, dtype=torch.bfloat16), torch.empty(N, device=DEV), torch.empty(N, device=DEV)
+    plan.forward(X, W, b, R, y, M, N, K, act="silu", pre=pre)
+    plan.backward(G, pre, X, W, dx, dw, db, M, N, K, act="silu")
+    x2, w2, y2, p2 = far[0][:M, :K], far[1][:K, :N], far[2][:M, :N], far[3][:M, :N]
+    x2.copy_(X), w2.copy_(W), y2.copy_(R)
+    plan.forward(x2, w2, b, y2, y2, M, N, K, act="silu", pre=p2, ldx=ld, ldw=ld, ldr=ld, ldy=ld, ldp=ld)
+    torch.cuda.synchronize()
+    assert torch.equal(y, y2) and torch.equal(pre, p2)
+    g2, dx2, dw2 = far[2][:M, 4096:4096 + N], far[2][:M, 8192:8192 + K], far[3][:K, 8192:8192 + N]
+    g2.copy_(G)
+    plan.backward(g2, p2, x2, w2, dx2, dw2, db2, M, N, K, act="silu", lddy=ld, ldp=ld, ldx=ld, ldw=ld, lddx=ld, lddw=ld)
+    torch.cuda.synchronize()
+    assert torch.equal(dx, dx2) and torch.equal(dw, dw2) and torch.equal(db, db2)
+    plan.close()
+
+
 def test_residual_in_place(ccn):
     """Y may be the residual itself."""
     for M, N, K in ((1, 200, 300), (40, 1024, 512), (300, 264, 100), (512, 4096, 128)):
