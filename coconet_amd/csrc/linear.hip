@@ -823,11 +823,14 @@ __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, co
 //   along (dX)         64 rows of W x 64 summed elements, fragments as they lie; row tiles are dealt so that a lane ends up
 //                      with eight neighbouring outputs
 // The four wavefronts of a workgroup take steps in turn and add up through LDS.  A strip whose sum is split over workgroups:
-// up to 16 rows, the workgroup that arrives last finishes it: partial sums go out and come back with the agent-scope bit (sc1:
-// written through to, and read from, where the XCDs are coherent), complete (vmcnt 0) before the workgroup counts itself in;
-// splits are added in ascending order whoever does it, and the counter is back at zero when the call ends.  With more rows one
-// workgroup would have too much to add (64 x 1024 x 1024: 17.9 us): the join kernel does it.
-constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16;
+// up to 16 rows, the one that arrives last finishes (each wavefront for the rows that it has held in every split): partial sums
+// go out and come back with the agent-scope bit (sc1: written through to, and read from, where the XCDs are coherent), complete
+// (vmcnt 0) before the wavefront counts itself in; splits are added in ascending order whoever does it, and the counter is back
+// at zero when the call ends.  With more rows a wavefront would have too much to add (64 x 1024 x 1024: 17.9 us): the join
+// kernel does it.  16 x 8192 x 4096 (67 MB of weights): 15.7 us, 4.3 TB/s; reading W alone takes this grid 10.5, X 0.8, the
+// split sums' way through memory 2.5.
+constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16, kFewCounter = 32;
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
 template <bool ALONG> struct Few {
   static constexpr int kWidth = ALONG ? 64 : 128;   // outputs of a strip
   static constexpr int kStep = ALONG ? 64 : 32;     // summed elements of a wavefront's step
@@ -840,8 +843,9 @@ struct FewArgs {
   int rows, cols, sum;
   int per_split;        // a multiple of kStep
   float* partial;       // [splits][rows][cols rounded up to 8]
-  uint32_t* counters;   // [strips], zero
+  uint32_t* counters;   // [strips][kFewWaves], zero, each on a cache line of its own (16 x 4096 x 4096: 11.2 us; 12.7 side by side)
 };
+constexpr size_t kFewStream = (size_t)48 << 20;   // elements of W: 96 MiB
 constexpr int kAuxSc1 = 16;   // agent scope, in a gfx950 buffer instruction's cache policy
 struct Through {
   __amdgpu_buffer_rsrc_t rs;
@@ -865,12 +869,13 @@ template <bool F16> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f3
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <bool F16, int MT, bool ALONG>
+// STREAM: W is read past the caches, where it is too large to stay there until the next call (us, 256 MB of Infinity Cache:
+// 16 x 8192 x 8192, 134 MB, 26.7 instead of 29.5; but 16 x 8192 x 4096, 67 MB, 17.1 instead of 15.7).
+template <bool F16, int MT, bool ALONG, bool STREAM>
 __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const FewArgs a, const LinEpi ep) {
   typedef Few<ALONG> D;
   constexpr int kStride = D::kWidth + 4;
   __shared__ __attribute__((aligned(16))) float red[kFewWaves][16 * kStride];
-  __shared__ uint32_t arrived;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), q = lane >> 4, c = lane & 15;
   const int strip = blockIdx.x, split = blockIdx.y, splits = gridDim.y;
   const int n0 = strip * D::kWidth;
@@ -899,8 +904,14 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
   };
   auto fetch = [&](Step& s, int k) {
     if (inside && k + D::kStep <= k_end) {
+      auto piece = [&](int i) { return ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw; };
+      if constexpr (STREAM) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) __builtin_memcpy(&s.w[i], ALONG ? wp[i >> 1] + k + 32 * (i & 1) : wp[0] + (size_t)(k + i) * a.ldw, 16);
+        for (int i = 0; i < 8; i++) s.w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u*>(piece(i)));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) __builtin_memcpy(&s.w[i], piece(i), 16);
+      }
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -965,15 +976,16 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
   constexpr int kPieces = D::kWidth / 8;
   const int row = t / kPieces, piece = t % kPieces, col = n0 + 8 * piece, n = a.cols - col;
   const size_t ldp = ((size_t)a.cols + 7) & ~(size_t)7;
-  auto finish = [&](float* v, int m) {
-    if (n <= 0) return;
-    const Places where = places<false>(ep, (size_t)(16 * m + row), (size_t)col, 0, 0, 0);
-    Bias8 bias;
-    Old8<false> old;
+  // what is read beside the product, on its way while the wavefronts' sums are added up
+  Bias8 bias;
+  Old8<false> old[MT];
+  auto where = [&](int m) { return places<false>(ep, (size_t)(16 * m + row), (size_t)col, 0, 0, 0); };
+  if ((MT == 1 || splits == 1) && row < 16 && n > 0) {
     load_bias(bias, ep, (size_t)col, n);
-    load_old<false>(old, ep, where, 0, n, col);
-    finish8<F16, false>(v, bias, old, ep, where, 0, n);
-  };
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+      if (16 * m + row < a.rows) load_old<false>(old[m], ep, where(m), 0, n, col);
+  }
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     if (m) __syncthreads();
@@ -999,9 +1011,10 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += x[e];
       }
-      if (splits == 1) {
-        finish(v, m);
-      } else if (n > 0) {
+      if (n <= 0) {
+      } else if (splits == 1) {
+        finish8<F16, false>(v, bias, old[m], ep, where(m), 0, n);
+      } else {
         float* const at = a.partial + ((size_t)split * a.rows + 16 * m + row) * ldp + col;
         if constexpr (MT == 1) Through(a.partial).store((uint32_t)((at - a.partial) * 4), v);
         else __builtin_memcpy(at, v, 32);
@@ -1009,12 +1022,16 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
     }
   }
   if (MT > 1 || splits == 1) return;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's partial sums have arrived
-  __syncthreads();
-  if (t == 0) arrived = __hip_atomic_fetch_add(a.counters + strip, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived != (uint32_t)splits - 1u) return;
-  if (t == 0) __hip_atomic_store(a.counters + strip, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // a wavefront joins the rows that it holds here, with the same wavefront of the other splits
+  const int first = wave * (kWave / kPieces);
+  if (first >= 16 || first >= a.rows) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // its partial sums have arrived
+  uint32_t* const counter = a.counters + ((size_t)strip * kFewWaves + wave) * kFewCounter;
+  uint32_t arrived = 0;
+  if (lane == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if ((uint32_t)__builtin_amdgcn_readfirstlane((int)arrived) != (uint32_t)splits - 1u) return;
+  asm volatile("" ::: "memory");                     // nothing below is read before
+  if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (row < a.rows && n > 0) {
     const Through through(a.partial);
     const uint32_t at = (uint32_t)((row * ldp + col) * 4), step = (uint32_t)(a.rows * ldp * 4);
@@ -1030,7 +1047,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += x[s][e];
       }
-    finish(v, 0);
+    finish8<F16, false>(v, bias, old[0], ep, where(0), 0, n);
   }
 }
 
@@ -1351,6 +1368,14 @@ int product_ring(LinProd& pr, const LinEpi& ep, bool out32, bool whole, int spli
   return launch_ring<F16, PA, QA, FR, FC, kOut16, false>(pr, ep, 1, s);
 }
 
+template <bool F16, bool ALONG, bool STREAM> void launch_few(dim3 grid, dim3 block, const FewArgs& a, const LinEpi& ep, hipStream_t s) {
+  switch ((a.rows + 15) / 16) {
+    case 1: hipLaunchKernelGGL((linear_few_kernel<F16, 1, ALONG, STREAM && !ALONG>), grid, block, 0, s, a, ep); break;
+    case 2: hipLaunchKernelGGL((linear_few_kernel<F16, 2, ALONG, STREAM && !ALONG>), grid, block, 0, s, a, ep); break;
+    case 3: hipLaunchKernelGGL((linear_few_kernel<F16, 3, ALONG, STREAM && !ALONG>), grid, block, 0, s, a, ep); break;
+    default: hipLaunchKernelGGL((linear_few_kernel<F16, 4, ALONG, STREAM && !ALONG>), grid, block, 0, s, a, ep); break;
+  }
+}
 // Up to kFewRows rows.
 template <bool F16, bool ALONG>
 int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint16_t* w, size_t ldw, int rows, int cols, int sum,
@@ -1387,12 +1412,8 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   splits = (sum + a.per_split - 1) / a.per_split;   // no empty split
   a.partial = plan->partial;
   const dim3 grid((unsigned)strips, (unsigned)splits), block(kFewWaves * kWave);
-  switch ((rows + 15) / 16) {
-    case 1: hipLaunchKernelGGL((linear_few_kernel<F16, 1, ALONG>), grid, block, 0, s, a, ep); break;
-    case 2: hipLaunchKernelGGL((linear_few_kernel<F16, 2, ALONG>), grid, block, 0, s, a, ep); break;
-    case 3: hipLaunchKernelGGL((linear_few_kernel<F16, 3, ALONG>), grid, block, 0, s, a, ep); break;
-    default: hipLaunchKernelGGL((linear_few_kernel<F16, 4, ALONG>), grid, block, 0, s, a, ep); break;
-  }
+  if (!ALONG && (size_t)cols * (size_t)sum > kFewStream) launch_few<F16, ALONG, true>(grid, block, a, ep, s);
+  else launch_few<F16, ALONG, false>(grid, block, a, ep, s);
   CCN_HIP(hipGetLastError());
   if (rows > 16 && splits > 1) return launch_join<F16, false>(a.partial, rows, cols, splits, ep, s);
   return CCN_OK;
@@ -1680,14 +1701,14 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t few_most = (size_t)kFewMaxSplits * few_cols, few_cap = 2 * (size_t)di->cu_count * 128;
   const size_t few = (few_most < few_cap ? few_most : few_cap) * (size_t)(max_M < kFewRows ? (max_M + 15) & ~15 : kFewRows);
   p->partial_floats = few > p->partial_floats ? few : p->partial_floats;
-  const size_t strips = few_cols / 64;
+  const size_t counters = few_cols / 64 * kFewWaves * kFewCounter;
   hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * pitch((size_t)max_K) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->pw, (size_t)max_K * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
-  if (e == hipSuccess) e = hipMalloc((void**)&p->counters, strips * sizeof(uint32_t));
-  if (e == hipSuccess) e = hipMemset(p->counters, 0, strips * sizeof(uint32_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->counters, counters * sizeof(uint32_t));
+  if (e == hipSuccess) e = hipMemset(p->counters, 0, counters * sizeof(uint32_t));
   if (e == hipSuccess) e = hipDeviceSynchronize();   // the zeros are there for calls on any stream
   if (e != hipSuccess) {
     ccn_linear_plan_destroy(p);

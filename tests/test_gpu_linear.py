@@ -143,7 +143,8 @@ def test_forward_strides_and_alignments(ccn, M, N, K, pad, shift):
 
 
 @pytest.mark.parametrize("M,N,K,half", [(4096, 4096, 256, False), (4096, 4104, 136, True), (4100, 4096, 520, False), (8192, 2048, 1024, False), (3000, 6000, 1000, True),
-                                         (2048, 4096, 1024, False), (2040, 4000, 1000, True), (2000, 4001, 1003, False)])
+                                         (2048, 4096, 1024, False), (2040, 4000, 1000, True), (2000, 4001, 1003, False),
+                                         (16, 8200, 6200, False), (40, 8193, 6203, True), (5, 6211, 8200, False)])
 def test_forward_large(ccn, M, N, K, half):
     forward_case(ccn, M, N, K, "gelu_tanh", half, resid=True, keep=True)
 
