@@ -395,6 +395,49 @@ def test_refusals(ccn):
 
 
 @pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("blocks", [1, 31, 32, 33, 1024, 1055, 8191, 8192, 8193, 20000])
+def test_flag_at_every_size(ccn, bits, blocks):
+    """The flag is written by every call, whatever it held: 1 for a gradient that is not finite in any block, else 0."""
+    n = 256 * blocks - 100
+    plan = ccn.AdamWPlan([n], bits=bits)
+    g = torch.randn(n, device=DEV, generator=gen(blocks))
+    w, flag = torch.zeros(n, device=DEV), torch.full((2,), 55, device=DEV, dtype=torch.int32)
+    m = torch.zeros(plan.elems, device=DEV, dtype=torch.uint8 if bits == 8 else torch.float32)
+    v, scales = torch.zeros_like(m), torch.zeros(2 * blocks, device=DEV) if bits == 8 else None
+    tables = plan.tables([[g]], [w])
+    st = ccn.Stream()
+
+    def step(stream=None):
+        plan.step(tables, m, v, 1e-3, 0.9, 0.98, 1e-8, 0.1, 1, scales=scales, overflow_flag=flag, stream=stream)
+
+    step()
+    torch.cuda.synchronize()
+    with ccn.Graph(st) as graph:
+        step(st.h)
+    for at in (None, 0, n - 1, None, n // 2, (n * 5) // 7, None):
+        for run in (step, graph.launch):
+            old = g[at].clone() if at is not None else None
+            if at is not None:
+                g[at] = math.inf if at else math.nan
+            flag[0] = 7 if at is None else 0
+            torch.cuda.synchronize()
+            run()
+            st.sync()
+            torch.cuda.synchronize()
+            assert flag.tolist() == [0 if at is None else 1, 55], at
+            if at is not None:
+                g[at] = old
+    g[0], g[n - 1] = -math.inf, 1e38     # two at once, the square of the second alone is not finite
+    torch.cuda.synchronize()
+    step()
+    torch.cuda.synchronize()
+    assert flag[0].item() == 1
+    graph.close()
+    plan.close()
+    st.close()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
 def test_offsets_past_32_bits(ccn, bits):
     """More blocks than a row of the grid takes (2^33 elements; 2^24 with fp32 moments: 2^32): tensors with the same
     values end alike, whichever their place."""
