@@ -284,13 +284,15 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f
 // spread between the matrix instructions, and one is waited for three steps after it was made.  An "along" stage holds rows
 // of 2*RK bytes, the 16-byte pieces swizzled so that the 32 rows of a fragment meet no bank twice; an "across" stage RK rows as
 // in memory, swizzled by 4*(k%4).  Tiles at the edge read the last row or the last 8 columns again (results not stored); a
-// sum that is no multiple of RK ends with a step loaded through registers with zeros behind the end.  One workgroup per CU.
+// sum that is no multiple of RK ends with a step loaded through registers with zeros behind the end.  The ring's LDS makes it one
+// workgroup per CU; a short sum takes one stage, through registers, and up to four share a CU.
 //   4 x 4   256 x 256, RK 32: 256 accumulators per lane, in the accumulation half of the register file; per 16 summed elements a
 //           wavefront reads eight fragments for sixteen matrix instructions
 //   4 x 2   256 x 128, RK 32: six fragments for eight
-//   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  What bounds it is the 64 bytes a clock that L2 gives a CU, so an
-//           "along" request covers whole 128-byte lines (RK 32, two workgroups per CU: half of every line fetched is wasted, and
-//           it does not matter how many wavefronts share the CU)
+//   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  What bounds it is LDS: a step of 64 summed elements writes 32 KiB
+//           and reads 64, 768 clocks at 128 bytes each beside 512 of matrix instructions.  An "along" request covers whole
+//           128-byte lines (RK 32, two workgroups per CU: half of every line fetched is wasted)
+// 8192 x 8192 x 4096 with bias, gelu_tanh and the kept pre-activation: 426 us, 1.29 PFLOP/s; dX and dW of it 412 and 390.
 constexpr size_t kRMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
 constexpr int kStages = 4;
 template <int FR, int FC> struct Ring {
@@ -826,9 +828,9 @@ __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, co
 // up to 16 rows, the one that arrives last finishes (each wavefront for the rows that it has held in every split): partial sums
 // go out and come back with the agent-scope bit (sc1: written through to, and read from, where the XCDs are coherent), complete
 // (vmcnt 0) before the wavefront counts itself in; splits are added in ascending order whoever does it, and the counter is back
-// at zero when the call ends.  With more rows a wavefront would have too much to add (64 x 1024 x 1024: 17.9 us): the join
-// kernel does it.  16 x 8192 x 4096 (67 MB of weights): 15.7 us, 4.3 TB/s; reading W alone takes this grid 10.5, X 0.8, the
-// split sums' way through memory 2.5.
+// at zero when the call ends.  With more rows a wavefront has too much to add, and the join kernel does it (64 x 1024 x 1024:
+// 10.1 us, 13.3 without; 32 x 4096 x 4096: 13.5, 14.5).  16 x 8192 x 4096 (67 MB of weights): 15.7 us, 4.3 TB/s; reading W alone
+// takes this grid 10.5, X 0.8, the split sums' way through memory 2.5.
 constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16, kFewCounter = 32;
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 template <bool ALONG> struct Few {
@@ -1419,15 +1421,15 @@ int product_few(ccn_linear_plan* plan, const uint16_t* x, size_t ldx, const uint
   return CCN_OK;
 }
 
-// How a product runs on the ring, by estimated time.  Measured in us (4096 x 4096 x 4096 and smaller): a step of 64 summed
-// elements takes a CU 0.42 with one 128 x 128 tile on it, 1.06 with two, 1.6 with a 256 x 256 tile; 3.5 or 8 go into the first
-// loads and the output; a split adds 1.8 for the join kernel and 0.4 per MB of partial sums, written and read.
-//   rows x sum x cols        256 x 256    128 x 128, splits 1 / 2 / 4 / 8
-//   256 x 4096 x 4096        74.1         33.0 / 23.6 / 21.7 / 27.3
-//   1024 x 8192 x 1024       132.8        54.1 / 35.7 / 28.9 / 34.8
-//   1024 x 1024 x 1024       30.2         12.2 / 13.1 / 15.1 / 20.5
-//   2048 x 4096 x 4096       77.7         71.2 / 110.7
-//   4096 x 4096 x 4096       110.9        134.2
+// How a product runs on the ring, by estimated time.  Measured in us: a step of 64 summed elements takes a CU 0.40 with one
+// 128 x 128 tile on it, 1.0 with two, 0.9 with a 256 x 128 tile and 1.6 with a 256 x 256 one; 5, 6 or 8 go into the first loads and
+// the output; a split adds 1.8 for the join kernel and 0.4 per MB of partial sums, written and read.
+//   rows x sum x cols        256 x 256    256 x 128    128 x 128, splits 1 / 2 / 4 / 8
+//   256 x 4096 x 4096        75           -            28 / 22 / 22 / 31
+//   1024 x 8192 x 1024       133          -            46.7 / 32.3 / 32.6 / 37.4
+//   1024 x 1024 x 1024       30.2         -            11.9 / 13.4 / 15.6 / 22.9
+//   2048 x 4096 x 4096       79           62.9         65.7
+//   4096 x 4096 x 4096       107.6        122.6        129
 enum RingTile { kTile256, kTile256x128, kTile128 };
 struct RingPlan {
   RingTile tile;
@@ -1452,7 +1454,7 @@ RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus
 }
 
 // Whether a product does without the ring: short sums (`brief`), where there are more tiles than CUs (four workgroups then share a
-// CU: 65 x 4096 x 4096, dW: 48 instead of 33 us of a whole backward pass), or where an operand would have to be copied first.
+// CU: 65 x 4096 x 4096, dW: 33 instead of 48 us for a whole backward pass), or where an operand would have to be copied first.
 bool brief_product(const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum, int cus) {
   if (sum > 192) return false;
   return (size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128) > (size_t)cus || !ring_fetches(p, p_along) || !ring_fetches(q, q_along);
