@@ -1249,14 +1249,15 @@ __global__ __launch_bounds__(kDbWaves * kWave) void linear_db_kernel(const DbArg
 }
 
 // Both products of a backward pass, and db, in one launch: the tiles of small ones run side by side on CUs that one product alone
-// would leave idle, and two launches are saved.  The product with the longer sum is dealt out first.
+// would leave idle, and two launches are saved.  SPLIT: 1 the sum of dX, or 2 that of dW, is split over workgroups (the join kernel
+// adds the splits up).  The product whose workgroups take longer is dealt out first.
 struct PairArgs {
   LinProd x, w;    // dX, dW
   LinEpi ex, ew;
   DbArgs db;
-  int nx, nw, w_first;   // tiles of each; the workgroups behind them are db's
+  int nx, nw, w_first;   // workgroups of each; those behind them are db's
 };
-template <bool F16, bool OUT32, bool WHOLE>
+template <bool F16, bool OUT32, bool WHOLE, int SPLIT>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 4))) void linear_pair_kernel(const PairArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds_ring[];
   const int b = (int)blockIdx.x;
@@ -1264,10 +1265,14 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 4))) 
     add_chunks<kBlock / kWave>(a.db, b - a.nx - a.nw, reinterpret_cast<float*>(lds_ring));
     return;
   }
-  if (a.w_first ? b >= a.nw : b < a.nx)
-    ring_tile<F16, true, true, 2, 2, kOut16, WHOLE>(a.x, a.ex, (uint32_t)(a.w_first ? b - a.nw : b), 0, lds_ring);
-  else
-    ring_tile<F16, false, false, 2, 2, OUT32 ? kOut32 : kOut16, WHOLE>(a.w, a.ew, (uint32_t)(a.w_first ? b : b - a.nx), 0, lds_ring);
+  if (a.w_first ? b >= a.nw : b < a.nx) {
+    const int at = a.w_first ? b - a.nw : b, tiles = a.x.tiles_r * a.x.tiles_c, split = SPLIT == 1 ? at / tiles : 0;
+    ring_tile<F16, true, true, 2, 2, SPLIT == 1 ? kOutPartial : kOut16, WHOLE || SPLIT == 1>(a.x, a.ex, (uint32_t)(at - split * tiles), split, lds_ring);
+  } else {
+    const int at = a.w_first ? b : b - a.nx, tiles = a.w.tiles_r * a.w.tiles_c, split = SPLIT == 2 ? at / tiles : 0;
+    ring_tile<F16, false, false, 2, 2, SPLIT == 2 ? kOutPartial : OUT32 ? kOut32 : kOut16, WHOLE || SPLIT == 2>(a.w, a.ew, (uint32_t)(at - split * tiles), split,
+                                                                                                          lds_ring);
+  }
 }
 
 constexpr size_t kMaxLd = (size_t)1 << 22;
@@ -1455,8 +1460,9 @@ RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus
 
 // Whether a product does without the ring: short sums (`brief`), where there are more tiles than CUs (four workgroups then share a
 // CU: 65 x 4096 x 4096, dW: 33 instead of 48 us for a whole backward pass), or where an operand would have to be copied first.
+constexpr int kBriefSum = 192;
 bool brief_product(const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum, int cus) {
-  if (sum > 192) return false;
+  if (sum > kBriefSum) return false;
   return (size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128) > (size_t)cus || !ring_fetches(p, p_along) || !ring_fetches(q, q_along);
 }
 // A product whose operands the ring can fetch (or a brief one): C [rows x cols].
@@ -1496,15 +1502,57 @@ int run_product(LinProd& pr, const LinEpi& ep, bool out32, RingPlan how, hipStre
   if (how.tile == kTile256x128) return product_ring<F16, PA, QA, 4, 2>(pr, ep, out32, whole, 1, s);
   return product_ring<F16, PA, QA, 2, 2>(pr, ep, out32, whole, how.splits, s);
 }
-template <bool F16, bool OUT32, bool WHOLE> int launch_pair(const PairArgs& a, hipStream_t s) {
+template <bool F16, bool OUT32, bool WHOLE, int SPLIT> int launch_pair(const PairArgs& a, hipStream_t s) {
   constexpr int kLds = Ring<2, 2>::kLds;
   static std::atomic<uint32_t> devices{0};
-  CCN_TRY(allow_lds((const void*)linear_pair_kernel<F16, OUT32, WHOLE>, kLds, devices));
+  CCN_TRY(allow_lds((const void*)linear_pair_kernel<F16, OUT32, WHOLE, SPLIT>, kLds, devices));
   const int lds = a.x.brief && a.w.brief ? Ring<2, 2>::kBriefLds : kLds;
   const int blocks = a.nx + a.nw + (a.db.db ? (a.db.cols + kWave - 1) / kWave : 0);
-  hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE>), dim3((unsigned)blocks), dim3(kBlock), lds, s, a);
+  hipLaunchKernelGGL((linear_pair_kernel<F16, OUT32, WHOLE, SPLIT>), dim3((unsigned)blocks), dim3(kBlock), lds, s, a);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
+}
+template <bool F16, bool OUT32> int product_pair(const PairArgs& a, int split, int splits, hipStream_t s) {
+  const bool wx = whole_pieces(a.ex, a.x.cols, false), ww = whole_pieces(a.ew, a.w.cols, OUT32);   // (of a split product: the join's)
+  if (split == 1) {
+    CCN_TRY((ww ? launch_pair<F16, OUT32, true, 1>(a, s) : launch_pair<F16, OUT32, false, 1>(a, s)));
+    return launch_join<F16, false>(a.x.partial, a.x.rows, a.x.cols, splits, a.ex, s);
+  }
+  if (split == 2) {
+    CCN_TRY((wx ? launch_pair<F16, OUT32, true, 2>(a, s) : launch_pair<F16, OUT32, false, 2>(a, s)));
+    return launch_join<F16, OUT32>(a.w.partial, a.w.rows, a.w.cols, splits, a.ew, s);
+  }
+  return wx && ww ? launch_pair<F16, OUT32, true, 0>(a, s) : launch_pair<F16, OUT32, false, 0>(a, s);
+}
+
+// How the two run side by side, by estimated time: as long as a workgroup's longest sum, and as all the work dealt over the CUs, in
+// steps of 64 summed elements (0.45 us), what a workgroup does before and after its sum being worth 8 of them.  Splitting one of
+// the sums pays where it is much the longer one; it costs a join kernel (5.5 us with its launch, and 0.4 per MB of partial sums), and
+// is left alone beside a product of many tiles with a short sum, which want the CUs themselves.  (Sizes alone decide: how an
+// operand is aligned does not change a result's bits.)  Whole backward passes in us, unsplit / split:
+//   M x N x K  128 x 1024 x 1024 12.9 / 14.9    1001 x 2049 x 515 30.9 / 28.2    8192 x 256 x 256 25.9 / 17.7    700 x 8000 x 128 31.1 / 21.1
+// split: 0 none, 1 the first one's, 2 the second one's.
+struct PairPlan {
+  int split, splits;
+  double us;
+};
+PairPlan choose_pair(const LinProd& x, const LinProd& w, size_t partial_floats, int cus) {
+  const double sx = (x.sum + 63) / 64, sw = (w.sum + 63) / 64, tx = (double)x.tiles_r * x.tiles_c, tw = (double)w.tiles_r * w.tiles_c;
+  const auto time = [&](double nx, double nw) {   // splits of each
+    const double lx = std::ceil(sx / nx) + 8.0, lw = std::ceil(sw / nw) + 8.0;
+    return 1.0 + 0.45 * std::fmax(std::fmax(lx, lw), (tx * nx * lx + tw * nw * lw) / cus);
+  };
+  PairPlan best{0, 1, time(1, 1)};
+  if ((x.sum <= kBriefSum && tx > cus) || (w.sum <= kBriefSum && tw > cus)) return best;
+  for (int which = 1; which <= 2; which++) {
+    const LinProd& p = which == 1 ? x : w;
+    const size_t each = (size_t)p.rows * round8((size_t)p.cols);
+    for (int n = 2; n <= kMaxSplits && n * 128 <= p.sum && (size_t)n * each <= partial_floats; n++) {
+      const double t = (which == 1 ? time(n, 1) : time(1, n)) + 5.5 + 0.4e-6 * 4.0 * (double)n * (double)each;
+      if (t < best.us) best = PairPlan{which, n, t};
+    }
+  }
+  return best;
 }
 
 // Aligned copies of up to two operands into the plan (nullptr: none).
@@ -1636,18 +1684,18 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
     hw = choose_ring(K, N, M, plan->partial_floats, di->cu_count);
   }
   if (ring_dx && dW) {
-    // Side by side, if that is estimated to be faster than one after the other (3 us for what is between two launches): as long as
-    // the longer sum, and as all steps dealt over the CUs.
-    const double sx = (N + 63) / 64, sw = (M + 63) / 64;
+    // side by side, if that is estimated to be faster than one after the other (3 us for what is between two launches)
+    PairPlan both = choose_pair(px, pw, plan->partial_floats, di->cu_count);
     const double tx = (double)px.tiles_r * px.tiles_c, tw = (double)pw.tiles_r * pw.tiles_c;
-    double longest = sx > sw ? sx : sw;
-    const double dealt = (tx * sx + tw * sw) / di->cu_count;
-    if (dealt > longest) longest = dealt;
-    if (5.0 + 0.5 * longest < hx.us + hw.us + (db_left ? 6.0 : 3.0) && tx + tw < 1e6) {
-      const PairArgs a{px, pw, dx_ep, dw_ep, dba, (int)tx, (int)tw, sw > sx ? 1 : 0};
-      const bool whole = whole_pieces(dx_ep, K, false) && whole_pieces(dw_ep, N, dw32);
-      if (dw32) return whole ? launch_pair<F16, true, true>(a, s) : launch_pair<F16, true, false>(a, s);
-      return whole ? launch_pair<F16, false, true>(a, s) : launch_pair<F16, false, false>(a, s);
+    if (both.us < hx.us + hw.us + (db_left ? 6.0 : 3.0) && tx + tw < 1e6) {
+      LinProd& p = both.split == 2 ? pw : px;
+      const int steps = (p.sum + 63) / 64;
+      p.per_split = 64 * ((steps + both.splits - 1) / both.splits);
+      both.splits = (p.sum + p.per_split - 1) / p.per_split;   // no empty split
+      const double lx = (N + 63) / 64 / (both.split == 1 ? (double)both.splits : 1.0), lw = (M + 63) / 64 / (both.split == 2 ? (double)both.splits : 1.0);
+      const int nx = (int)tx * (both.split == 1 ? both.splits : 1), nw = (int)tw * (both.split == 2 ? both.splits : 1);
+      const PairArgs a{px, pw, dx_ep, dw_ep, dba, nx, nw, lw > lx ? 1 : 0};
+      return dw32 ? product_pair<F16, true>(a, both.split, both.splits, s) : product_pair<F16, false>(a, both.split, both.splits, s);
     }
   }
   if (db_left) {

@@ -320,8 +320,8 @@ int  ccn_matmul_f16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, in
  *      or leaves them when accumulating.
  *      Products are accumulated in fp32 on the matrix cores, Y is computed from the fp32 z, every output is rounded to
  *      nearest even once.  dz is rounded to the operands' type before the two products when there is an activation (the
- *      matrix cores take 16-bit operands); db is summed in fp32 from the unrounded dz.  Sums run in a fixed order: the
- *      same call gives the same bits.
+ *      matrix cores take 16-bit operands); db is summed in fp32 from the unrounded dz.  Sums run in a fixed order, which
+ *      the sizes and the plan's decide: the same call gives the same bits, whatever its strides.
  *      act: CCN_ACT_*; GELU is z*Phi(z), GELU_TANH its tanh form, SILU z*sigmoid(z); the slope of RELU at 0 is 0.
  *      bias, resid, pre may be NULL (not wanted); so may any of dX, dW, db.  backward needs pre unless act is NONE (it is
  *      then ignored and dz is dY itself); it needs W for dX and X for dW.  accumulate != 0: db, and dW, which must be fp32

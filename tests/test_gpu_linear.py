@@ -247,7 +247,8 @@ def backward_case(ccn, M, N, K, act, half, dw32=False, accumulate=False, pad=0, 
 
 BSHAPES = [(1, 1, 1), (1, 64, 128), (2, 513, 70), (7, 130, 1031), (16, 1024, 512), (33, 65, 129), (64, 256, 256), (128, 128, 128), (130, 257, 131), (255, 1000, 72),
            (256, 512, 1024), (515, 264, 2049), (1001, 515, 1025), (2048, 256, 256), (4097, 136, 200),
-           (300, 3, 5), (100, 5, 300), (500, 300, 5), (1000, 6, 40), (20, 2100, 2060), (190, 2100, 2053)]
+           (300, 3, 5), (100, 5, 300), (500, 300, 5), (1000, 6, 40), (20, 2100, 2060), (190, 2100, 2053),
+           (4500, 120, 264), (3000, 301, 100), (300, 3000, 296), (257, 2999, 131)]
 
 
 @pytest.mark.parametrize("M,N,K", BSHAPES)
