@@ -186,3 +186,60 @@ def test_a_recorded_step(ccn):
         assert torch.equal(blocks[0].w[0], blocks[1].w[0]) and torch.equal(plans[0][1], plans[1][1]) and torch.equal(plans[0][3], plans[1][3]), rep
     graph.close()
     st.close()
+
+
+def test_two_plans_at_once_on_two_streams(ccn):
+    """Calls on plans of their own do not disturb each other: the same calls one after the other give the same bits.  Rows that take
+    the split sums, the joined few-row kernel and the pair kernel; AdamW steps with and without a flag launch."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(9)
+
+    def layer(M, N, K):
+        rand = lambda *sh: torch.randn(*sh, device=DEV, generator=g).bfloat16()  # noqa: E731
+        x, w, dy = rand(M, K), rand(K, N), rand(M, N)
+        plan = ccn.LinearPlan(M, N, K)
+
+        def run(out, stream):
+            for _ in range(8):
+                plan.forward(x, w, None, None, out[0], M, N, K, act="silu", pre=out[1], stream=stream)
+                plan.backward(dy, out[1], x, w, out[2], out[3], out[4], M, N, K, act="silu", stream=stream)
+
+        def new():
+            return [torch.zeros_like(dy), torch.zeros_like(dy), torch.zeros_like(x), torch.zeros_like(w), torch.zeros(N, device=DEV)]
+        return plan, run, new
+
+    def step(n, bits):
+        grad, w0 = torch.randn(n, device=DEV, generator=g), torch.randn(n, device=DEV, generator=g)
+        grad[n // 3] = math.inf
+        plan = ccn.AdamWPlan([n], bits=bits)
+
+        def run(out, stream):
+            for t in range(1, 5):
+                plan.step(plan.tables([[grad]], [out[0]]), out[1], out[2], LR, B1, B2, 1e-8, WD, t, scales=out[3] if bits == 8 else None,
+                          overflow_flag=out[4], stream=stream)
+
+        def new():
+            m = torch.zeros(plan.elems, device=DEV, dtype=torch.uint8 if bits == 8 else torch.float32)
+            return [w0.clone(), m, torch.zeros_like(m), torch.zeros(2 * plan.blocks, device=DEV), torch.zeros(1, device=DEV, dtype=torch.int32)]
+        return plan, run, new
+
+    jobs = [layer(16, 512, 4096), layer(48, 520, 2048), layer(300, 1500, 72), layer(2000, 136, 264), layer(7, 1000, 3000), step(100_000, 8), step(100_000, 32),
+            step(3_000_000, 8)]
+    for i in range(len(jobs)):
+        (pa, ra, na), (pb, rb, nb) = jobs[i], jobs[(i + 1) % len(jobs)]
+        alone_a, alone_b, a, b = na(), nb(), na(), nb()
+        torch.cuda.synchronize()
+        ra(alone_a, None)
+        torch.cuda.synchronize()
+        rb(alone_b, None)
+        torch.cuda.synchronize()
+        sa, sb = ccn.Stream(), ccn.Stream()
+        ra(a, sa.h)
+        rb(b, sb.h)
+        torch.cuda.synchronize()
+        for got, want in zip(a + b, alone_a + alone_b):
+            assert torch.equal(got, want), i
+        sa.close()
+        sb.close()
+    for plan, _run, _new in jobs:
+        plan.close()
