@@ -787,31 +787,32 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
 }
 
 // ---- operands whose rows are not made of aligned 16-byte pieces --------------------------------------------------------------
-// A copy with aligned rows, zeros behind each row's end: the ring then runs on it.  It costs a launch and two passes over the
-// operand at the memory's rate, less than matrix instructions fed from unaligned loads through registers lose at any size (129 x
-// 129 x 129: 11.1 instead of 11.8 us, 777 x 1537 x 2049: 27 instead of 57, 2049 x 2049 x 2049: 54 instead of 90).
+// A copy with aligned rows, zeros behind each row's end up to the next row: the ring then runs on it.  It costs a launch and two
+// passes over the operand at the memory's rate, less than matrix instructions fed from unaligned loads through registers lose at
+// any size (129 x 129 x 129: 11.1 instead of 11.8 us, 777 x 1537 x 2049: 24 instead of 57, 2049 x 2049 x 2049: 54 instead of 90).
 struct PackJob {
   const uint16_t* src;
   uint16_t* dst;
   size_t ld, ldd;   // ldd: a multiple of 8
-  int rows, cols;
+  int rows, cols, rows_out;   // rows_out: rows written, those from `rows` on zeros
 };
 constexpr int kPackRows = 16;
 __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, const PackJob b) {
   const PackJob& job = blockIdx.z ? b : a;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = ((int)blockIdx.x * kWave + lane) * 8;
-  if (col >= job.cols) return;
-  for (int r0 = (int)blockIdx.y * kPackRows; r0 < job.rows; r0 += (int)gridDim.y * kPackRows) {
+  if ((size_t)col >= job.ldd) return;
+  for (int r0 = (int)blockIdx.y * kPackRows; r0 < job.rows_out; r0 += (int)gridDim.y * kPackRows) {
     u32x4 v[kPackRows / 4];
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
       const int r = r0 + 4 * u + wave;
+      v[u] = u32x4{0u, 0u, 0u, 0u};
       if (r < job.rows) v[u] = fetch_piece(job.src + (size_t)r * job.ld, col, job.cols);
     }
 #pragma unroll
     for (int u = 0; u < kPackRows / 4; u++) {
       const int r = r0 + 4 * u + wave;
-      if (r < job.rows) *reinterpret_cast<u32x4*>(job.dst + (size_t)r * job.ldd + col) = trim_piece(v[u], job.cols - col, job.cols);
+      if (r < job.rows_out) *reinterpret_cast<u32x4*>(job.dst + (size_t)r * job.ldd + col) = trim_piece(v[u], job.cols - col, job.cols);
     }
   }
 }
@@ -1556,16 +1557,18 @@ PairPlan choose_pair(const LinProd& x, const LinProd& w, size_t partial_floats, 
 }
 
 // Aligned copies of up to two operands into the plan (nullptr: none).
-int pack(const Operand* a, int a_cols, uint16_t* a_to, const Operand* b, int b_cols, uint16_t* b_to, hipStream_t s) {
-  const auto job = [](const Operand* o, int cols, uint16_t* to) { return o ? PackJob{o->p, to, o->ld, pitch((size_t)cols), o->rows, cols} : PackJob{}; };
-  PackJob x = job(a, a_cols, a_to), y = job(b, b_cols, b_to);
+int pack(const Operand* a, int a_cols, uint16_t* a_to, const Operand* b, int b_cols, uint16_t* b_to, int b_rows_out, hipStream_t s) {
+  const auto job = [](const Operand* o, int cols, uint16_t* to, int rows_out) {
+    return o ? PackJob{o->p, to, o->ld, pitch((size_t)cols), o->rows, cols, rows_out} : PackJob{};
+  };
+  PackJob x = job(a, a_cols, a_to, a ? a->rows : 0), y = job(b, b_cols, b_to, b_rows_out);
   if (!a) {
     x = y;
     y = PackJob{};
   }
-  const int cols = x.cols > y.cols ? x.cols : y.cols, rows = x.rows > y.rows ? x.rows : y.rows;
-  const int gy = (rows + kPackRows - 1) / kPackRows;
-  const dim3 grid((unsigned)((cols + 511) / 512), (unsigned)(gy < 65535 ? gy : 65535), a && b ? 2u : 1u);
+  const size_t width = x.ldd > y.ldd ? x.ldd : y.ldd;
+  const int rows = x.rows_out > y.rows_out ? x.rows_out : y.rows_out, gy = (rows + kPackRows - 1) / kPackRows;
+  const dim3 grid((unsigned)((width + 511) / 512), (unsigned)(gy < 65535 ? gy : 65535), a && b ? 2u : 1u);
   hipLaunchKernelGGL(linear_pack_kernel, grid, dim3(kBlock), 0, s, x, y);
   CCN_HIP(hipGetLastError());
   return CCN_OK;
@@ -1602,12 +1605,15 @@ int linear_forward(ccn_linear_plan* plan, const uint16_t* X, size_t ldx, const u
   if (M <= kFewRows) return product_few<F16, false>(plan, X, ldx, W, ldw, M, N, K, ep, di->cu_count, s);
   Operand x{X, ldx, M, K}, w{W, ldw, K, N};
   const bool cx = !ring_fetches(x, true), cw = !ring_fetches(w, false);
+  int sum = K;
   if ((cx || cw) && !brief_product(x, true, w, false, M, N, K, di->cu_count)) {
-    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
+    // both copied: the sum goes on over zeros to whole steps, and has no last step through registers (K = 1537: 2 us less)
+    if (cx && cw) sum = (int)pitch((size_t)K);
+    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, sum, s));
     if (cx) x = Operand{plan->px, pitch((size_t)K), M, (int)round8((size_t)K)};
-    if (cw) w = Operand{plan->pw, pitch((size_t)N), K, (int)round8((size_t)N)};
+    if (cw) w = Operand{plan->pw, pitch((size_t)N), sum, (int)round8((size_t)N)};
   }
-  LinProd pr = make_product(plan, x, true, w, false, M, N, K, di->cu_count);
+  LinProd pr = make_product(plan, x, true, w, false, M, N, sum, di->cu_count);
   return run_product<F16, true, false>(pr, ep, false, choose_ring(M, N, K, plan->partial_floats, di->cu_count), s);
 }
 
@@ -1668,7 +1674,7 @@ int linear_backward(ccn_linear_plan* plan, const uint16_t* dY, size_t lddy, cons
   const LinEpi dx_ep{nullptr, nullptr, nullptr, dX, 0, 0, lddx, CCN_ACT_NONE, 0};
   const LinEpi dw_ep{nullptr, nullptr, nullptr, dW, 0, 0, lddw, CCN_ACT_NONE, accumulate ? 1 : 0};
   if (cw || cx) {
-    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, s));
+    CCN_TRY(pack(cx ? &x : nullptr, K, plan->px, cw ? &w : nullptr, N, plan->pw, K, s));
     if (cx) x = Operand{plan->px, pitch((size_t)K), M, (int)round8((size_t)K)};
     if (cw) w = Operand{plan->pw, pitch((size_t)N), K, (int)round8((size_t)N)};
   }
@@ -1754,7 +1760,7 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t counters = few_cols / 64 * kFewWaves * kFewCounter;
   hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * pitch((size_t)max_K) * sizeof(uint16_t));
-  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, (size_t)max_K * pitch((size_t)max_N) * sizeof(uint16_t));
+  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, pitch((size_t)max_K) * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->counters, counters * sizeof(uint32_t));
