@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
     const float v1 = k.b2 * v0 + k.omb2 * g * g;
     // a gradient that is not finite, or whose square is not: the element keeps its weight and moments
     const bool bad = !(v1 < __builtin_inff());
-    any_bad = any_bad || bad;
+    any_bad = any_bad || (bad && (wide || e + j < n));   // behind the tensor's end the moments may hold anything
     const float r1 = square_root(v1);
     const float w1 = wp.d[j] * keep - (k.rate * m1) * __builtin_amdgcn_rcpf(r1 * k.root_bc2 + k.eps);
     wp.d[j] = bad ? wp.d[j] : w1;

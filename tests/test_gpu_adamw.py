@@ -470,3 +470,32 @@ def test_offsets_past_32_bits(ccn, bits):
     torch.cuda.synchronize()
     assert torch.equal(first, w[0]) and torch.equal(m1, m[:each]) and torch.equal(v1, v[:each])
     plan.close()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("last", [3, 8300 * 256 - 7], ids=["few-blocks", "many-blocks"])
+def test_what_lies_behind_a_tensors_end(ccn, bits, last):
+    """Moment arrays that hold anything behind the tensors' ends (a state restored into uninitialised memory): the flag and the
+    live elements are those of a step over zeros there."""
+    counts = [1, 255, 257, 1000, 513, 256, last]
+    a, b = (Case(ccn, counts, 2, "bf16", "bf16", bits, seed=6) for _ in range(2))
+    behind = torch.ones(a.plan.elems, dtype=torch.bool, device=DEV)
+    for o, n in zip(a.starts, counts):
+        behind[o:o + n] = False
+    for t, fill in enumerate((None, math.nan, math.inf, -math.inf, 3e38), 1):
+        for c in (a, b):
+            c.gen = gen(t)
+            c.new_gradients()
+        if fill is not None:
+            # 8 bits: the two NaN codes, and the largest values
+            code = {math.nan: 0x7f, math.inf: 0xff, -math.inf: 0xfe}.get(fill, 0x7e)
+            for x in (a.m, a.v):
+                x[behind] = fill if bits == 32 else code
+        for c in (a, b):
+            c.step(t)
+        torch.cuda.synchronize()
+        assert a.flag.item() == 0 and b.flag.item() == 0, fill
+        for x, y in zip(a.w + a.w16 + [a.m[~behind], a.v[~behind]], b.w + b.w16 + [b.m[~behind], b.v[~behind]]):
+            assert torch.equal(x, y), fill
+        if bits == 8:
+            assert torch.equal(a.scales, b.scales) and not a.m[behind].any() and not a.v[behind].any(), fill
