@@ -200,15 +200,17 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
     const float m0 = mp.d[j], v0 = BITS == 8 ? vp.d[j] * vp.d[j] : vp.d[j];
     const float m1 = k.b1 * m0 + k.omb1 * g;
     const float v1 = k.b2 * v0 + k.omb2 * g * g;
-    // a gradient that is not finite, or whose square is not: the element keeps its weight and moments
-    const bool bad = !(v1 < __builtin_inff());
+    // A gradient that is not finite, or whose square is not: the element keeps its weight and moments.  Asked of the gradient alone:
+    // in v1 its square is weighted by 1-b2, and v0 is added.  A v1 that is not finite all the same (a restored v0 that is not) is
+    // held too, without the flag.
+    const bool bad = !(g * g < __builtin_inff()), hold = bad || !(v1 < __builtin_inff());
     any_bad = any_bad || (bad && (wide || e + j < n));   // behind the tensor's end the moments may hold anything
     const float r1 = square_root(v1);
     const float w1 = wp.d[j] * keep - (k.rate * m1) * __builtin_amdgcn_rcpf(r1 * k.root_bc2 + k.eps);
-    wp.d[j] = bad ? wp.d[j] : w1;
-    mp.d[j] = bad ? m0 : m1;
-    if constexpr (BITS == 8) root[j] = bad ? vp.d[j] : r1;
-    else vp.d[j] = bad ? v0 : v1;
+    wp.d[j] = hold ? wp.d[j] : w1;
+    mp.d[j] = hold ? m0 : m1;
+    if constexpr (BITS == 8) root[j] = hold ? vp.d[j] : r1;
+    else vp.d[j] = hold ? v0 : v1;
   }
   store4(w, e, n, wide, wp);
   if (a.w16_type) {

@@ -374,7 +374,8 @@ int  ccn_linear_backward_f16(ccn_linear_plan* plan, const uint16_t* dY, size_t l
  *      Elements behind a tensor's end are not part of the state; an 8-bit step writes zeros there.
  *      grad_scale: DEVICE fp32 scalar (a clipping factor, a loss scale's inverse), or NULL for 1.
  *      overflow_flag (DEVICE uint32, or NULL): set by the call, 1 if the gradient of any element, or its square, is not
- *      finite in fp32, else 0.  Such an element keeps its w, m, v (8-bit ones rounded again with the block's new scale).
+ *      finite in fp32, else 0.  Such an element keeps its w, m, v (8-bit ones rounded again with the block's new scale); so does
+ *      one whose new v is not finite although its gradient is, which does not set the flag.
  *      eps > 0 keeps the quotient defined where v is zero.  CCN_ERANGE: more than 2^31 blocks.
  *      The device's pointer table is refreshed on the call's stream when pointers change; such a call cannot be recorded, and
  *      once a call on the plan has been recorded its pointers stay (CCN_EINVAL for others).  `step` is evaluated on the host,

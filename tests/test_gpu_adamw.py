@@ -499,3 +499,44 @@ def test_what_lies_behind_a_tensors_end(ccn, bits, last):
             assert torch.equal(x, y), fill
         if bits == 8:
             assert torch.equal(a.scales, b.scales) and not a.m[behind].any() and not a.v[behind].any(), fill
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("beta2", [0.0, 0.5, 0.98, 0.9999])
+def test_the_flags_border(ccn, bits, beta2):
+    """The square of a gradient overflows fp32 from 2^64 on, whatever beta2: such an element keeps its state and sets the flag, the
+    float below does neither."""
+    below = (2.0 - 2.0 ** -23) * 2.0 ** 63
+    for x, bad in ((below, False), (-below, False), (2.0 ** 64, True), (3e19, True), (-5e20, True)):
+        c = Case(ccn, [700, 20], 1, "f32", None, bits, seed=2)
+        c.new_gradients()
+        c.step(1, beta2=beta2)
+        c.new_gradients()
+        c.g[0][0][300] = x
+        old, before = [w.clone() for w in c.w], c.state()
+        c.step(2, beta2=beta2)
+        torch.cuda.synchronize()
+        assert c.flag.item() == int(bad), (x, beta2)
+        assert (c.w[0][300] == old[0][300]).item() == bad and not torch.equal(c.w[1], old[1])
+        now = c.state()
+        if bad and bits == 32:
+            assert now[1][0][300] == before[1][0][300] and now[2][0][300] == before[2][0][300]
+        assert all(torch.isfinite(y).all() for part in now for y in part)
+
+
+def test_a_second_moment_that_is_not_finite(ccn):
+    """A restored v that is inf or NaN says nothing about the gradient: no flag, and the element stays as it is."""
+    c = Case(ccn, [700], 1)
+    c.new_gradients()
+    c.step(1)
+    c.v[5], c.v[400], c.v[699] = math.inf, math.nan, math.inf
+    at = torch.tensor([5, 400, 699], device=DEV)
+    w, m = c.w[0].clone(), c.m.clone()
+    c.new_gradients()
+    c.step(2)
+    torch.cuda.synchronize()
+    assert c.flag.item() == 0
+    assert torch.equal(c.w[0][at], w[at]) and torch.equal(c.m[at], m[at]) and not torch.isfinite(c.v[at]).any()
+    fine = torch.ones(700, dtype=torch.bool, device=DEV)
+    fine[at] = False
+    assert torch.isfinite(c.w[0]).all() and not torch.equal(c.w[0][fine], w[fine])
