@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
     sr = a.scales[a.blocks + blk];
   }
   const float gs = a.grad_scale ? k.inv_scale * *a.grad_scale : k.inv_scale;
-  const float keep = 1.0f - k.lr_wd * buf.decay;
+  const float shrink = k.lr_wd * buf.decay;
   bool any_bad = false;
   if constexpr (BITS == 8) {
     from_e4m3(mc, sm, mp.d);
@@ -206,7 +206,9 @@ __global__ __launch_bounds__(kWave) void adamw_kernel(const AdamwArgs a, const A
     const bool bad = !(g * g < __builtin_inff()), hold = bad || !(v1 < __builtin_inff());
     any_bad = any_bad || (bad && (wide || e + j < n));   // behind the tensor's end the moments may hold anything
     const float r1 = square_root(v1);
-    const float w1 = wp.d[j] * keep - (k.rate * m1) * __builtin_amdgcn_rcpf(r1 * k.root_bc2 + k.eps);
+    // The decay is a term of the update: 1 - shrink in fp32 is a multiple of 2^-24, a decay of 1e-7 would act as 1.2e-7 and one below
+    // 3e-8 not at all, on every weight and step alike.
+    const float w1 = wp.d[j] - fmaf(shrink, wp.d[j], (k.rate * m1) * __builtin_amdgcn_rcpf(r1 * k.root_bc2 + k.eps));
     wp.d[j] = hold ? wp.d[j] : w1;
     mp.d[j] = hold ? m0 : m1;
     if constexpr (BITS == 8) root[j] = hold ? vp.d[j] : r1;

@@ -540,3 +540,44 @@ def test_a_second_moment_that_is_not_finite(ccn):
     fine = torch.ones(700, dtype=torch.bool, device=DEV)
     fine[at] = False
     assert torch.isfinite(c.w[0]).all() and not torch.equal(c.w[0][fine], w[fine])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("rate", [1e-7, 4.7e-8, 2e-8, 3.3e-4])
+def test_decay_is_not_rounded(ccn, bits, rate):
+    """A step without gradients: w*(1 - lr*wd), off by half a step of the result and by three roundings of the decay itself."""
+    n, lr = 1 << 20, 1e-5
+    c = Case(ccn, [n], 1, bits=bits)
+    c.g[0][0].zero_()
+    w0 = c.w[0].double()
+    c.step(1, lr=lr, wd=rate / lr)
+    torch.cuda.synchronize()
+    want = w0 * (1 - rate)
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 25)
+    d = (c.w[0].double() - want).abs()
+    assert (d <= half + 3 * U * rate * w0.abs()).all(), (d / half).max().item()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("rate", [1e-7, 2e-8])
+def test_decay_beside_updates(ccn, bits, rate):
+    """Updates of all sizes (from a state of their own): what rounds the new weights, each to half a step of 2^-23, averages out over
+    2^20 of them (6 sigma of a uniform error), so that the mean shows a decay far below a weight's last bit.  The update itself is off
+    by some 64 roundings at most."""
+    n, lr = 1 << 20, 1e-5
+    c = Case(ccn, [n], 1, bits=bits)
+    for t in (1, 2):
+        c.new_gradients()
+        c.step(t, lr=0.0, wd=0.0)
+    c.w[0].copy_(1 + torch.rand(n, device=DEV, generator=c.gen) * 0.99)
+    torch.cuda.synchronize()
+    (w0,), (m0,), (r0,) = c.state()
+    c.new_gradients()
+    c.step(3, lr=lr, wd=rate / lr)
+    torch.cuda.synchronize()
+    b1, b2 = HYPER["beta1"], HYPER["beta2"]
+    g = c.g[0][0].double()
+    m, v = b1 * m0 + (1 - b1) * g, b2 * r0.square() + (1 - b2) * g * g
+    u = lr * (m / (1 - b1 ** 3)) / ((v / (1 - b2 ** 3)).sqrt() + HYPER["eps"])
+    d = c.w[0].double() - (w0 - rate * w0 - u)
+    assert d.mean().abs() <= 6 * 2.0 ** -23 / math.sqrt(12 * n) + 64 * U * u.abs().mean() + 3 * U * rate * w0.mean(), d.mean().item()
