@@ -467,3 +467,29 @@ def test_refusals(ccn):
     torch.cuda.synchronize()
     assert bool((Y == 5).all()) and bool((dW == 5).all()) and bool((dX == 5).all())
     plan.close()
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M", [2, 20, 70])
+def test_gelu_far_left(ccn, M, half):
+    """GELU and its slope where both are a small tail: within 2^-18 relative (the fit, a dozen fp32 roundings, exp2 and the reciprocal at 1
+    ulp) and the exponent's roundings (four of 2^-24 of z^2/2), beside the output's own half step."""
+    N, K = 1400, 8
+    X = torch.zeros(M, K, device=DEV, dtype=TYPES[half])
+    X[:, 0] = 1.0
+    W = torch.zeros(K, N, device=DEV, dtype=TYPES[half])
+    W[0] = torch.linspace(-10.0, -3.0, N, device=DEV)
+    z = W[0].double()
+    phi, Phi = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), torch.erfc(-z * math.sqrt(0.5)) / 2   # (ndtr on the device is 0 below -8)
+    rel = 2.0 ** -18 + 4 * U24 * z * z / 2
+    Y = torch.empty(M, N, device=DEV, dtype=TYPES[half])
+    plan = ccn.LinearPlan(M, N, K)
+    plan.forward(X, W, None, None, Y, M, N, K, act="gelu", half=half)
+    y = (z * Phi).expand(M, N)
+    h = half_step(half)
+    within(Y, y, (h + (1 + h) * rel) * y.abs() + tiny(half), f"Y {M}")
+    pre, dY, db = W[0].expand(M, N).contiguous(), torch.ones(M, N, device=DEV, dtype=TYPES[half]), torch.empty(N, device=DEV)
+    plan.backward(dY, pre, None, None, None, None, db, M, N, K, act="gelu", half=half)
+    s = M * (Phi + z * phi)
+    within(db, s, M * (rel + (M + 2) * U24) * (Phi + z.abs() * phi), f"db {M}")
+    plan.close()
