@@ -2,7 +2,9 @@
 
 Thin by design: every function below forwards device pointers and sizes to the C ABI and raises
 CoconetError on a non-zero return code.  torch is used by callers only to own device memory and streams;
-arguments here are raw addresses (ints), torch tensors (their data_ptr() is taken) or None.
+arguments here are raw addresses (ints), torch tensors (their data_ptr() is taken) or None.  The plans of the dense layer
+and of AdamW, whose arrays come in several types and layouts, refuse a tensor that is not of the type, on the device or in the
+order in which the call will read it (CoconetError); of the other calls' tensors only the address is looked at.
 
 There is no CPU fallback: if the shared library is missing, loading raises.
 """
@@ -167,11 +169,18 @@ def ptr_table(bufs):
     return C.cast(tbl, _pp), tbl
 
 
+_stream_of = None
+
+
 def current_stream():
     """The HIP stream torch is currently issuing work on, as an address (without the Stream object that
     torch.cuda.current_stream() builds first: 3 us a call, as long as a small kernel)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    global _stream_of
+    if _stream_of is None:
+        import torch
+        torch.cuda.init()
+        _stream_of = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    return _stream_of[0](_stream_of[1]())
 
 
 # ---- runtime ---------------------------------------------------------------------------------------------------------
@@ -504,6 +513,63 @@ def matmul_16(X, W, Cmat, M, N, K, stream=None, half=False):
 
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 TYPES = {"f32": 0, "bf16": 1, "f16": 2}
+_DTYPES = {}
+
+
+def _dtypes(name):
+    """The torch dtypes in which an array of the element type `name` may come: its own, and those that hold its bit patterns."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update(f32=(torch.float32,), bf16=(torch.bfloat16, torch.int16, torch.uint16), f16=(torch.float16, torch.int16, torch.uint16),
+                       e4m3=(torch.float8_e4m3fn, torch.uint8, torch.int8), u32=(torch.int32, torch.uint32))
+    return _DTYPES[name]
+
+
+def _refuse(x, what, needs, code=CCN_EINVAL):
+    raise CoconetError(code, f"{what} needs {needs}, not {x.dtype} of {tuple(x.shape)} with strides {tuple(x.stride())} on {x.device}")
+
+
+def _matrix(x, ld, types, what):
+    """Device address of a matrix whose rows start `ld` elements apart.  A torch tensor has to be one: the type, on the GPU, elements of
+    a row side by side, rows (over all its leading dimensions) that far apart, or everything end to end.  How many rows and columns
+    of it are used is the caller's word, as in the ABI: the call with one row takes 5.5 us, and this much of it 0.1 us a tensor."""
+    if x is None:
+        return None
+    try:
+        if x.dtype is types[0] and x.is_cuda and x.stride() == (ld, 1):
+            return x.data_ptr()
+    except AttributeError:
+        return addr(x)
+    if x.dtype not in types or not x.is_cuda:
+        _refuse(x, what, f"{types[0]} on the GPU")
+    if not x.is_contiguous():
+        size, stride = x.shape, x.stride()
+        flat = len(size) >= 2 and (stride[-1] == 1 or size[-1] == 1) and all(stride[i] == stride[i + 1] * size[i + 1] for i in range(len(size) - 2))
+        if not flat or x.numel() > size[-1] and (stride[-2] == 0 or ld % stride[-2]):
+            _refuse(x, what, f"the elements of a row side by side, rows {ld} apart")
+    return x.data_ptr()
+
+
+def _array(x, n, types, what):
+    """Device address of n elements that lie end to end, checked as a matrix is."""
+    if x is None:
+        return None
+    try:
+        if x.dtype in types and x.is_cuda and x.numel() >= n and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        return addr(x)
+    _refuse(x, what, f"{n} elements of {types[0]} on the GPU, end to end", CCN_ERANGE if x.numel() < n else CCN_EINVAL)
+
+
+def _order(x):
+    """The order in which the elements of a tensor that is not contiguous lie, as something to compare; False: with gaps or overlaps."""
+    at = 1
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride != at:
+            return False
+        at *= size
+    return tuple(x.shape), tuple(x.stride())
 
 
 class LinearPlan:
@@ -511,27 +577,41 @@ class LinearPlan:
 
     def __init__(self, max_m, max_n, max_k):
         h = C.c_void_p()
-        _check(load().ccn_linear_plan_create(max_m, max_n, max_k, C.byref(h)), "ccn_linear_plan_create")
+        L = load()
+        _check(L.ccn_linear_plan_create(max_m, max_n, max_k, C.byref(h)), "ccn_linear_plan_create")
         self.h = h
+        self._calls = {False: (L.ccn_linear_bf16, L.ccn_linear_backward_bf16, _dtypes("bf16")), True: (L.ccn_linear_f16, L.ccn_linear_backward_f16, _dtypes("f16"))}
 
     def forward(self, X, W, bias, resid, Y, M, N, K, act="none", pre=None, half=False, ldx=0, ldw=0, ldr=0, ldy=0, ldp=0,
                 stream=None):
         """Y = act(X.W + bias) + resid; pre receives X.W + bias.  bias, resid, pre: or None.  ld* 0: the rows lie end to end."""
-        L = load()
-        fn = L.ccn_linear_f16 if half else L.ccn_linear_bf16
-        rc = fn(self.h, addr(X), ldx or K, addr(W), ldw or N, addr(bias), addr(resid), ldr or N, addr(Y), ldy or N, addr(pre),
-                ldp or N, M, N, K, ACTS[act], stream)
+        fn, _, t = self._calls[bool(half)]
+        t0, f32 = t[0], _DTYPES["f32"]
+        ldx, ldw, ldr, ldy, ldp = ldx or K, ldw or N, ldr or N, ldy or N, ldp or N
+        try:   # as _matrix and _array do it, without the calls
+            ok = (X.dtype is t0 and W.dtype is t0 and Y.dtype is t0 and X.is_cuda and W.is_cuda and Y.is_cuda and
+                  X.stride() == (ldx, 1) and W.stride() == (ldw, 1) and Y.stride() == (ldy, 1) and
+                  (bias is None or bias.dtype is f32[0] and bias.is_cuda and bias.numel() >= N and bias.is_contiguous()))
+        except AttributeError:
+            ok = False
+        if ok:
+            x, w, y, b = X.data_ptr(), W.data_ptr(), Y.data_ptr(), None if bias is None else bias.data_ptr()
+        else:
+            x, w, y, b = _matrix(X, ldx, t, "X"), _matrix(W, ldw, t, "W"), _matrix(Y, ldy, t, "Y"), _array(bias, N, f32, "bias")
+        rc = fn(self.h, x, ldx, w, ldw, b, None if resid is None else _matrix(resid, ldr, t, "resid"), ldr, y, ldy,
+                None if pre is None else _matrix(pre, ldp, t, "pre"), ldp, M, N, K, ACTS[act], stream)
         if rc:
             _check(rc, "ccn_linear_f16" if half else "ccn_linear_bf16")
 
     def backward(self, dY, pre, X, W, dX, dW, db, M, N, K, act="none", half=False, dw_f32=False, accumulate=False, lddy=0, ldp=0,
                  ldx=0, ldw=0, lddx=0, lddw=0, stream=None):
         """The layer's gradients; any of dX, dW, db may be None.  dw_f32: dW is fp32; accumulate: dW and db are added to."""
-        L = load()
-        fn = L.ccn_linear_backward_f16 if half else L.ccn_linear_backward_bf16
-        rc = fn(self.h, addr(dY), lddy or N, addr(pre), ldp or N, addr(X), ldx or K, addr(W), ldw or N, addr(dX), lddx or K,
-                addr(dW), lddw or N, 0 if dw_f32 else (2 if half else 1), addr(db), 1 if accumulate else 0, M, N, K, ACTS[act],
-                stream)
+        _, fn, t = self._calls[bool(half)]
+        f32 = _DTYPES["f32"]
+        lddy, ldp, ldx, ldw, lddx, lddw = lddy or N, ldp or N, ldx or K, ldw or N, lddx or K, lddw or N
+        rc = fn(self.h, _matrix(dY, lddy, t, "dY"), lddy, None if act == "none" else _matrix(pre, ldp, t, "pre"), ldp, _matrix(X, ldx, t, "X"), ldx,
+                _matrix(W, ldw, t, "W"), ldw, _matrix(dX, lddx, t, "dX"), lddx, _matrix(dW, lddw, f32 if dw_f32 else t, "dW"), lddw,
+                0 if dw_f32 else (2 if half else 1), _array(db, N, f32, "db"), 1 if accumulate else 0, M, N, K, ACTS[act], stream)
         if rc:
             _check(rc, "ccn_linear_backward_f16" if half else "ccn_linear_backward_bf16")
 
@@ -565,22 +645,62 @@ class AdamWPlan:
         e, b = _sz(0), _sz(0)
         _check(load().ccn_adamw_plan_sizes(h, C.byref(e), C.byref(b)), "ccn_adamw_plan_sizes")
         self.elems, self.blocks = e.value, b.value
+        self._step, self._moment = load().ccn_adamw_scattered, _dtypes("f32" if bits == 32 else "e4m3")
 
     def tables(self, g, w, w16=None):
         """The host pointer tables of a step: g P lists of tensors, w and w16 (or None) one list each.  A program whose tensors
         stay where they are makes them once; they hold addresses only, the tensors have to be kept alive beside them."""
         n = len(self.counts)
         assert len(w) == n and all(len(gp) == n for gp in g) and (w16 is None or len(w16) == n)
-        return ((C.c_void_p * (len(g) * n))(*[addr(x) for gp in g for x in gp]), len(g), (C.c_void_p * n)(*[addr(x) for x in w]),
-                None if w16 is None else (C.c_void_p * n)(*[addr(x) for x in w16]))
+
+        seen, order = [False] * n, [None] * n   # of each tensor: whether one of its arrays was looked at, and how that one lies
+
+        def table(lists, what, *names):
+            """Addresses of tensors of one dtype; the table keeps which of `names` that may be (all, where it holds addresses only)."""
+            t, dtype, i = (C.c_void_p * (len(lists) * n))(), None, 0
+            for part in lists:
+                for b, (x, count) in enumerate(zip(part, self.counts)):
+                    if count and hasattr(x, "dtype"):
+                        if x.dtype is not dtype:
+                            if dtype is not None or not any(x.dtype in _dtypes(k) for k in names):
+                                _refuse(x, f"{what} {b}", str(dtype or " or ".join(names)))
+                            dtype = x.dtype
+                        if not x.is_cuda:
+                            _refuse(x, f"{what} {b}", "the GPU")
+                        if x.numel() < count:
+                            _refuse(x, f"{what} {b}", f"{count} elements", CCN_ERANGE)
+                        lies = None if x.is_contiguous() else _order(x)
+                        if lies is False or (seen[b] and lies != order[b]):   # elements are taken as they lie in memory
+                            _refuse(x, f"{what} {b}", "elements without gaps, in the order of the tensor's other arrays")
+                        seen[b], order[b] = True, lies
+                    t[i] = addr(x)
+                    i += 1
+            t.names = [k for k in names if dtype is None or dtype in _dtypes(k)]
+            return t
+
+        return table(g, "gradient", "f32", "bf16", "f16"), len(g), table([w], "weight", "f32"), None if w16 is None else table([w16], "weight copy", "bf16", "f16")
 
     def step(self, tables, m, v, lr, beta1, beta2, eps, wd, step, scales=None, g_type="f32", w16_type="bf16", inv_scale=1.0,
              grad_scale=None, overflow_flag=None, stream=None):
         """One step.  tables: from tables().  grad_scale: device fp32 scalar; overflow_flag: device uint32 / int32 scalar."""
         gt, ranks, wt, ht = tables
-        _check(load().ccn_adamw_scattered(self.h, gt, ranks, TYPES[g_type], wt, ht, TYPES[w16_type] if ht is not None else 0, addr(m), addr(v),
-                                          addr(scales), lr, beta1, beta2, eps, wd, step, inv_scale, addr(grad_scale),
-                                          addr(overflow_flag), stream), "ccn_adamw_scattered")
+        if g_type not in gt.names or (ht is not None and w16_type not in ht.names):
+            raise CoconetError(CCN_EINVAL, f"tables of {gt.names}, {ht.names if ht is not None else ''} taken as {g_type}, {w16_type}")
+        t, n, f32, u32 = self._moment, self.elems, _DTYPES["f32"], _DTYPES["u32"]
+        try:   # as _array does it, without the calls
+            ok = (m.dtype in t and v.dtype in t and m.is_cuda and v.is_cuda and m.numel() >= n and v.numel() >= n and m.is_contiguous() and v.is_contiguous() and
+                  (overflow_flag is None or overflow_flag.dtype in u32 and overflow_flag.is_cuda))
+        except AttributeError:
+            ok = False
+        if ok:
+            ma, va, fa = m.data_ptr(), v.data_ptr(), None if overflow_flag is None else overflow_flag.data_ptr()
+        else:
+            ma, va, fa = _array(m, n, t, "m"), _array(v, n, t, "v"), _array(overflow_flag, 1, u32, "overflow_flag")
+        rc = self._step(self.h, gt, ranks, TYPES[g_type], wt, ht, 0 if ht is None else TYPES[w16_type], ma, va,
+                        None if scales is None else _array(scales, 2 * self.blocks, f32, "scales"), lr, beta1, beta2, eps, wd, step, inv_scale,
+                        None if grad_scale is None else _array(grad_scale, 1, f32, "grad_scale"), fa, stream)
+        if rc:
+            _check(rc, "ccn_adamw_scattered")
 
     def close(self):
         if self.h:

@@ -581,3 +581,43 @@ def test_decay_beside_updates(ccn, bits, rate):
     u = lr * (m / (1 - b1 ** 3)) / ((v / (1 - b2 ** 3)).sqrt() + HYPER["eps"])
     d = c.w[0].double() - (w0 - rate * w0 - u)
     assert d.mean().abs() <= 6 * 2.0 ** -23 / math.sqrt(12 * n) + 64 * U * u.abs().mean() + 3 * U * rate * w0.mean(), d.mean().item()
+
+
+def test_tensors_that_are_not_what_they_are_taken_for(ccn):
+    """Types, orders and sizes of the Python call's tensors are refused; transposed tensors are taken where all of a tensor's arrays
+    are, element for element as they lie."""
+    c = Case(ccn, [300, 40], 1, "bf16", "bf16", 8)
+    c.new_gradients()
+    old = [x.clone() for x in c.w]
+
+    def refused(code, f, *a, **k):
+        with pytest.raises(ccn.CoconetError) as e:
+            f(*a, **k)
+        assert e.value.code == code
+
+    E, R = ccn.CCN_EINVAL, ccn.CCN_ERANGE
+    refused(E, c.plan.tables, [[x.float() for x in c.g[0][:1]] + c.g[0][1:]], c.w, c.w16)
+    refused(E, c.plan.tables, c.g, [x.bfloat16() for x in c.w], c.w16)
+    refused(E, c.plan.tables, [[x.cpu() for x in c.g[0]]], c.w, c.w16)
+    refused(R, c.plan.tables, c.g, [c.w[0], c.w[1][:39]], c.w16)
+    tables = c.plan.tables(c.g, c.w, c.w16)
+    h = (1e-3, 0.9, 0.98, 1e-8, 0.1, 1)
+    good = dict(scales=c.scales, g_type="bf16", w16_type="bf16")
+    refused(E, c.plan.step, tables, c.m, c.v, *h, **{**good, "g_type": "f32"})
+    refused(E, c.plan.step, tables, c.m, c.v, *h, **{**good, "w16_type": "f16"})
+    refused(E, c.plan.step, tables, c.m.float(), c.v, *h, **good)
+    refused(R, c.plan.step, tables, c.m, c.v[:-1], *h, **good)
+    refused(R, c.plan.step, tables, c.m, c.v, *h, **{**good, "scales": c.scales[1:]})
+    refused(E, c.plan.step, tables, c.m, c.v, *h, **good, grad_scale=torch.ones(1, device=DEV, dtype=torch.float64))
+    refused(E, c.plan.step, tables, c.m, c.v, *h, **good, overflow_flag=torch.zeros(1, device=DEV))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(old, c.w)) and not c.m.any()
+
+    plan, out = ccn.AdamWPlan([300]), []
+    g, w = torch.randn(20, 15, device=DEV, generator=c.gen), torch.randn(20, 15, device=DEV, generator=c.gen)
+    for turn in (lambda x: x, lambda x: x.t()):
+        m, v, x = torch.zeros(plan.elems, device=DEV), torch.zeros(plan.elems, device=DEV), w.clone()
+        plan.step(plan.tables([[turn(g)]], [turn(x)]), m, v, *h)
+        out.append(x)
+    assert torch.equal(*out) and not torch.equal(out[0], w)
+    refused(E, plan.tables, [[g.t()]], [w])

@@ -493,3 +493,43 @@ def test_gelu_far_left(ccn, M, half):
     s = M * (Phi + z * phi)
     within(db, s, M * (rel + (M + 2) * U24) * (Phi + z.abs() * phi), f"db {M}")
     plan.close()
+
+
+def test_tensors_that_are_not_what_they_are_taken_for(ccn):
+    """Types, devices and orders of the Python call's tensors: refused before anything is launched.  What lies as the call
+    reads it is taken, however it is shaped."""
+    M, N, K = 6, 16, 24
+    g = gen(1)
+    X, W, b = matrix(g, M, K, False), matrix(g, K, N, False), torch.randn(N, device=DEV, generator=g)
+    Y, dW, db = torch.full((M, N), 5.0, device=DEV, dtype=torch.bfloat16), torch.full((K, N), 5.0, device=DEV), torch.full((N,), 5.0, device=DEV)
+    dX = torch.full((M, K), 5.0, device=DEV, dtype=torch.bfloat16)
+    plan = ccn.LinearPlan(2 * M, N, K)
+    E, R = ccn.CCN_EINVAL, ccn.CCN_ERANGE
+
+    def refused(code, f, *a, **k):
+        with pytest.raises(ccn.CoconetError) as e:
+            f(*a, **k)
+        assert e.value.code == code
+
+    for X2, W2, b2, Y2 in ((X.float(), W, b, Y), (X.half(), W, b, Y), (X.cpu(), W, b, Y), (X, W.t().contiguous().t(), b, Y), (X, W, b.bfloat16(), Y),
+                           (X, W, b, Y.float()), (torch.cat([X, X], 1)[:, :K], W, b, Y)):
+        refused(E, plan.forward, X2, W2, b2, None, Y2, M, N, K)
+    refused(R, plan.forward, X, W, b[:8], None, Y, M, N, K)
+    refused(E, plan.forward, X, W, b, Y.half(), Y, M, N, K)
+    refused(E, plan.forward, X, W, b, None, Y, M, N, K, pre=Y.float())
+    refused(E, plan.forward, X, W, b, None, Y, M, N, K, half=True)
+    refused(E, plan.backward, Y, None, X, W, dX, dW, db, M, N, K)                       # an fp32 dW without dw_f32
+    refused(E, plan.backward, Y, None, X, W, dX, dW.bfloat16(), db, M, N, K, dw_f32=True)
+    refused(E, plan.backward, Y, X.float(), X, W, dX, dW, db, M, N, K, act="silu", dw_f32=True)
+    refused(E, plan.backward, Y, None, X, W, dX.t().contiguous().t(), dW, db, M, N, K, dw_f32=True)
+    torch.cuda.synchronize()
+    assert all(bool((x == 5).all()) for x in (Y, dW, db, dX))
+    want, got = (torch.empty(M, N, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    plan.forward(X, W, b, None, want, M, N, K)
+    every_other, wide = torch.zeros(2 * M, K, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 3, K + 8, device=DEV, dtype=torch.bfloat16)
+    every_other[::2], wide[..., :K] = X, X.view(2, 3, K)
+    for x, ldx in ((X.reshape(-1), 0), (X.view(2, 3, K), 0), (every_other, 2 * K), (every_other[::2], 2 * K), (wide[..., :K], K + 8), (X.view(torch.int16), 0), (X.data_ptr(), 0)):
+        got.zero_()
+        plan.forward(x, W, b, None, got, M, N, K, ldx=ldx)
+        assert torch.equal(got, want)
+    plan.close()
