@@ -107,8 +107,8 @@ __device__ __forceinline__ float wave_max(float f) {
   const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
   return __uint_as_float(ab > cd ? ab : cd);
 }
-// The correctly rounded square root from the 1-ulp one by a Newton step on the residual (its result before the last
-// rounding is within 2^-46 of the root).  Below 2^-96 the argument is scaled: the instruction flushes denormals.
+// The square root from the 1-ulp one by a Newton step on the residual: before its last rounding the result is within 2^-46 of the
+// root, so that it is the correctly rounded one but for roots that close to the middle of two floats.  Below 2^-96 the argument is scaled: the instruction flushes denormals.
 __device__ __forceinline__ float square_root(float x) {
   const bool small = x < 1.262177448353619e-29f;
   const float z = x * (small ? 18446744073709551616.0f : 1.0f);
@@ -117,8 +117,9 @@ __device__ __forceinline__ float square_root(float x) {
   return x > 0.0f ? r : 0.0f;
 }
 
-// 1/s, and x / s (inv: 1/s), correctly rounded by a Newton step each.  A code then depends on the values alone and not on
-// how a quotient next to a rounding border came about; the IEEE division sequence is three times as long.
+// 1/s, and x / s (inv: 1/s), by a Newton step each: correctly rounded but for quotients within 2^-46 of the middle of two floats.  A
+// code then depends on the values and hardly ever on how a quotient next to a rounding border came about; the IEEE division
+// sequence is three times as long.
 __device__ __forceinline__ float inverse(float s) {
   const float r = __builtin_amdgcn_rcpf(s);
   return fmaf(fmaf(-s, r, 1.0f), r, r);

@@ -297,10 +297,13 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f
 //   4 x 4   256 x 256, RK 32: 256 accumulators per lane, in the accumulation half of the register file; per 16 summed elements a
 //           wavefront reads eight fragments for sixteen matrix instructions
 //   4 x 2   256 x 128, RK 32: six fragments for eight
-//   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  What bounds it is LDS: a step of 64 summed elements writes 32 KiB
-//           and reads 64, 768 clocks at 128 bytes each beside 512 of matrix instructions.  An "along" request covers whole
-//           128-byte lines (RK 32, two workgroups per CU: half of every line fetched is wasted)
-// 8192 x 8192 x 4096 with bias, gelu_tanh and the kept pre-activation: 426 us, 1.29 PFLOP/s; dX and dW of it 412 and 390.
+//   2 x 2   128 x 128, RK 64: for outputs of few large tiles.  A step of 64 summed elements takes 0.40 us; its matrix instructions
+//           fill 512 clocks of it and its LDS reads 300 (counted over 777 x 1537 x 2049): neither bounds it, one wavefront per SIMD
+//           waits for the other's part of the stage.  An "along" request covers whole 128-byte lines (RK 32, two workgroups per
+//           CU: half of every line fetched is wasted)
+// 8192 x 8192 x 4096 with bias, gelu_tanh and the kept pre-activation: 426 to 457 us from card to card, 1.2-1.29 PFLOP/s; dX and dW of it
+// 412-465 and 390-424.  The clock falls to 1.55 GHz under these products; of its cycles the matrix units are busy in 75 %, the LDS
+// reads in 20 % (GRBM_GUI_ACTIVE, SQ_VALU_MFMA_BUSY_CYCLES, SQ_LDS_IDX_ACTIVE).
 constexpr size_t kRMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
 constexpr int kStages = 4;
 template <int FR, int FC> struct Ring {
@@ -796,8 +799,8 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const float* __rest
 
 // ---- operands whose rows are not made of aligned 16-byte pieces --------------------------------------------------------------
 // A copy with aligned rows, zeros behind each row's end up to the next row: the ring then runs on it.  It costs a launch and two
-// passes over the operand at the memory's rate, less than matrix instructions fed from unaligned loads through registers lose at
-// any size (129 x 129 x 129: 11.1 instead of 11.8 us, 777 x 1537 x 2049: 24 instead of 57, 2049 x 2049 x 2049: 54 instead of 90).
+// passes over the operand at the memory's rate, less than matrix instructions fed from unaligned loads through registers lose over
+// a long sum (777 x 1537 x 2049: 24 instead of 57 us, 2049 x 2049 x 2049: 54 instead of 90).  A short sum is not worth it: brief_product.
 struct PackJob {
   const uint16_t* src;
   uint16_t* dst;
@@ -838,8 +841,9 @@ __global__ __launch_bounds__(kBlock) void linear_pack_kernel(const PackJob a, co
 // go out and come back with the agent-scope bit (sc1: written through to, and read from, where the XCDs are coherent), complete
 // (vmcnt 0) before the wavefront counts itself in; splits are added in ascending order whoever does it, and the counter is back
 // at zero when the call ends.  With more rows a wavefront has too much to add, and the join kernel does it (64 x 1024 x 1024:
-// 10.1 us, 13.3 without; 32 x 4096 x 4096: 13.5, 14.5).  16 x 8192 x 4096 (67 MB of weights): 15.7 us, 4.3 TB/s; reading W alone
-// takes this grid 10.5, X 0.8, the split sums' way through memory 2.5.
+// 10.1 us, 13.3 without; 32 x 4096 x 4096: 13.5, 14.5).  16 x 8192 x 4096 (67 MB of weights): 14.9 us, 4.5 TB/s, where the weights
+// are still in the Infinity Cache from the call before, of which reading W alone takes this grid 10.5, X 0.8, the split sums' way
+// through memory 2.5; 18.7 where other layers' weights have been read since.
 constexpr int kFewRows = 64, kFewWaves = 4, kFewMaxSplits = 16, kFewCounter = 32;
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 template <bool ALONG> struct Few {
@@ -880,8 +884,15 @@ template <bool F16> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f3
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// STREAM: W is read past the caches, where it is too large to stay there until the next call (us, 256 MB of Infinity Cache:
-// 16 x 8192 x 8192, 134 MB, 26.7 instead of 29.5; but 16 x 8192 x 4096, 67 MB, 17.1 instead of 15.7).
+// STREAM: W is read past the caches.  That is faster where it is no longer there, and slower where it still is, from the last call of
+// the same layer (us, cached / past the caches, 256 MB of Infinity Cache):
+//   rows x sum x cols                   the same weights again    other weights in between
+//   16 x 8192 x 8192, 134 MB            24.2 / 26.1               28.2 / 26.8
+//   16 x 8192 x 6144, 101 MB            24.4 / 27.1               30.4 / 27.9
+//   16 x 8192 x 4096, 67 MB (64 rows)   15.5 / 15.8 (21.5 / 23.3) 18.7 / 16.6 (24.6 / 23.4)
+//   16 x 4096 x 4096, 34 MB (64 rows)    8.8 /  9.8 (15.7 / 18.1) 11.5 / 11.0 (17.0 / 18.4)
+// A call cannot know which it is.  kFewStream supposes that less than 96 MiB may still be there and that more is not.  A model that reads
+// more than the cache between two calls of a layer of 67 MB would gain 5 to 12 % from a lower bound; one that does not would lose 1 to 8.
 template <bool F16, int MT, bool ALONG, bool STREAM>
 __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const FewArgs a, const LinEpi ep) {
   typedef Few<ALONG> D;
@@ -1063,7 +1074,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void linear_few_kernel(const Few
 }
 
 // Up to 4 rows, forward: strips of 32 columns and no split of the sum over workgroups, whose joining costs as long as the reading of
-// a small W (1 x 1024 x 8192: 8.0 us).  A wavefront's step is 128 summed elements x 32 columns: lane (kr, c2) = (lane/4, lane%4)
+// a small W (1 x 1024 x 8192: 8.5 us).  A wavefront's step is 128 summed elements x 32 columns: lane (kr, c2) = (lane/4, lane%4)
 // loads rows 8kr .. 8kr+7 of columns 8*c2 .. and turns the 8 x 8 block over as above.  One v_mfma_f32_16x16x32 then has the four
 // column groups of four different eights of summed elements (h = kr%4) as its rows, and four rows of X with the same four eights
 // as its columns: of its 16 x 16 results the 4 x 4 blocks with equal h are sums, the others are dropped.  The wavefronts of a
@@ -1160,7 +1171,9 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_one_kernel(const FewArgs
 
 // ---- dz and the column sums ------------------------------------------------------------------------------------------------
 // dz = dY * act'(pre), rounded to the operands' type into the workspace (aligned rows, zeros up to a multiple of 8 columns), and
-// fp32 sums over a chunk of rows of the unrounded dz.  LANES lanes share a row's strip of 8*LANES columns, a workgroup of WAVES
+// fp32 sums over a chunk of rows of the unrounded dz.  The rounding is the matrix instructions': both their operands have the type of W
+// and X, and to carry dz in two parts would double both products.  It is the only rounding beside the output's own, and as large: dX
+// and dW of a bf16 layer are off by 2.35e-3 of their norm, 1.66e-3 with an unrounded dz.  LANES lanes share a row's strip of 8*LANES columns, a workgroup of WAVES
 // wavefronts works on WAVES * 64/LANES rows at a time, ROWS times that in flight.
 //   64, 4, 2     many rows (8192 x 4096, gelu_tanh: 45 us; 48 with four in flight): a strip of 512 columns, chunks of rows over the chip, linear_db_kernel adds the chunks up
 //   16, 16, 1    up to 64 rows, all at once: one chunk, its sums are db itself (`add`: added to it)
@@ -1468,7 +1481,10 @@ RingPlan choose_ring(int rows, int cols, int sum, size_t partial_floats, int cus
 }
 
 // Whether a product does without the ring: short sums (`brief`), where there are more tiles than CUs (four workgroups then share a
-// CU: 65 x 4096 x 4096, dW: 33 instead of 48 us for a whole backward pass), or where an operand would have to be copied first.
+// CU: 65 x 4096 x 4096, dW: 33 instead of 48 us for a whole backward pass), or where an operand would have to be copied first (us,
+// M x N x K, rows of odd length, through registers / with the copy: forward 129 x 129 x 129 9.8 / 10.3, 200 x 131 x 135 9.8 / 12.2, 777 x 2049 x
+// 190 10.9 / 12.3, 2000 x 1001 x 190 12.8 / 12.6; backward 129 x 129 x 129 12.4 / 14.2, 100 x 515 x 2049 17.5 / 18.2, 190 x 2001 x 2001 33.9 / 32.5.
+// Rows of fewer than 8 elements are fetched one by one: 100 x 5 x 190 13.0 / 9.8).
 constexpr int kBriefSum = 192;
 bool brief_product(const Operand& p, bool p_along, const Operand& q, bool q_along, int rows, int cols, int sum, int cus) {
   if (sum > kBriefSum) return false;
