@@ -1323,7 +1323,7 @@ struct ccn_linear_plan {
   int max_m = 0, max_n = 0, max_k = 0;
   uint16_t* dz = nullptr;
   uint16_t* px = nullptr;    // aligned copies of X and W
-  uint16_t* pw = nullptr;
+  uint16_t* pw = nullptr;    // (nullptr: up to kFewRows rows)
   float* sums = nullptr;
   float* partial = nullptr;
   size_t partial_floats = 0;
@@ -1768,13 +1768,17 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   p->max_m = max_M;
   p->max_n = max_N;
   p->max_k = max_K;
-  // A split product has at most two 128 x 128 tiles on every CU, over all its splits, and two steps of 64 in each split.
-  auto floats = [&](int rows, int cols, int sum) {
+  // A split product has at most two 128 x 128 tiles on every CU, over all its splits, and two steps of 64 in each split (a sum of up
+  // to three steps is not split).
+  auto floats = [&](int rows, int cols, int sum) -> size_t {
+    if (sum <= 3 * 64) return 0;
     const size_t tiles = (size_t)((rows + 127) / 128) * (size_t)((cols + 127) / 128);
     const size_t most = tiles * (size_t)(sum / 128 + 1), cap = 2 * (size_t)di->cu_count;
     return (most < cap ? most : cap) * (size_t)(128 * 128);
   };
-  const size_t need[3] = {floats(max_M, max_N, max_K), floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
+  // (with few rows the ring works on dW alone, and W is read as it lies: a plan for them has neither copy nor partial sums of more)
+  const bool few_only = max_M <= kFewRows;
+  const size_t need[3] = {few_only ? 0 : floats(max_M, max_N, max_K), few_only ? 0 : floats(max_M, max_K, max_N), floats(max_K, max_N, max_M)};
   for (const size_t f : need) p->partial_floats = f > p->partial_floats ? f : p->partial_floats;
   const size_t few_cols = ((size_t)(max_N > max_K ? max_N : max_K) + 127) & ~(size_t)127;
   // A split sum of few rows has fewer than two workgroups for every CU, over all its splits, of up to 128 outputs each.
@@ -1784,7 +1788,7 @@ int ccn_linear_plan_create(int max_M, int max_N, int max_K, ccn_linear_plan** ou
   const size_t counters = few_cols / 64 * kFewWaves * kFewCounter;
   hipError_t e = hipMalloc((void**)&p->dz, (size_t)max_M * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->px, (size_t)max_M * pitch((size_t)max_K) * sizeof(uint16_t));
-  if (e == hipSuccess) e = hipMalloc((void**)&p->pw, pitch((size_t)max_K) * pitch((size_t)max_N) * sizeof(uint16_t));
+  if (e == hipSuccess && !few_only) e = hipMalloc((void**)&p->pw, pitch((size_t)max_K) * pitch((size_t)max_N) * sizeof(uint16_t));
   if (e == hipSuccess) e = hipMalloc((void**)&p->sums, (size_t)kMaxChunks * (size_t)max_N * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->partial, p->partial_floats * sizeof(float));
   if (e == hipSuccess) e = hipMalloc((void**)&p->counters, counters * sizeof(uint32_t));

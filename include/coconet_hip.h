@@ -329,11 +329,11 @@ int  ccn_matmul_f16(const uint16_t* X, const uint16_t* W, uint16_t* C, int M, in
  *      Y may be resid itself (same address and ld); otherwise outputs must not overlap inputs or each other.
  *      Rows and columns outside the matrices (the padding of a row) are neither read for the result nor written.
  *
- *      A plan owns the workspace for calls of up to max_M x max_N x max_K: dz and aligned copies of X and W (2 bytes for each
- *      of their elements, rows rounded up to 64) up to 32 MiB of partial sums and 1 KiB for each column
- *      of dz; one plan serves any number of layers of up to that size.  Calls on one plan must be ordered (one stream, or
- *      events), also calls replayed from recordings.  Every call on a plan can be recorded.  CCN_ERANGE: a size beyond the plan's, N or K of a plan beyond 2^21
- *      or M beyond 2^30, ld beyond 2^22. ---- */
+ *      A plan owns the workspace for calls of up to max_M x max_N x max_K: dz and aligned copies of X and, from 65 rows on, of W (2
+ *      bytes for each of their elements, rows rounded up to 64), up to 32 MiB of partial sums and 1 KiB for each column of dz; one
+ *      plan serves any number of layers of up to that size.  Calls on one plan must be ordered (one stream, or events), also calls
+ *      replayed from recordings.  Every call on a plan can be recorded.  CCN_ERANGE: a size beyond the plan's, N or K of a plan
+ *      beyond 2^21 or M beyond 2^30, ld beyond 2^22. ---- */
 #define CCN_ACT_NONE      0
 #define CCN_ACT_RELU      1
 #define CCN_ACT_GELU      2
@@ -378,8 +378,9 @@ int  ccn_linear_backward_f16(ccn_linear_plan* plan, const uint16_t* dY, size_t l
  *      one whose new v is not finite although its gradient is, which does not set the flag.
  *      eps > 0 keeps the quotient defined where v is zero.  CCN_ERANGE: more than 2^31 blocks.
  *      The device's pointer table is refreshed on the call's stream when pointers change; such a call cannot be recorded, and
- *      once a call on the plan has been recorded its pointers stay (CCN_EINVAL for others).  `step` is evaluated on the host,
- *      as for Adam.  Calls on one plan must be ordered. ---- */
+ *      once a call on the plan has been recorded its pointers stay (CCN_EINVAL for others).  `step`, lr and the other scalars are
+ *      evaluated on the host, as for Adam: a replayed call applies those that it was recorded with.  Calls on one plan must be
+ *      ordered. ---- */
 typedef struct ccn_adamw_plan ccn_adamw_plan;
 int  ccn_adamw_plan_create(const size_t* counts, const float* decay, int nbuff, int bits, ccn_adamw_plan** plan);
 int  ccn_adamw_plan_destroy(ccn_adamw_plan* plan);

@@ -533,3 +533,17 @@ def test_tensors_that_are_not_what_they_are_taken_for(ccn):
         plan.forward(x, W, b, None, got, M, N, K, ldx=ldx)
         assert torch.equal(got, want)
     plan.close()
+
+
+def test_a_plan_for_few_rows_is_small(ccn):
+    """Up to 64 rows the weights are read as they lie and a sum over the rows is never split: such a plan holds neither a copy of W
+    (64 MiB here) nor that product's partial sums (32 MiB), and serves both directions."""
+    M, N, K = 16, 4096, 8192
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    plan = ccn.LinearPlan(M, N, K)
+    taken = free - torch.cuda.mem_get_info()[0]
+    assert taken < 24 << 20, taken
+    forward_case(ccn, M, N, K, "gelu", False, pad=3, shift=1, plan=plan)
+    plan.close()
+    backward_case(ccn, 64, 1000, 1504, "silu", False, pad=3, shift=1)
