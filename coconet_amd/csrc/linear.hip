@@ -301,9 +301,9 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f
 //           fill 512 clocks of it and its LDS reads 300 (counted over 777 x 1537 x 2049): neither bounds it, one wavefront per SIMD
 //           waits for the other's part of the stage.  An "along" request covers whole 128-byte lines (RK 32, two workgroups per
 //           CU: half of every line fetched is wasted)
-// 8192 x 8192 x 4096 with bias, gelu_tanh and the kept pre-activation: 426 to 457 us from card to card, 1.2-1.29 PFLOP/s; dX and dW of it
-// 412-465 and 390-424.  The clock falls to 1.55 GHz under these products; of its cycles the matrix units are busy in 75 %, the LDS
-// reads in 20 % (GRBM_GUI_ACTIVE, SQ_VALU_MFMA_BUSY_CYCLES, SQ_LDS_IDX_ACTIVE).
+// 8192 x 8192 x 4096 with bias, gelu_tanh and the kept pre-activation: 416 to 457 us from card to card, 1.2-1.32 PFLOP/s; dX and dW of it
+// 412-465 and 390-424.  The clock falls to 1.55-1.7 GHz under these products; of its cycles the matrix units are busy in 75 % (dX 69, dW
+// 78), the LDS reads in 20 % (GRBM_GUI_ACTIVE, SQ_VALU_MFMA_BUSY_CYCLES, SQ_LDS_IDX_ACTIVE).
 constexpr size_t kRMaxLd = (size_t)1 << 21;  // 256 rows of it stay inside the 2 GiB that a buffer descriptor spans
 constexpr int kStages = 4;
 template <int FR, int FC> struct Ring {
