@@ -529,6 +529,11 @@ def _refuse(x, what, needs, code=CCN_EINVAL):
     raise CoconetError(code, f"{what} needs {needs}, not {x.dtype} of {tuple(x.shape)} with strides {tuple(x.stride())} on {x.device}")
 
 
+def _reachable(x):
+    """Whether the GPU can read a tensor: its own memory, or pinned host memory."""
+    return x.is_cuda or x.is_pinned()
+
+
 def _matrix(x, ld, types, what):
     """Device address of a matrix whose rows start `ld` elements apart.  A torch tensor has to be one: the type, on the GPU, elements of
     a row side by side, rows (over all its leading dimensions) that far apart, or everything end to end.  How many rows and columns
@@ -540,7 +545,7 @@ def _matrix(x, ld, types, what):
             return x.data_ptr()
     except AttributeError:
         return addr(x)
-    if x.dtype not in types or not x.is_cuda:
+    if x.dtype not in types or not _reachable(x):
         _refuse(x, what, f"{types[0]} on the GPU")
     if not x.is_contiguous():
         size, stride = x.shape, x.stride()
@@ -555,7 +560,7 @@ def _array(x, n, types, what):
     if x is None:
         return None
     try:
-        if x.dtype in types and x.is_cuda and x.numel() >= n and x.is_contiguous():
+        if x.dtype in types and x.numel() >= n and x.is_contiguous() and _reachable(x):
             return x.data_ptr()
     except AttributeError:
         return addr(x)
@@ -665,7 +670,7 @@ class AdamWPlan:
                             if dtype is not None or not any(x.dtype in _dtypes(k) for k in names):
                                 _refuse(x, f"{what} {b}", str(dtype or " or ".join(names)))
                             dtype = x.dtype
-                        if not x.is_cuda:
+                        if not _reachable(x):
                             _refuse(x, f"{what} {b}", "the GPU")
                         if x.numel() < count:
                             _refuse(x, f"{what} {b}", f"{count} elements", CCN_ERANGE)
@@ -684,17 +689,18 @@ class AdamWPlan:
              grad_scale=None, overflow_flag=None, stream=None):
         """One step.  tables: from tables().  grad_scale: device fp32 scalar; overflow_flag: device uint32 / int32 scalar."""
         gt, ranks, wt, ht = tables
-        if g_type not in gt.names or (ht is not None and w16_type not in ht.names):
-            raise CoconetError(CCN_EINVAL, f"tables of {gt.names}, {ht.names if ht is not None else ''} taken as {g_type}, {w16_type}")
         t, n, f32, u32 = self._moment, self.elems, _DTYPES["f32"], _DTYPES["u32"]
         try:   # as _array does it, without the calls
-            ok = (m.dtype in t and v.dtype in t and m.is_cuda and v.is_cuda and m.numel() >= n and v.numel() >= n and m.is_contiguous() and v.is_contiguous() and
+            ok = (g_type in gt.names and (ht is None or w16_type in ht.names) and m.dtype in t and v.dtype in t and m.is_cuda and v.is_cuda and m.numel() >= n and v.numel() >= n and m.is_contiguous() and v.is_contiguous() and
                   (overflow_flag is None or overflow_flag.dtype in u32 and overflow_flag.is_cuda))
         except AttributeError:
             ok = False
         if ok:
             ma, va, fa = m.data_ptr(), v.data_ptr(), None if overflow_flag is None else overflow_flag.data_ptr()
         else:
+            for table, name, what in ((gt, g_type, "gradients"), (ht, w16_type, "weight copies")):   # (a table of the caller's own says nothing)
+                if name not in getattr(table, "names", TYPES):
+                    raise CoconetError(CCN_EINVAL, f"{what} of {' or '.join(table.names)} taken as {name}")
             ma, va, fa = _array(m, n, t, "m"), _array(v, n, t, "v"), _array(overflow_flag, 1, u32, "overflow_flag")
         rc = self._step(self.h, gt, ranks, TYPES[g_type], wt, ht, 0 if ht is None else TYPES[w16_type], ma, va,
                         None if scales is None else _array(scales, 2 * self.blocks, f32, "scales"), lr, beta1, beta2, eps, wd, step, inv_scale,

@@ -57,6 +57,11 @@ class OnGpu(torch.Tensor):
     is_cuda = True
 
 
+class Pinned(torch.Tensor):
+    def is_pinned(self):
+        return True
+
+
 def gpu(*shape, dtype=torch.bfloat16):
     return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
 
@@ -84,6 +89,8 @@ def test_matrices_that_are_refused(x, ld):
 def test_arrays():
     for x, n in ((gpu(8, dtype=torch.float32), 8), (gpu(8, dtype=torch.float32), 3), (gpu(2, 4, dtype=torch.float32), 8)):
         assert capi._array(x, n, F32, "b") == x.data_ptr()
+    pinned = torch.zeros(4, 8).as_subclass(Pinned)      # host memory that the GPU reads
+    assert capi._array(pinned, 32, F32, "b") == pinned.data_ptr() and capi._matrix(pinned, 8, F32, "b") == pinned.data_ptr()
     assert capi._array(None, 8, F32, "b") is None and capi._array(4096, 8, F32, "b") == 4096
     assert capi._matrix(None, 8, BF, "b") is None and capi._matrix(4096, 8, BF, "b") == 4096
     for x, code in ((gpu(8), capi.CCN_EINVAL), (torch.zeros(8), capi.CCN_EINVAL), (gpu(16, dtype=torch.float32)[::2], capi.CCN_EINVAL),

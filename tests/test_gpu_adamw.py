@@ -4,6 +4,7 @@ Tolerances count fp32 roundings (2^-24 each): a gradient that is the sum of P bu
 the sum of magnitudes; m and v by a few more; the update by those of m plus a dozen in the square root and division.  An
 8-bit moment has to be within half a step (2^-4 relative, 2^-10 among the subnormals, in units of the scale) of the exact
 value, plus what fp32 moved it by."""
+import ctypes
 import math
 
 import pytest
@@ -621,3 +622,6 @@ def test_tensors_that_are_not_what_they_are_taken_for(ccn):
         out.append(x)
     assert torch.equal(*out) and not torch.equal(out[0], w)
     refused(E, plan.tables, [[g.t()]], [w])
+    m, v, x = torch.zeros(plan.elems, device=DEV), torch.zeros(plan.elems, device=DEV), w.clone()
+    plan.step(((ctypes.c_void_p * 1)(g.data_ptr()), 1, (ctypes.c_void_p * 1)(x.data_ptr()), None), m, v, *h)      # a caller's own tables
+    assert torch.equal(x, out[0])
